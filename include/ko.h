@@ -159,6 +159,98 @@ int ko_layernorm_16(const void *in, void *out, float *mean, float *rstd, const v
                     const void *beta, int64_t rows, int64_t cols, float eps, int unbiased, int dtype,
                     int policy, ko_stream_t stream);
 
+/* ---- gradients of the row operators ------------------------------------------------------------------------
+ * The reference has forward operators only; these are what training through them needs.  Conventions:
+ * Workspace: calls that can use device memory for partial results take it from the caller - `workspace` points to at
+ * least the number of bytes that the operator's *_workspace_bytes function returns for the call's sizes (a function of
+ * the sizes alone; 0: none is needed), 16-byte aligned; its contents need no preparation and mean nothing after the
+ * call.  NULL is always accepted: the operator then takes a slower path without one.  A workspace smaller than
+ * needed is refused.  Calls that may overlap in time (two streams, two captured graphs) need workspaces of their own;
+ * nothing is allocated, so any call may be captured, the first one included.
+ * Results are the same bits from call to call: nothing depends on timing. */
+
+/* Gradient of the row softmax: y is ko_softmax_*'s output, dy the gradient with respect to it,
+ *      dx = y (dy - sum_k y_k dy_k).
+ * Same shapes, types and mask as the forward call.  dx may be y or dy.  Columns j >= valid_len[seq] were constants of
+ * the forward pass: their dx is 0; their y and dy count in the sum where their y is not 0 (only in rows whose valid
+ * inputs all lie below about -9900) and are not read otherwise.  A row with valid_len 0 gets zeros. */
+size_t ko_softmax_backward_workspace_bytes(int64_t rows, int64_t cols);
+int ko_softmax_backward_f32(const float *y, const float *dy, float *dx, int64_t rows, int64_t cols, const int32_t *valid_len,
+                            int64_t rows_per_seq, void *workspace, size_t workspace_bytes, ko_stream_t stream);
+int ko_softmax_backward_16(const void *y, const void *dy, void *dx, int64_t rows, int64_t cols, const int32_t *valid_len,
+                           int64_t rows_per_seq, int dtype, void *workspace, size_t workspace_bytes, ko_stream_t stream);
+
+/* Gradient of LayerNorm: in, mean, rstd, gamma and unbiased as in the forward call (mean and rstd are its outputs).  With
+ * xh = (in - mean) rstd, g = dy gamma and D = cols or cols - 1:
+ *      dx = rstd (g - sum(g) / cols - xh sum(g xh) / D) + dres,   dgamma = sum_rows dy xh,   dbeta = sum_rows dy.
+ * gamma NULL: 1.  dres (NULL: 0): the gradient that reaches `in` beside the norm, a residual branch's.  dgamma, dbeta:
+ * fp32 in every entry, each NULL if not wanted; rows == 0 sets them to 0.  dx may be dy, in or dres.
+ * Any cols; multiples of 4 (16-bit: 8) on 16-byte aligned tensors are the fast case, others are walked element by
+ * element.  Rows longer than 16384 columns (8192 element by element) are read twice and dgamma / dbeta
+ * take another pass. */
+size_t ko_layernorm_backward_workspace_bytes(int64_t rows, int64_t cols);
+int ko_layernorm_backward_f32(const float *dy, const float *in, const float *mean, const float *rstd, const float *gamma,
+                              const float *dres, float *dx, float *dgamma, float *dbeta, int64_t rows, int64_t cols,
+                              int unbiased, void *workspace, size_t workspace_bytes, ko_stream_t stream);
+int ko_layernorm_backward_16(const void *dy, const void *in, const float *mean, const float *rstd, const void *gamma,
+                             const void *dres, void *dx, float *dgamma, float *dbeta, int64_t rows, int64_t cols, int unbiased,
+                             int dtype, void *workspace, size_t workspace_bytes, ko_stream_t stream);
+
+/* ---- losses over rows of logits --------------------------------------------------------------------------------
+ * logits: [rows] rows of cols elements, ld >= cols elements from one row to the next (what lies between is never read
+ * or, in dlogits with its ldd, written).  Any cols, ld and element-aligned address run on 16-byte vectors; a
+ * dlogits whose rows lie differently in their 16-byte vectors than the logits' rows is walked element by element.
+ * labels: device int32[rows].  A negative label marks a row that takes no part (a prompt's, padding): its logits are
+ * never read, its outputs and its gradient are 0.  A label >= cols reads nothing out of place and makes the row's
+ * outputs and its gradient NaN.  scale multiplies the logits (1 / temperature), from 1e-30 to 1e30.
+ * Special values: a NaN or +inf among a row's logits makes its outputs NaN; -inf elements have probability 0.
+ * One workspace size serves all of them (see above). */
+size_t ko_token_logprob_workspace_bytes(int64_t rows, int64_t cols);
+
+/* logp[r] = log softmax(scale logits[r])[labels[r]].  row_stats (NULL if not wanted): [rows][2], the row's maximum logit
+ * and log sum_j exp(scale (logits_j - maximum)); the gradient call needs them. */
+int ko_token_logprob_f32(const float *logits, int64_t ld, const int32_t *labels, float scale, float *logp, float *row_stats,
+                         int64_t rows, int64_t cols, void *workspace, size_t workspace_bytes, ko_stream_t stream);
+int ko_token_logprob_16(const void *logits, int64_t ld, const int32_t *labels, float scale, float *logp, float *row_stats,
+                        int64_t rows, int64_t cols, int dtype, void *workspace, size_t workspace_bytes, ko_stream_t stream);
+/* dlogits = dlogp scale (onehot(label) - softmax(scale logits)).  dlogits may be logits (with ldd = ld).  A row whose dlogp
+ * is 0 gets zeros, its logits unread. */
+int ko_token_logprob_backward_f32(const float *logits, int64_t ld, const int32_t *labels, float scale, const float *row_stats,
+                                  const float *dlogp, float *dlogits, int64_t ldd, int64_t rows, int64_t cols,
+                                  ko_stream_t stream);
+int ko_token_logprob_backward_16(const void *logits, int64_t ld, const int32_t *labels, float scale, const float *row_stats,
+                                 const float *dlogp, void *dlogits, int64_t ldd, int64_t rows, int64_t cols, int dtype,
+                                 ko_stream_t stream);
+
+/* Clipped policy loss with a KL term, and its gradient with respect to the logits, in one call.  Per row with a label and a
+ * weight that is not 0, with logp as above:
+ *      ratio = exp(logp - old_logp),  s = min(ratio A, clip(ratio, 1 - clip_low, 1 + clip_high) A),  A = advantage[r],
+ *      kl = exp(d) - 1 - d,  d = ref_logp - logp,  loss = weight (-s + kl_coef kl),
+ * loss_sum = sum_r loss[r] (NULL if not wanted), dlogits = d loss_sum / d logits (NULL if not wanted; may be logits with
+ * ldd = ld).  At a border of the clip range the gradient is the unclipped side's.  old_logp NULL: ratio 1, the policy that sampled is the one that trains.  ref_logp NULL:
+ * no KL term.  weight NULL: 1; a row whose weight is 0 is treated as one without a label.  logp, kl (unweighted): [rows],
+ * NULL if not wanted; loss: [rows].  clip_low in [0, 1], clip_high >= 0. */
+int ko_policy_loss_f32(const float *logits, int64_t ld, const int32_t *labels, const float *old_logp, const float *ref_logp,
+                       const float *advantage, const float *weight, float scale, float clip_low, float clip_high, float kl_coef,
+                       float *logp, float *kl, float *loss, float *loss_sum, float *dlogits, int64_t ldd, int64_t rows,
+                       int64_t cols, void *workspace, size_t workspace_bytes, ko_stream_t stream);
+int ko_policy_loss_16(const void *logits, int64_t ld, const int32_t *labels, const float *old_logp, const float *ref_logp,
+                      const float *advantage, const float *weight, float scale, float clip_low, float clip_high, float kl_coef,
+                      float *logp, float *kl, float *loss, float *loss_sum, void *dlogits, int64_t ldd, int64_t rows, int64_t cols,
+                      int dtype, void *workspace, size_t workspace_bytes, ko_stream_t stream);
+
+/* Preference loss on pairs of sequences of tokens whose log-probabilities stand one after the other in logp and ref_logp
+ * [tokens].  Sequence i is the tokens [offsets[i], offsets[i + 1]) (device int32[2 pairs + 1], ascending; what leads
+ * outside the tokens or backwards is taken as an empty stretch); 2p is pair p's chosen sequence, 2p + 1 its rejected one.
+ *      reward_i = beta sum (logp - ref_logp),  h = reward_chosen - reward_rejected,
+ *      pair_loss = -(1 - label_smoothing) log sigmoid(h) - label_smoothing log sigmoid(-h),
+ * loss_sum = pair_weight sum pair_loss, dlogp = d loss_sum / d logp.  labels (NULL: every token counts): tokens with a
+ * negative label count for nothing, whatever logp and ref_logp hold there, and get dlogp 0.  rewards [2 pairs], dlogp,
+ * loss_sum: NULL if not wanted.  dlogp of tokens that belong to no sequence is left as it was. */
+int ko_preference_loss_f32(const float *logp, const float *ref_logp, const int32_t *labels, const int32_t *offsets, int64_t pairs,
+                           int64_t tokens, float beta, float label_smoothing, float pair_weight, float *pair_loss,
+                           float *rewards, float *dlogp, float *loss_sum, ko_stream_t stream);
+
 /* ---- SIMT-path SGEMM: replaces
  *      gemm<GemmKernelSimt<...>><<<grid, K::thread_per_block, K::smem_total_size_in_bytes, stream>>>
  *          (shape::GemmCoord problem_size, ElementA *A, ElementB *B, ElementC *C, ElementC *D)

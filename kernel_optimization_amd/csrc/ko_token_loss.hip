@@ -1,0 +1,1029 @@
+// Losses over rows of logits for gfx950: log-probabilities of labels and their gradient, the clipped policy loss with
+// a KL term from the logits to their gradient, and the preference loss on paired sequences.  fp32 / binary16 / bfloat16
+// logits, fp32 arithmetic; differences of log-probabilities are taken in 64 bits.
+//
+// Per row with label l and z = scale x:  m = max x, S = sum_{j != l} exp(scale (x_j - m)), e = exp(scale (x_l - m)),
+//   logp = log(e / (S + e)) = -log1p(S / e).
+// The label's own column stays out of S: for a likely label (logp near 0) the others' sum is what matters, and in
+// 1 + S it would be rounded away.  Gradient of c * logp:  dx_j = -c scale exp(scale (x_j - m)) / (S + e) for j != l, and
+// c scale S / (S + e) for the label.
+//
+// Rows.  A row of logits starts anywhere (ld elements after the last one): its columns are a head of up to E - 1
+// elements up to the first 16-byte boundary, whole 16-byte vectors, and a tail.  Head and tail elements are taken one by
+// one by the first threads; the vectors carry the row.  So a vocabulary of 50257 contiguous columns runs on vectors, too.
+//
+// Bound: memory.  The sums are one pass with a running maximum; the policy loss keeps the whole row in a workgroup's
+// registers between the sum and the gradient, so that the logits are read once and the gradient written once.
+#include "ko_internal.h"
+
+#include "row_reduce.h"
+
+#include <cfloat>
+#include <initializer_list>
+
+namespace ko {
+namespace {
+
+constexpr float kLog2e = 0x1.715476p+0f;
+
+// ---- a row's columns
+template <int IO>
+struct RowSpan {
+    int head;     // single elements before the first vector
+    int nvec;     // vectors, from column `head` on
+    int singles;  // single elements in all: the head, and what is left after the last vector
+};
+template <int IO>
+__device__ __forceinline__ RowSpan<IO> span_of(const typename Io<IO>::elem *row, int cols) {
+    constexpr int E = Io<IO>::E;
+    RowSpan<IO> s;
+    if constexpr (E == 1) {
+        s.head = 0;
+        s.nvec = cols;
+        s.singles = 0;
+    } else {
+        const int past = static_cast<int>((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(typename Io<IO>::elem));
+        s.head = (E - past) % E;
+        if (s.head > cols) s.head = cols;
+        s.nvec = (cols - s.head) / E;
+        s.singles = cols - s.nvec * E;
+    }
+    return s;
+}
+// column of the i-th single element
+template <int IO>
+__device__ __forceinline__ int single_column(const RowSpan<IO> &s, int i) {
+    return i < s.head ? i : s.nvec * Io<IO>::E + i;
+}
+
+// ---- running (maximum, sum of exp(scale (x - maximum))); c = scale log2(e)
+struct Pair {
+    float m, s;
+};
+__device__ __forceinline__ float exp_scaled(float d, float c) { return __builtin_amdgcn_exp2f(d * c); }
+// An empty pair is (-FLT_MAX, 0).
+
+// Adds N values (absent ones: -inf) at once: the sum is rescaled at most once for all of them.
+template <int N>
+__device__ __forceinline__ void add_values(Pair &p, const float (&v)[N], float c) {
+    float m = v[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) m = fmaxf(m, v[i]);
+    if (m > p.m) {
+        p.s *= exp_scaled(p.m - m, c);
+        p.m = m;
+    }
+    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < N; ++i) s[i % 4] += exp_scaled(v[i] - p.m, c);
+    p.s += (s[0] + s[1]) + (s[2] + s[3]);
+}
+
+// The pairs of a workgroup's threads, the same bits in every thread.  One barrier; `slot` as in block_sum.
+template <int WAVES>
+__device__ __forceinline__ Pair block_pair(Pair p, Pair *slot, float c) {
+    const float m = wave::allreduce<64, wave::Max>(p.m);
+    Pair r{m, wave::allreduce<64, wave::Sum>(p.s * exp_scaled(p.m - m, c))};
+    if constexpr (WAVES > 1) {
+        if ((threadIdx.x & 63) == 0) slot[threadIdx.x >> 6] = r;
+        __syncthreads();
+        float top = slot[0].m;
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) top = fmaxf(top, slot[w].m);
+        float s = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) s += slot[w].s * exp_scaled(slot[w].m - top, c);
+        r = Pair{top, s};
+    }
+    return r;
+}
+
+// A thread's share of the pair over the vectors [lo, hi) and, if `with_singles`, the single elements of a row, without
+// the label's column.
+template <int IO, int THREADS>
+__device__ __forceinline__ Pair thread_pair(const typename Io<IO>::elem *row, const RowSpan<IO> &span, int lo, int hi,
+                                            bool with_singles, int label, float c) {
+    constexpr int E = Io<IO>::E;
+    constexpr int UNROLL = E == 8 ? 4 : 8;
+    Pair p{-FLT_MAX, 0.0f};
+    const typename Io<IO>::elem *vecs = row + span.head;
+    const int in_vecs = label - span.head;                // the label's place among the vectors' elements
+    const int label_vec = in_vecs >= 0 ? in_vecs / E : -1;
+    for (int j0 = lo + static_cast<int>(threadIdx.x); j0 < hi; j0 += THREADS * UNROLL) {
+        typename Io<IO>::raw r[UNROLL];
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            const int j = j0 + u * THREADS;
+            r[u] = typename Io<IO>::raw{};
+            if (j < hi) r[u] = Io<IO>::template load_raw<true>(vecs + static_cast<int64_t>(E) * j);
+        }
+        float v[UNROLL * E];
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            const int j = j0 + u * THREADS;
+            float x[E];
+            Io<IO>::unpack(r[u], x);
+            if (j >= hi || j == label_vec) {
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    if (j >= hi || E * j + e == in_vecs) x[e] = -INFINITY;
+            }
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[u * E + e] = x[e];
+        }
+        add_values(p, v, c);
+    }
+    if (with_singles && static_cast<int>(threadIdx.x) < span.singles) {
+        const int column = single_column(span, threadIdx.x);
+        const float v[1] = {column == label ? -INFINITY : Io<IO>::scalar(row + column)};
+        add_values(p, v, c);
+    }
+    return p;
+}
+
+// ---- a row's scalars
+// Logarithms here are of the size of 10 and get subtracted from each other: in fp32 they would carry an error of 5e-7,
+// ten times that of the sums.  So they are 64-bit numbers, put together from fp32 functions of arguments whose result is
+// small (64-bit functions would take as long as 1.5 us per row and, their constants kept in registers, a hundred
+// registers of kernels that need them for the row).
+struct RowScore {
+    double logp;     // log probability of the label
+    double logsum;   // log sum_j exp(scale (x_j - top)), the label included
+    float top;       // maximum of the row
+    float inv_total; // 1 / (S + e)
+    float rest;      // S / (S + e): what the label's probability leaves
+};
+// log(t) of a positive t, within 3e-8 absolute
+__device__ __forceinline__ double log_in_parts(float t) {
+    if (!(t < INFINITY)) return t;
+    int k;
+    float f = frexpf(t, &k);
+    if (f < 0.70710678f) {
+        f *= 2.0f;
+        --k;
+    }
+    return __builtin_fma(static_cast<double>(k), 0.69314718055994531, static_cast<double>(logf(f)));
+}
+// From the pair of the other columns and the label's logit.
+__device__ __forceinline__ RowScore score_row(Pair p, float at_label, float scale, float c) {
+    RowScore r;
+    r.top = fmaxf(p.m, at_label);
+    const float s = p.s * exp_scaled(p.m - r.top, c);
+    const double z = (static_cast<double>(at_label) - static_cast<double>(r.top)) * static_cast<double>(scale);
+    const float e = expf(static_cast<float>(z));
+    const float total = s + e;
+    if (s <= e) {  // a likely label: relative to a logarithm close to 0
+        r.logp = -log1pf(s / e);
+        r.logsum = z - r.logp;
+    } else {
+        r.logsum = log_in_parts(total);
+        r.logp = z - r.logsum;
+    }
+    r.inv_total = 1.0f / total;
+    r.rest = s / total;
+    return r;
+}
+__device__ __forceinline__ RowScore nan_score() {
+    const float nan = __builtin_nanf("");
+    return RowScore{nan, nan, nan, nan, nan};
+}
+
+// The values of one vector, the first of them element `first` of the row's vectors, become their gradient.
+template <int E, class LabelGrad>
+__device__ __forceinline__ void gradient_of(float (&x)[E], int first, bool live, int in_vecs, bool holds_label, float top,
+                                            float a, LabelGrad label_grad, float c) {
+    float at_label = 0.0f;
+    if (holds_label) {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (first + e == in_vecs) at_label = x[e];
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] = live ? a * exp_scaled(x[e] - top, c) : 0.0f;
+    if (live && holds_label) {
+        const float g = label_grad(at_label);
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (first + e == in_vecs) x[e] = g;
+    }
+}
+
+// Gradient of one row's vectors [lo, hi) and, if `with_singles`, its single elements: a exp(scale (x - top)) beside the
+// label, label_grad(x) at the label.  `live` false: zeros, nothing read.  Every thread reads what it overwrites and nothing
+// else, so `out` may be `row`.
+template <int IO, int THREADS, class LabelGrad>
+__device__ __forceinline__ void write_gradient(const typename Io<IO>::elem *row, typename Io<IO>::elem *out,
+                                               const RowSpan<IO> &span, int lo, int hi, bool with_singles, bool live,
+                                               int label, float top, float a, LabelGrad label_grad, float c) {
+    constexpr int E = Io<IO>::E;
+    constexpr int UNROLL = E == 8 ? 2 : 4;
+    typedef typename Io<IO>::elem Elem;
+    const Elem *vecs = row + span.head;
+    Elem *out_vecs = out + span.head;
+    const int in_vecs = label - span.head;
+    const int label_vec = in_vecs >= 0 ? in_vecs / E : -1;
+    // whole lines are written through (see store_row_vec)
+    const bool whole_lines = (reinterpret_cast<uintptr_t>(out_vecs) & 63) == 0;
+    for (int j0 = lo + static_cast<int>(threadIdx.x); j0 < hi; j0 += THREADS * UNROLL) {
+        typename Io<IO>::raw r[UNROLL];
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            const int j = j0 + u * THREADS;
+            r[u] = typename Io<IO>::raw{};
+            if (live && j < hi) r[u] = Io<IO>::template load_raw<true>(vecs + static_cast<int64_t>(E) * j);
+        }
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            const int j = j0 + u * THREADS;
+            if (j >= hi) break;
+            float x[E];
+            Io<IO>::unpack(r[u], x);
+            gradient_of(x, E * j, live, in_vecs, j == label_vec, top, a, label_grad, c);
+            store_row_vec<IO>(whole_lines, out_vecs, Io<IO>::kBytes * static_cast<uint32_t>(j), x);
+        }
+    }
+    if constexpr (E > 1) {
+        if (with_singles && static_cast<int>(threadIdx.x) < span.singles) {
+            constexpr int ONE = io_by_element(IO);
+            const int column = single_column(span, threadIdx.x);
+            float x[1] = {0.0f};
+            if (live) {
+                x[0] = Io<IO>::scalar(row + column);
+                x[0] = column == label ? label_grad(x[0]) : a * exp_scaled(x[0] - top, c);
+            }
+            Io<ONE>::template store<true>(out + column, x);
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------- token log-probabilities
+template <int IO>
+struct ScoreArgs {
+    typedef typename Io<IO>::elem Elem;
+    const Elem *logits;
+    int64_t ld;
+    const int32_t *labels;
+    float scale, c;
+    float *logp;
+    float *row_stats;  // [rows][2]: maximum, log sum
+    int64_t rows;
+    int cols;
+    hipStream_t stream;
+};
+
+template <class A>
+__device__ __forceinline__ void put_score(const A &a, int64_t row, bool live, const RowScore &r) {
+    a.logp[row] = live ? static_cast<float>(r.logp) : 0.0f;
+    if (a.row_stats) {
+        a.row_stats[2 * row] = live ? r.top : 0.0f;
+        a.row_stats[2 * row + 1] = live ? static_cast<float>(r.logsum) : 0.0f;
+    }
+}
+
+// One workgroup per row.
+template <int IO, int THREADS>
+__global__ __launch_bounds__(THREADS) void token_logprob_row_kernel(ScoreArgs<IO> a) {
+    __shared__ Pair slots[2][THREADS / 64];
+    int turn = 0;
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
+        const int label = a.labels[row];
+        RowScore r = nan_score();
+        if (label >= 0 && label < a.cols) {
+            const typename Io<IO>::elem *src = a.logits + row * a.ld;
+            const float at_label = Io<IO>::scalar(src + label);
+            const RowSpan<IO> span = span_of<IO>(src, a.cols);
+            const Pair p = block_pair<THREADS / 64>(thread_pair<IO, THREADS>(src, span, 0, span.nvec, true, label, a.c),
+                                                    slots[turn], a.c);
+            if (threadIdx.x == 0) r = score_row(p, at_label, a.scale, a.c);
+        }
+        if (threadIdx.x == 0) put_score(a, row, label >= 0, r);
+    }
+}
+
+// A few rows: workgroup (p, row) takes the row's p-th piece; pieces' pairs and the label's logit pass through the
+// workspace.
+struct PieceHeader {
+    float at_label;
+    float unused;
+};
+static_assert(sizeof(PieceHeader) == sizeof(Pair), "");
+// layout: Pair [rows][1 + parts], the first slot of a row being its header
+template <int IO, int THREADS>
+__global__ __launch_bounds__(THREADS) void token_pieces_kernel(const typename Io<IO>::elem *logits, int64_t ld,
+                                                               const int32_t *__restrict__ labels,
+                                                               const float *__restrict__ weight, int cols, float c,
+                                                               Pair *__restrict__ pairs) {
+    __shared__ Pair slot[THREADS / 64];
+    const int64_t row = blockIdx.y;
+    const int label = labels[row];
+    if (label < 0 || label >= cols || (weight && weight[row] == 0.0f)) return;
+    const typename Io<IO>::elem *src = logits + row * ld;
+    const RowSpan<IO> span = span_of<IO>(src, cols);
+    const int parts = static_cast<int>(gridDim.x), part = static_cast<int>(blockIdx.x);
+    const int piece = (span.nvec + parts - 1) / parts;
+    const int lo = part * piece < span.nvec ? part * piece : span.nvec;
+    const int hi = span.nvec - lo < piece ? span.nvec : lo + piece;
+    const Pair p = block_pair<THREADS / 64>(thread_pair<IO, THREADS>(src, span, lo, hi, part == 0, label, c), slot, c);
+    if (threadIdx.x == 0) {
+        Pair *mine = pairs + row * (1 + parts);
+        if (part == 0) mine[0] = Pair{Io<IO>::scalar(src + label), 0.0f};
+        mine[1 + part] = p;
+    }
+}
+__device__ __forceinline__ Pair fold_pieces(const Pair *mine, int parts, float c) {
+    float m = mine[1].m;
+    for (int i = 2; i <= parts; ++i) m = fmaxf(m, mine[i].m);
+    float s = 0.0f;
+    for (int i = 1; i <= parts; ++i) s += mine[i].s * exp_scaled(mine[i].m - m, c);
+    return Pair{m, s};
+}
+
+template <int IO>
+__global__ __launch_bounds__(64) void token_logprob_fold_kernel(ScoreArgs<IO> a, const Pair *__restrict__ pairs, int parts) {
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * 64 + threadIdx.x;
+    if (row >= a.rows) return;
+    const int label = a.labels[row];
+    RowScore r = nan_score();
+    const Pair *mine = pairs + row * (1 + parts);
+    if (label >= 0 && label < a.cols) r = score_row(fold_pieces(mine, parts, a.c), mine[0].m, a.scale, a.c);
+    put_score(a, row, label >= 0, r);
+}
+
+// Workgroup (p, row): a piece of the row's gradient.
+template <int IO, int THREADS>
+__global__ __launch_bounds__(THREADS) void token_logprob_backward_kernel(const typename Io<IO>::elem *logits, int64_t ld,
+                                                                         const int32_t *__restrict__ labels, float scale,
+                                                                         float c, const float *__restrict__ row_stats,
+                                                                         const float *__restrict__ dlogp,
+                                                                         typename Io<IO>::elem *dlogits, int64_t ldd,
+                                                                         int64_t rows, int cols) {
+    typedef typename Io<IO>::elem Elem;
+    for (int64_t row = blockIdx.y; row < rows; row += gridDim.y) {
+        const int label = labels[row];
+        float coeff = dlogp[row] * scale;
+        const bool live = label >= 0 && coeff != 0.0f;
+        if (label >= cols) coeff = __builtin_nanf("");
+        const Elem *src = logits + row * ld;
+        Elem *dst = dlogits + row * ldd;
+        const RowSpan<IO> span = span_of<IO>(dst, cols);
+        const int parts = static_cast<int>(gridDim.x), part = static_cast<int>(blockIdx.x);
+        const int piece = (span.nvec + parts - 1) / parts;
+        const int lo = part * piece < span.nvec ? part * piece : span.nvec;
+        const int hi = span.nvec - lo < piece ? span.nvec : lo + piece;
+        const float top = live ? row_stats[2 * row] : 0.0f;
+        const float logsum = live ? row_stats[2 * row + 1] : 0.0f;
+        const float a = -coeff * __builtin_amdgcn_exp2f(-logsum * kLog2e);
+        // coeff (1 - p), from p's logarithm: close to 0 that is where p has lost the difference
+        const auto label_grad = [&](float x) { return -coeff * expm1f((x - top) * scale - logsum); };
+        write_gradient<IO, THREADS>(src, dst, span, lo, hi, part == 0, live, label, top, a, label_grad, c);
+    }
+}
+
+// ------------------------------------------------------------------------------------------ clipped policy loss
+// Per row with a label and a weight w that is not 0, A its advantage:
+//   r = exp(logp - old), L = -min(r A, clip(r, 1 - low, 1 + high) A) + kl_coef k, k = exp(d) - d - 1, d = ref - logp;
+//   loss = w L;  d loss / d logp = w (-A r where r is not clipped, + kl_coef (1 - exp(d))).
+template <int IO>
+struct PolicyArgs {
+    typedef typename Io<IO>::elem Elem;
+    const Elem *logits;
+    int64_t ld;
+    const int32_t *labels;
+    const float *old_logp;   // null: the policy that sampled is the one that trains, r = 1
+    const float *ref_logp;   // null: no KL term
+    const float *advantage;
+    const float *weight;     // null: 1
+    float scale, c, clip_low, clip_high, kl_coef;
+    float *logp;
+    float *kl;
+    float *loss;
+    Elem *dlogits;           // null: no gradient
+    int64_t ldd;
+    int64_t rows;
+    int cols;
+    hipStream_t stream;
+};
+
+// What the gradient's writers need of a row.
+struct RowGradient {
+    float a, label_grad, top;
+    bool live;
+};
+
+template <int IO>
+__device__ __forceinline__ bool policy_row_counts(const PolicyArgs<IO> &a, int64_t row, int &label) {
+    label = a.labels[row];
+    return label >= 0 && (!a.weight || a.weight[row] != 0.0f);
+}
+
+// exp(d) - 1 - d, given up = exp(d) - 1: close to 0 the difference cancels, and the series takes over
+// (d^2 sum_n d^n / (n + 2)!, the first term left out is below 1e-8 of the first).
+__device__ __forceinline__ float kl_of(float d, float up) {
+    if (!(fabsf(d) < 0.5f)) return up - d;
+    float s = 1.0f / 362880.0f;
+    s = __builtin_fmaf(s, d, 1.0f / 40320.0f);
+    s = __builtin_fmaf(s, d, 1.0f / 5040.0f);
+    s = __builtin_fmaf(s, d, 1.0f / 720.0f);
+    s = __builtin_fmaf(s, d, 1.0f / 120.0f);
+    s = __builtin_fmaf(s, d, 1.0f / 24.0f);
+    s = __builtin_fmaf(s, d, 1.0f / 6.0f);
+    s = __builtin_fmaf(s, d, 0.5f);
+    return s * d * d;
+}
+
+// One thread's work: the row's outputs (if `put`) and its gradient's factors.
+template <int IO>
+__device__ __forceinline__ RowGradient policy_row(const PolicyArgs<IO> &a, int64_t row, bool counts, const RowScore &r, bool put) {
+    RowGradient g{0.0f, 0.0f, 0.0f, false};
+    double kl = 0.0, loss = 0.0;
+    if (counts) {
+        const double adv = a.advantage[row], w = a.weight ? a.weight[row] : 1.0f;
+        const double ratio = a.old_logp ? expf(static_cast<float>(r.logp - static_cast<double>(a.old_logp[row])))
+                                        : 1.0 + 0.0 * r.logp;
+        const double low = 1.0 - a.clip_low, high = 1.0 + a.clip_high;
+        double kept = ratio, slope = -adv * ratio;
+        if (adv > 0.0 ? ratio > high : ratio < low) {
+            kept = adv > 0.0 ? high : low;
+            slope = 0.0;
+        }
+        if (adv == 0.0) slope = kept = 0.0;  // (no surrogate, however large the ratio)
+        double total = -adv * kept;
+        if (a.ref_logp) {
+            const float d = static_cast<float>(static_cast<double>(a.ref_logp[row]) - r.logp);
+            const float up = expm1f(d);
+            kl = kl_of(d, up);
+            if (a.kl_coef != 0.0f) {
+                total += a.kl_coef * kl;
+                slope -= a.kl_coef * up;
+            }
+        }
+        loss = w * total;
+        const float coeff = static_cast<float>(w * slope * a.scale);
+        // a row whose gradient is 0 is written without a second look at its logits
+        g = RowGradient{-coeff * r.inv_total, coeff * r.rest, r.top, coeff != 0.0f};
+    }
+    if (put) {
+        if (a.logp) a.logp[row] = counts ? static_cast<float>(r.logp) : 0.0f;
+        if (a.kl) a.kl[row] = static_cast<float>(kl);
+        a.loss[row] = static_cast<float>(loss);
+    }
+    return g;
+}
+
+// One workgroup per row, any length and alignment: the sums, then a second read.
+template <int IO, int THREADS>
+__global__ __launch_bounds__(THREADS) void policy_reread_kernel(PolicyArgs<IO> a) {
+    __shared__ Pair slots[2][THREADS / 64];
+    __shared__ RowGradient shared[2];
+    int turn = 0;
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
+        int label;
+        const bool counts = policy_row_counts(a, row, label);
+        const typename Io<IO>::elem *src = a.logits + row * a.ld;
+        const RowSpan<IO> span = span_of<IO>(src, a.cols);
+        if (counts) {
+            RowScore r = nan_score();
+            if (label < a.cols) {
+                const float at_label = Io<IO>::scalar(src + label);
+                const Pair p = block_pair<THREADS / 64>(
+                    thread_pair<IO, THREADS>(src, span, 0, span.nvec, true, label, a.c), slots[turn], a.c);
+                if (threadIdx.x == 0) r = score_row(p, at_label, a.scale, a.c);
+            }
+            if (threadIdx.x == 0) shared[turn] = policy_row(a, row, true, r, true);
+            __syncthreads();
+        } else if (threadIdx.x == 0) {
+            policy_row(a, row, false, nan_score(), true);
+        }
+        if (!a.dlogits) continue;
+        const RowGradient g = counts ? shared[turn] : RowGradient{0.0f, 0.0f, 0.0f, false};
+        const auto label_grad = [&](float) { return g.label_grad; };
+        write_gradient<IO, THREADS>(src, a.dlogits + row * a.ldd, span, 0, span.nvec, true, g.live, label, g.top, g.a,
+                                    label_grad, a.c);
+    }
+}
+
+// A few rows, after token_pieces_kernel: workgroup (p, row) folds the row's pairs and writes the p-th piece.
+template <int IO, int THREADS>
+__global__ __launch_bounds__(THREADS) void policy_pieces_kernel(PolicyArgs<IO> a, const Pair *__restrict__ pairs, int parts) {
+    __shared__ RowGradient shared;
+    const int64_t row = blockIdx.y;
+    const int part = static_cast<int>(blockIdx.x);
+    int label;
+    const bool counts = policy_row_counts(a, row, label);
+    if (threadIdx.x == 0) {
+        RowScore r = nan_score();
+        const Pair *mine = pairs + row * (1 + parts);
+        if (counts && label < a.cols) r = score_row(fold_pieces(mine, parts, a.c), mine[0].m, a.scale, a.c);
+        shared = policy_row(a, row, counts, r, part == 0);
+    }
+    __syncthreads();
+    if (!a.dlogits) return;
+    const RowGradient g = shared;
+    const typename Io<IO>::elem *src = a.logits + row * a.ld;
+    const RowSpan<IO> span = span_of<IO>(src, a.cols);
+    const int piece = (span.nvec + parts - 1) / parts;
+    const int lo = part * piece < span.nvec ? part * piece : span.nvec;
+    const int hi = span.nvec - lo < piece ? span.nvec : lo + piece;
+    const auto label_grad = [&](float) { return g.label_grad; };
+    write_gradient<IO, THREADS>(src, a.dlogits + row * a.ldd, span, lo, hi, part == 0, g.live, label, g.top, g.a, label_grad,
+                                a.c);
+}
+
+// One workgroup per row at a time, the row in its registers, VPT vectors per thread: one read, one write.  While a row's
+// gradient is written the next row is loaded into the registers it leaves, so the workgroup always has loads or stores on
+// their way but for the two reductions.
+template <int IO, int THREADS, int VPT>
+__global__ __launch_bounds__(THREADS) void policy_onchip_kernel(PolicyArgs<IO> a) {
+    constexpr int E = Io<IO>::E;
+    typedef typename Io<IO>::elem Elem;
+    __shared__ Pair slots[2][THREADS / 64];
+    __shared__ RowGradient shared[2];
+
+    typename Io<IO>::raw r[VPT];
+    float single = -INFINITY, at_label = 0.0f;
+    int label;
+    bool counts, reads;
+    RowSpan<IO> span;
+    auto enter = [&](int64_t row) {  // (the row's scalars; rows past the last one count for nothing)
+        counts = false;
+        label = -1;
+        if (row < a.rows) counts = policy_row_counts(a, row, label);
+        reads = counts && label < a.cols;
+        span = span_of<IO>(a.logits + (row < a.rows ? row : 0) * a.ld, a.cols);
+        single = -INFINITY;
+        if (reads) {
+            const Elem *src = a.logits + row * a.ld;
+            if (static_cast<int>(threadIdx.x) < span.singles)
+                single = Io<IO>::scalar(src + single_column(span, threadIdx.x));
+            if (threadIdx.x == 0) at_label = Io<IO>::scalar(src + label);
+        }
+    };
+    auto load_vec = [&](int64_t row, int k) {
+        const int j = threadIdx.x + k * THREADS;
+        r[k] = typename Io<IO>::raw{};
+        if (reads && j < span.nvec)
+            r[k] = Io<IO>::template load_raw<true>(byte_offset(a.logits + row * a.ld + span.head, Io<IO>::kBytes * j));
+    };
+    enter(blockIdx.x);
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) load_vec(blockIdx.x, k);
+
+    int turn = 0;
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
+        const int in_vecs = label - span.head;
+        const int label_vec = in_vecs >= 0 ? in_vecs / E : -1;
+        RowGradient g{0.0f, 0.0f, 0.0f, false};
+        if (counts) {
+            RowScore score = nan_score();
+            if (reads) {
+                Pair p{-FLT_MAX, 0.0f};
+                constexpr int GROUP = 32 / E < VPT ? 32 / E : VPT;  // vectors whose sum is rescaled together
+                static_assert(VPT % GROUP == 0, "");
+#pragma unroll
+                for (int k0 = 0; k0 < VPT; k0 += GROUP) {
+                    float v[GROUP * E];
+                    // one group after the other: all of them converted at once would be twice the row's registers
+#pragma unroll
+                    for (int u = 0; u < GROUP; ++u) asm volatile("" : "+v"(r[k0 + u]), "+v"(p.s));
+#pragma unroll
+                    for (int u = 0; u < GROUP; ++u) {
+                        const int j = threadIdx.x + (k0 + u) * THREADS;
+                        float x[E];
+                        Io<IO>::unpack(r[k0 + u], x);
+                        if (j >= span.nvec || j == label_vec) {
+#pragma unroll
+                            for (int e = 0; e < E; ++e)
+                                if (j >= span.nvec || E * j + e == in_vecs) x[e] = -INFINITY;
+                        }
+#pragma unroll
+                        for (int e = 0; e < E; ++e) v[u * E + e] = x[e];
+                    }
+                    add_values(p, v, a.c);
+                }
+                const bool one_more = static_cast<int>(threadIdx.x) < span.singles && single_column(span, threadIdx.x) != label;
+                const float v[1] = {one_more ? single : -INFINITY};
+                add_values(p, v, a.c);
+                p = block_pair<THREADS / 64>(p, slots[turn], a.c);
+                if (threadIdx.x == 0) score = score_row(p, at_label, a.scale, a.c);
+            }
+            if (threadIdx.x == 0) shared[turn] = policy_row(a, row, true, score, true);
+            __syncthreads();
+            g = shared[turn];
+        } else if (threadIdx.x == 0) {
+            policy_row(a, row, false, nan_score(), true);
+        }
+        // this row's gradient out, the next row in
+        const RowSpan<IO> here = span;
+        const int here_label = label;
+        const float here_single = single;
+        const int64_t next = row + gridDim.x;
+        enter(next);
+        Elem *dst = a.dlogits + row * a.ldd;
+        Elem *dst_vecs = dst + here.head;
+        const bool whole_lines = (reinterpret_cast<uintptr_t>(dst_vecs) & 63) == 0;
+        const auto label_grad = [&](float) { return g.label_grad; };
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) {
+            const int j = threadIdx.x + k * THREADS;
+            if (j < here.nvec) {
+                float x[E];
+                convert_again<IO>(r[k]);
+                Io<IO>::unpack(r[k], x);
+                gradient_of(x, E * j, g.live, in_vecs, j == label_vec, g.top, g.a, label_grad, a.c);
+                store_row_vec<IO>(whole_lines, dst_vecs, Io<IO>::kBytes * static_cast<uint32_t>(j), x);
+            }
+            load_vec(next, k);
+        }
+        if (static_cast<int>(threadIdx.x) < here.singles) {
+            constexpr int ONE = io_by_element(IO);
+            const int column = single_column(here, threadIdx.x);
+            float x[1] = {0.0f};
+            if (g.live) x[0] = column == here_label ? g.label_grad : g.a * exp_scaled(here_single - g.top, a.c);
+            Io<ONE>::template store<true>(dst + column, x);
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------- sums
+__device__ __forceinline__ double wave_sum(double v) {
+#pragma unroll
+    for (int step = 1; step < 64; step <<= 1) v += __shfl_xor(v, step, 64);
+    return v;
+}
+
+// out[0] = factor * sum of n values, in 64 bits and in a fixed order: one workgroup.
+__global__ __launch_bounds__(1024) void loss_sum_kernel(const float *__restrict__ values, int64_t n, float factor, float *out) {
+    __shared__ double sums[16];
+    double s = 0.0;
+    for (int64_t i = threadIdx.x; i < n; i += 1024) s += values[i];
+    s = wave_sum(s);
+    if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    s = 0.0;
+    for (int w = 0; w < 16; ++w) s += sums[w];
+    out[0] = static_cast<float>(factor * s);
+}
+
+// ------------------------------------------------------------------------------------------------ preference loss
+// Pair p: sequence 2p is the chosen one, 2p + 1 the rejected one; sequence i's tokens are [offsets[i], offsets[i + 1]).
+//   reward_i = beta sum (logp - ref), h = reward_chosen - reward_rejected,
+//   loss = (1 - eps) softplus(-h) + eps softplus(h),  d loss / d h = eps - 1 / (1 + exp(h)).
+// One workgroup per pair, sums in 64 bits.
+struct PreferenceArgs {
+    const float *logp;
+    const float *ref_logp;
+    const int32_t *labels;   // null, or: tokens with a negative label count for nothing
+    const int32_t *offsets;
+    int64_t pairs, tokens;
+    float beta, eps, pair_weight;
+    float *pair_loss;
+    float *rewards;
+    float *dlogp;
+};
+constexpr int kPreferenceThreads = 512;
+
+__global__ __launch_bounds__(kPreferenceThreads) void preference_kernel(PreferenceArgs a) {
+    constexpr int WAVES = kPreferenceThreads / 64;
+    __shared__ double sums[2][WAVES];
+    for (int64_t pair = blockIdx.x; pair < a.pairs; pair += gridDim.x) {
+        // offsets are the caller's device data: none of them leads outside the tokens
+        int64_t at[3];
+        for (int i = 0; i < 3; ++i) {
+            at[i] = a.offsets[2 * pair + i];
+            if (at[i] < (i ? at[i - 1] : 0)) at[i] = i ? at[i - 1] : 0;
+            if (at[i] > a.tokens) at[i] = a.tokens;
+        }
+        double s[2] = {0.0, 0.0};
+        constexpr int UNROLL = 4;
+        for (int64_t t0 = at[0] + threadIdx.x; t0 < at[2]; t0 += kPreferenceThreads * UNROLL) {
+            float lp[UNROLL], ref[UNROLL];
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u) {
+                const int64_t t = t0 + u * kPreferenceThreads;
+                lp[u] = ref[u] = 0.0f;
+                if (t < at[2] && (!a.labels || a.labels[t] >= 0)) {
+                    lp[u] = a.logp[t];
+                    ref[u] = a.ref_logp[t];
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u)
+                s[t0 + u * kPreferenceThreads < at[1] ? 0 : 1] += static_cast<double>(lp[u]) - static_cast<double>(ref[u]);
+        }
+        __syncthreads();  // the previous pair's sums have been read
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            s[i] = wave_sum(s[i]);
+            if ((threadIdx.x & 63) == 0) sums[i][threadIdx.x >> 6] = s[i];
+        }
+        __syncthreads();
+        double reward[2];
+        for (int i = 0; i < 2; ++i) {
+            reward[i] = 0.0;
+            for (int w = 0; w < WAVES; ++w) reward[i] += sums[i][w];
+            reward[i] *= a.beta;
+        }
+        const double h = reward[0] - reward[1];
+        const double slope = a.eps - 1.0 / (1.0 + exp(h));
+        if (threadIdx.x == 0) {
+            const double both = log1p(exp(-fabs(h)));
+            double loss = (1.0 - a.eps) * (both + (h < 0.0 ? -h : 0.0));
+            if (a.eps != 0.0f) loss += a.eps * (both + (h > 0.0 ? h : 0.0));
+            a.pair_loss[pair] = static_cast<float>(loss);
+            if (a.rewards) {
+                a.rewards[2 * pair] = static_cast<float>(reward[0]);
+                a.rewards[2 * pair + 1] = static_cast<float>(reward[1]);
+            }
+        }
+        if (!a.dlogp) continue;
+        const float up = static_cast<float>(slope * a.beta * a.pair_weight);
+        for (int64_t t = at[0] + threadIdx.x; t < at[2]; t += kPreferenceThreads)
+            a.dlogp[t] = a.labels && a.labels[t] < 0 ? 0.0f : t < at[1] ? up : -up;
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------- dispatch
+// Pieces per row of a few rows: a function of the sizes alone, so that the workspace can be sized without a device.
+constexpr int kPieceUnits = 256;  // compute units of an MI355X
+constexpr int64_t kPieceColumns = 4096;
+int pieces_per_row(int64_t rows, int64_t cols) {
+    if (rows <= 0 || rows * 2 > kPieceUnits) return 1;
+    int64_t parts = 2 * kPieceUnits / rows;
+    if (parts > cols / kPieceColumns) parts = cols / kPieceColumns;
+    return parts < 2 ? 1 : static_cast<int>(parts);
+}
+size_t workspace_bytes(int64_t rows, int64_t cols) {
+    if (rows <= 0 || cols <= 0 || cols > (1 << 30)) return 0;
+    const int parts = pieces_per_row(rows, cols);
+    return parts > 1 ? static_cast<size_t>(rows) * (1 + parts) * sizeof(Pair) : 0;
+}
+
+unsigned row_grid(int64_t rows) { return static_cast<unsigned>(rows > 0x7fffffff ? 0x7fffffff : rows); }
+
+// What every entry on rows of logits checks.
+int check_logits(const char *who, const void *logits, int64_t ld, const void *labels, size_t size, float scale, int64_t rows,
+                 int64_t cols, const void *workspace, size_t bytes) {
+    if (rows < 0 || cols <= 0) return fail(KO_ERR_INVALID_ARGUMENT, "%s: rows=%lld cols=%lld", who, (long long)rows, (long long)cols);
+    if (cols > (1 << 30)) return fail(KO_ERR_UNSUPPORTED_SHAPE, "%s: cols=%lld too large", who, (long long)cols);
+    if (ld < cols) return fail(KO_ERR_INVALID_ARGUMENT, "%s: ld=%lld is less than cols=%lld", who, (long long)ld, (long long)cols);
+    if (!(scale >= 1e-30f && scale <= 1e30f)) return fail(KO_ERR_INVALID_ARGUMENT, "%s: scale=%g", who, static_cast<double>(scale));
+    if (rows > 0 && (!logits || !labels)) return fail(KO_ERR_INVALID_ARGUMENT, "%s: null logits/labels pointer", who);
+    if ((reinterpret_cast<uintptr_t>(logits) & (size - 1)) || (reinterpret_cast<uintptr_t>(labels) & 3))
+        return fail(KO_ERR_INVALID_ARGUMENT, "%s: logits/labels must be aligned to their element type", who);
+    if (workspace && bytes < workspace_bytes(rows, cols))
+        return fail(KO_ERR_INVALID_ARGUMENT, "%s: workspace of %zu bytes, %zu needed", who, bytes, workspace_bytes(rows, cols));
+    if (reinterpret_cast<uintptr_t>(workspace) & 15)
+        return fail(KO_ERR_INVALID_ARGUMENT, "%s: workspace must be 16-byte aligned", who);
+    return KO_OK;
+}
+int check_gradient(const char *who, const void *dlogits, int64_t ldd, size_t size, int64_t cols) {
+    if (ldd < cols) return fail(KO_ERR_INVALID_ARGUMENT, "%s: ldd=%lld is less than cols=%lld", who, (long long)ldd, (long long)cols);
+    if (reinterpret_cast<uintptr_t>(dlogits) & (size - 1))
+        return fail(KO_ERR_INVALID_ARGUMENT, "%s: dlogits must be aligned to its element type", who);
+    return KO_OK;
+}
+int check_floats(const char *who, std::initializer_list<const void *> pointers) {
+    for (const void *p : pointers)
+        if (reinterpret_cast<uintptr_t>(p) & 3) return fail(KO_ERR_INVALID_ARGUMENT, "%s: fp32 arrays must be 4-byte aligned", who);
+    return KO_OK;
+}
+// Rows of logits and of their gradient lie alike: every row starts at the same place of a 16-byte vector in both.
+bool rows_lie_alike(const void *logits, int64_t ld, const void *dlogits, int64_t ldd, size_t size) {
+    const uintptr_t base = reinterpret_cast<uintptr_t>(logits) ^ reinterpret_cast<uintptr_t>(dlogits);
+    return (base & 15) == 0 && ((static_cast<uint64_t>(ld) - static_cast<uint64_t>(ldd)) * size & 15) == 0;
+}
+
+template <int IO, int THREADS>
+int launch_pieces(const typename Io<IO>::elem *logits, int64_t ld, const int32_t *labels, const float *weight, int64_t rows,
+                  int cols, float c, Pair *pairs, int parts, hipStream_t stream) {
+    token_pieces_kernel<IO, THREADS><<<dim3(static_cast<unsigned>(parts), static_cast<unsigned>(rows)), dim3(THREADS), 0, stream>>>(
+        logits, ld, labels, weight, cols, c, pairs);
+    KO_CHECK_LAUNCH();
+    return KO_OK;
+}
+
+template <int IO>
+int logprob_entry(const void *logits, int64_t ld, const int32_t *labels, float scale, float *logp, float *row_stats,
+                  int64_t rows, int64_t cols, void *workspace, size_t bytes, ko_stream_t stream) {
+    typedef typename Io<IO>::elem Elem;
+    static const char *const who = "token_logprob";
+    if (const int st = check_logits(who, logits, ld, labels, sizeof(Elem), scale, rows, cols, workspace, bytes); st != KO_OK) return st;
+    if (const int st = check_floats(who, {logp, row_stats}); st != KO_OK) return st;
+    if (rows == 0) return KO_OK;
+    if (!logp) return fail(KO_ERR_INVALID_ARGUMENT, "%s: null logp pointer", who);
+    const ScoreArgs<IO> a{static_cast<const Elem *>(logits), ld, labels, scale, scale * kLog2e, logp, row_stats, rows,
+                          static_cast<int>(cols), as_stream(stream)};
+    const int parts = pieces_per_row(rows, cols);
+    if (workspace && parts > 1) {
+        Pair *pairs = static_cast<Pair *>(workspace);
+        if (const int st = launch_pieces<IO, 256>(a.logits, ld, labels, nullptr, rows, a.cols, a.c, pairs, parts, a.stream); st != KO_OK)
+            return st;
+        token_logprob_fold_kernel<IO><<<dim3(static_cast<unsigned>((rows + 63) / 64)), dim3(64), 0, a.stream>>>(a, pairs, parts);
+        KO_CHECK_LAUNCH();
+        return KO_OK;
+    }
+    const dim3 grid(row_grid(rows));
+    if (cols <= 4096) token_logprob_row_kernel<IO, 256><<<grid, dim3(256), 0, a.stream>>>(a);
+    else if (cols <= 32768 || rows >= 1024) token_logprob_row_kernel<IO, 512><<<grid, dim3(512), 0, a.stream>>>(a);
+    else token_logprob_row_kernel<IO, 1024><<<grid, dim3(1024), 0, a.stream>>>(a);
+    KO_CHECK_LAUNCH();
+    return KO_OK;
+}
+
+template <int IO>
+int launch_logprob_backward(const void *logits, int64_t ld, const int32_t *labels, float scale, const float *row_stats,
+                            const float *dlogp, void *dlogits, int64_t ldd, int64_t rows, int64_t cols, hipStream_t stream) {
+    typedef typename Io<IO>::elem Elem;
+    constexpr int THREADS = 256;
+    // pieces of two trips of a workgroup
+    const int64_t piece = int64_t{THREADS} * 4 * Io<IO>::E;
+    const unsigned parts = static_cast<unsigned>((cols + piece - 1) / piece);
+    const unsigned grid_rows = static_cast<unsigned>(rows > 65535 ? 65535 : rows);
+    token_logprob_backward_kernel<IO, THREADS><<<dim3(parts, grid_rows), dim3(THREADS), 0, stream>>>(
+        static_cast<const Elem *>(logits), ld, labels, scale, scale * kLog2e, row_stats, dlogp, static_cast<Elem *>(dlogits), ldd,
+        rows, static_cast<int>(cols));
+    KO_CHECK_LAUNCH();
+    return KO_OK;
+}
+
+template <int IO>
+int logprob_backward_entry(const void *logits, int64_t ld, const int32_t *labels, float scale, const float *row_stats,
+                           const float *dlogp, void *dlogits, int64_t ldd, int64_t rows, int64_t cols, ko_stream_t stream) {
+    constexpr size_t kSize = sizeof(typename Io<IO>::elem);
+    static const char *const who = "token_logprob_backward";
+    if (const int st = check_logits(who, logits, ld, labels, kSize, scale, rows, cols, nullptr, 0); st != KO_OK) return st;
+    if (const int st = check_gradient(who, dlogits, ldd, kSize, cols); st != KO_OK) return st;
+    if (const int st = check_floats(who, {row_stats, dlogp}); st != KO_OK) return st;
+    if (rows == 0) return KO_OK;
+    if (!row_stats || !dlogp || !dlogits) return fail(KO_ERR_INVALID_ARGUMENT, "%s: null row_stats/dlogp/dlogits pointer", who);
+    if (rows_lie_alike(logits, ld, dlogits, ldd, kSize))
+        return launch_logprob_backward<IO>(logits, ld, labels, scale, row_stats, dlogp, dlogits, ldd, rows, cols, as_stream(stream));
+    return launch_logprob_backward<io_by_element(IO)>(logits, ld, labels, scale, row_stats, dlogp, dlogits, ldd, rows, cols,
+                                                      as_stream(stream));
+}
+
+template <int IO, int THREADS, int VPT>
+int launch_onchip(const PolicyArgs<IO> &a) {
+    // as many workgroups as are resident at once walk over the rows
+    constexpr int kPerUnit = THREADS * VPT <= 1024 * 4 ? 4096 / (THREADS * VPT) * 2 : THREADS * VPT <= 1024 * 8 ? 2 : 1;
+    int64_t grid = static_cast<int64_t>(compute_units()) * (kPerUnit * THREADS > 2048 ? 2048 / THREADS : kPerUnit);
+    if (grid > a.rows) grid = a.rows;
+    policy_onchip_kernel<IO, THREADS, VPT><<<dim3(static_cast<unsigned>(grid)), dim3(THREADS), 0, a.stream>>>(a);
+    KO_CHECK_LAUNCH();
+    return KO_OK;
+}
+
+template <int IO>
+int launch_policy(const PolicyArgs<IO> &a, void *workspace) {
+    const int parts = pieces_per_row(a.rows, a.cols);
+    if (workspace && parts > 1) {
+        Pair *pairs = static_cast<Pair *>(workspace);
+        if (const int st = launch_pieces<IO, 256>(a.logits, a.ld, a.labels, a.weight, a.rows, a.cols, a.c, pairs, parts, a.stream);
+            st != KO_OK)
+            return st;
+        const dim3 grid(a.dlogits ? static_cast<unsigned>(parts) : 1u, static_cast<unsigned>(a.rows));
+        policy_pieces_kernel<IO, 256><<<grid, dim3(256), 0, a.stream>>>(a, pairs, parts);
+        KO_CHECK_LAUNCH();
+        return KO_OK;
+    }
+    if constexpr (Io<IO>::E > 1) {
+        const int nvec = a.cols / Io<IO>::E;
+        if (a.dlogits) {
+            if (nvec <= 512) return launch_onchip<IO, 256, 2>(a);
+            if (nvec <= 1024) return launch_onchip<IO, 256, 4>(a);
+            if (nvec <= 2048) return launch_onchip<IO, 512, 4>(a);
+            if (nvec <= 4096) return launch_onchip<IO, 1024, 4>(a);
+            if (nvec <= 8192) return launch_onchip<IO, 1024, 8>(a);
+        }
+    }
+    const dim3 grid(row_grid(a.rows));
+    if (a.cols <= 4096) policy_reread_kernel<IO, 256><<<grid, dim3(256), 0, a.stream>>>(a);
+    else if (a.cols <= 32768) policy_reread_kernel<IO, 512><<<grid, dim3(512), 0, a.stream>>>(a);
+    else policy_reread_kernel<IO, 1024><<<grid, dim3(1024), 0, a.stream>>>(a);
+    KO_CHECK_LAUNCH();
+    return KO_OK;
+}
+
+int launch_loss_sum(const float *values, int64_t n, float factor, float *out, hipStream_t stream) {
+    loss_sum_kernel<<<dim3(1), dim3(1024), 0, stream>>>(values, n, factor, out);
+    KO_CHECK_LAUNCH();
+    return KO_OK;
+}
+
+template <int IO>
+int policy_entry(const void *logits, int64_t ld, const int32_t *labels, const float *old_logp, const float *ref_logp,
+                 const float *advantage, const float *weight, float scale, float clip_low, float clip_high, float kl_coef,
+                 float *logp, float *kl, float *loss, float *loss_sum, void *dlogits, int64_t ldd, int64_t rows, int64_t cols,
+                 void *workspace, size_t bytes, ko_stream_t stream) {
+    typedef typename Io<IO>::elem Elem;
+    static const char *const who = "policy_loss";
+    if (const int st = check_logits(who, logits, ld, labels, sizeof(Elem), scale, rows, cols, workspace, bytes); st != KO_OK) return st;
+    if (dlogits) {
+        if (const int st = check_gradient(who, dlogits, ldd, sizeof(Elem), cols); st != KO_OK) return st;
+    }
+    if (const int st = check_floats(who, {old_logp, ref_logp, advantage, weight, logp, kl, loss, loss_sum}); st != KO_OK) return st;
+    if (!(clip_low >= 0.0f && clip_low <= 1.0f) || !(clip_high >= 0.0f && clip_high < INFINITY))
+        return fail(KO_ERR_INVALID_ARGUMENT, "%s: clip_low=%g clip_high=%g", who, static_cast<double>(clip_low), static_cast<double>(clip_high));
+    if (!(kl_coef > -INFINITY && kl_coef < INFINITY)) return fail(KO_ERR_INVALID_ARGUMENT, "%s: kl_coef=%g", who, static_cast<double>(kl_coef));
+    const hipStream_t s = as_stream(stream);
+    if (rows == 0) return loss_sum ? launch_loss_sum(nullptr, 0, 1.0f, loss_sum, s) : KO_OK;
+    if (!advantage || !loss) return fail(KO_ERR_INVALID_ARGUMENT, "%s: null advantage/loss pointer", who);
+    auto run = [&](auto kind) {
+        constexpr int KIND = decltype(kind)::value;
+        const PolicyArgs<KIND> a{static_cast<const Elem *>(logits), ld, labels, old_logp, ref_logp, advantage, weight, scale,
+                                 scale * kLog2e, clip_low, clip_high, kl_coef, logp, kl, loss, static_cast<Elem *>(dlogits), ldd,
+                                 rows, static_cast<int>(cols), s};
+        return launch_policy<KIND>(a, workspace);
+    };
+    const bool alike = !dlogits || rows_lie_alike(logits, ld, dlogits, ldd, sizeof(Elem));
+    const int st = alike ? run(std::integral_constant<int, IO>{}) : run(std::integral_constant<int, io_by_element(IO)>{});
+    if (st != KO_OK || !loss_sum) return st;
+    return launch_loss_sum(loss, rows, 1.0f, loss_sum, s);
+}
+
+}  // namespace
+}  // namespace ko
+
+KO_EXPORT size_t ko_token_logprob_workspace_bytes(int64_t rows, int64_t cols) { return ko::workspace_bytes(rows, cols); }
+
+KO_EXPORT int ko_token_logprob_f32(const float *logits, int64_t ld, const int32_t *labels, float scale, float *logp,
+                                   float *row_stats, int64_t rows, int64_t cols, void *workspace, size_t workspace_bytes,
+                                   ko_stream_t stream) {
+    return ko::logprob_entry<ko::IO_F32>(logits, ld, labels, scale, logp, row_stats, rows, cols, workspace, workspace_bytes, stream);
+}
+
+KO_EXPORT int ko_token_logprob_16(const void *logits, int64_t ld, const int32_t *labels, float scale, float *logp,
+                                  float *row_stats, int64_t rows, int64_t cols, int dtype, void *workspace,
+                                  size_t workspace_bytes, ko_stream_t stream) {
+    if (dtype == KO_F16)
+        return ko::logprob_entry<ko::IO_F16>(logits, ld, labels, scale, logp, row_stats, rows, cols, workspace, workspace_bytes, stream);
+    if (dtype == KO_BF16)
+        return ko::logprob_entry<ko::IO_BF16>(logits, ld, labels, scale, logp, row_stats, rows, cols, workspace, workspace_bytes, stream);
+    return ko::fail(KO_ERR_INVALID_ARGUMENT, "token_logprob: dtype=%d is neither KO_F16 nor KO_BF16", dtype);
+}
+
+KO_EXPORT int ko_token_logprob_backward_f32(const float *logits, int64_t ld, const int32_t *labels, float scale,
+                                            const float *row_stats, const float *dlogp, float *dlogits, int64_t ldd, int64_t rows,
+                                            int64_t cols, ko_stream_t stream) {
+    return ko::logprob_backward_entry<ko::IO_F32>(logits, ld, labels, scale, row_stats, dlogp, dlogits, ldd, rows, cols, stream);
+}
+
+KO_EXPORT int ko_token_logprob_backward_16(const void *logits, int64_t ld, const int32_t *labels, float scale,
+                                           const float *row_stats, const float *dlogp, void *dlogits, int64_t ldd, int64_t rows,
+                                           int64_t cols, int dtype, ko_stream_t stream) {
+    if (dtype == KO_F16)
+        return ko::logprob_backward_entry<ko::IO_F16>(logits, ld, labels, scale, row_stats, dlogp, dlogits, ldd, rows, cols, stream);
+    if (dtype == KO_BF16)
+        return ko::logprob_backward_entry<ko::IO_BF16>(logits, ld, labels, scale, row_stats, dlogp, dlogits, ldd, rows, cols, stream);
+    return ko::fail(KO_ERR_INVALID_ARGUMENT, "token_logprob_backward: dtype=%d is neither KO_F16 nor KO_BF16", dtype);
+}
+
+KO_EXPORT int ko_policy_loss_f32(const float *logits, int64_t ld, const int32_t *labels, const float *old_logp,
+                                 const float *ref_logp, const float *advantage, const float *weight, float scale, float clip_low,
+                                 float clip_high, float kl_coef, float *logp, float *kl, float *loss, float *loss_sum,
+                                 float *dlogits, int64_t ldd, int64_t rows, int64_t cols, void *workspace, size_t workspace_bytes,
+                                 ko_stream_t stream) {
+    return ko::policy_entry<ko::IO_F32>(logits, ld, labels, old_logp, ref_logp, advantage, weight, scale, clip_low, clip_high,
+                                        kl_coef, logp, kl, loss, loss_sum, dlogits, ldd, rows, cols, workspace, workspace_bytes,
+                                        stream);
+}
+
+KO_EXPORT int ko_policy_loss_16(const void *logits, int64_t ld, const int32_t *labels, const float *old_logp,
+                                const float *ref_logp, const float *advantage, const float *weight, float scale, float clip_low,
+                                float clip_high, float kl_coef, float *logp, float *kl, float *loss, float *loss_sum,
+                                void *dlogits, int64_t ldd, int64_t rows, int64_t cols, int dtype, void *workspace,
+                                size_t workspace_bytes, ko_stream_t stream) {
+    if (dtype == KO_F16)
+        return ko::policy_entry<ko::IO_F16>(logits, ld, labels, old_logp, ref_logp, advantage, weight, scale, clip_low, clip_high,
+                                            kl_coef, logp, kl, loss, loss_sum, dlogits, ldd, rows, cols, workspace,
+                                            workspace_bytes, stream);
+    if (dtype == KO_BF16)
+        return ko::policy_entry<ko::IO_BF16>(logits, ld, labels, old_logp, ref_logp, advantage, weight, scale, clip_low, clip_high,
+                                             kl_coef, logp, kl, loss, loss_sum, dlogits, ldd, rows, cols, workspace,
+                                             workspace_bytes, stream);
+    return ko::fail(KO_ERR_INVALID_ARGUMENT, "policy_loss: dtype=%d is neither KO_F16 nor KO_BF16", dtype);
+}
+
+KO_EXPORT int ko_preference_loss_f32(const float *logp, const float *ref_logp, const int32_t *labels, const int32_t *offsets,
+                                     int64_t pairs, int64_t tokens, float beta, float label_smoothing, float pair_weight,
+                                     float *pair_loss, float *rewards, float *dlogp, float *loss_sum, ko_stream_t stream) {
+    static const char *const who = "preference_loss";
+    if (pairs < 0 || tokens < 0 || tokens > 0x7fffffff)
+        return ko::fail(KO_ERR_INVALID_ARGUMENT, "%s: pairs=%lld tokens=%lld", who, (long long)pairs, (long long)tokens);
+    if (!(beta > -INFINITY && beta < INFINITY) || !(pair_weight > -INFINITY && pair_weight < INFINITY))
+        return ko::fail(KO_ERR_INVALID_ARGUMENT, "%s: beta=%g pair_weight=%g", who, static_cast<double>(beta), static_cast<double>(pair_weight));
+    if (!(label_smoothing >= 0.0f && label_smoothing <= 1.0f))
+        return ko::fail(KO_ERR_INVALID_ARGUMENT, "%s: label_smoothing=%g", who, static_cast<double>(label_smoothing));
+    if (const int st = ko::check_floats(who, {logp, ref_logp, labels, offsets, pair_loss, rewards, dlogp, loss_sum}); st != KO_OK)
+        return st;
+    const hipStream_t s = ko::as_stream(stream);
+    if (pairs == 0) return loss_sum ? ko::launch_loss_sum(nullptr, 0, pair_weight, loss_sum, s) : KO_OK;
+    if (!offsets || !pair_loss || (tokens > 0 && (!logp || !ref_logp)))
+        return ko::fail(KO_ERR_INVALID_ARGUMENT, "%s: null logp/ref_logp/offsets/pair_loss pointer", who);
+    const ko::PreferenceArgs a{logp, ref_logp, labels, offsets, pairs, tokens, beta, label_smoothing, pair_weight, pair_loss,
+                               rewards, dlogp};
+    ko::preference_kernel<<<dim3(ko::row_grid(pairs)), dim3(ko::kPreferenceThreads), 0, s>>>(a);
+    KO_CHECK_LAUNCH();
+    return loss_sum ? ko::launch_loss_sum(pair_loss, pairs, pair_weight, loss_sum, s) : KO_OK;
+}
