@@ -198,6 +198,10 @@ class Stream:
         check(lib().ko_stream_create(ctypes.byref(h)))
         self.handle = h
 
+    @property
+    def _as_parameter_(self):
+        return self.handle
+
     def synchronize(self):
         check(lib().ko_stream_synchronize(self.handle))
 
@@ -255,6 +259,10 @@ class DeviceBuffer:
         p = _vp()
         check(lib().ko_malloc(ctypes.byref(p), self.nbytes))
         self.ptr = p.value or 0
+
+    @property
+    def _as_parameter_(self):
+        return self.ptr or None
 
     @classmethod
     def from_numpy(cls, a):
@@ -319,20 +327,23 @@ def layernorm16(inp, out, rows, cols, mean=None, rstd=None, gamma=None, beta=Non
                                 int(bool(unbiased)), dtype, policy, _h(stream)))
 
 
+# The operators below are called once per layer or per step of a training loop, on pointers that the caller has in hand: a
+# pointer is a DeviceBuffer, an address or None, a stream a Stream, a hipStream_t value or None, and ctypes takes them as
+# they are (_as_parameter_).
 def softmax_backward_workspace_bytes(rows, cols):
     return lib().ko_softmax_backward_workspace_bytes(rows, cols)
 
 
 def softmax_backward(y, dy, dx, rows, cols, valid_len=None, rows_per_seq=0, workspace=None, workspace_bytes=0, stream=None):
     """dx = y (dy - sum y dy) per row; workspace: softmax_backward_workspace_bytes(rows, cols) bytes, or None."""
-    check(lib().ko_softmax_backward_f32(_p(y), _p(dy), _p(dx), rows, cols, _p(valid_len), rows_per_seq, _p(workspace),
-                                        workspace_bytes, _h(stream)))
+    check(lib().ko_softmax_backward_f32(y, dy, dx, rows, cols, valid_len, rows_per_seq, workspace,
+                                        workspace_bytes, stream))
 
 
 def softmax_backward16(y, dy, dx, rows, cols, valid_len=None, rows_per_seq=0, dtype=F16, workspace=None, workspace_bytes=0,
                        stream=None):
-    check(lib().ko_softmax_backward_16(_p(y), _p(dy), _p(dx), rows, cols, _p(valid_len), rows_per_seq, dtype, _p(workspace),
-                                       workspace_bytes, _h(stream)))
+    check(lib().ko_softmax_backward_16(y, dy, dx, rows, cols, valid_len, rows_per_seq, dtype, workspace,
+                                       workspace_bytes, stream))
 
 
 def layernorm_backward_workspace_bytes(rows, cols):
@@ -343,16 +354,16 @@ def layernorm_backward(dy, inp, mean, rstd, dx, rows, cols, gamma=None, dres=Non
                        workspace=None, workspace_bytes=0, stream=None):
     """dx (+ dres), and dgamma and dbeta where wanted, from the forward pass's input, mean and rstd; workspace:
     layernorm_backward_workspace_bytes(rows, cols) bytes, or None."""
-    check(lib().ko_layernorm_backward_f32(_p(dy), _p(inp), _p(mean), _p(rstd), _p(gamma), _p(dres), _p(dx), _p(dgamma),
-                                          _p(dbeta), rows, cols, int(bool(unbiased)), _p(workspace), workspace_bytes,
-                                          _h(stream)))
+    check(lib().ko_layernorm_backward_f32(dy, inp, mean, rstd, gamma, dres, dx, dgamma,
+                                          dbeta, rows, cols, int(bool(unbiased)), workspace, workspace_bytes,
+                                          stream))
 
 
 def layernorm_backward16(dy, inp, mean, rstd, dx, rows, cols, gamma=None, dres=None, dgamma=None, dbeta=None, unbiased=False,
                          dtype=F16, workspace=None, workspace_bytes=0, stream=None):
-    check(lib().ko_layernorm_backward_16(_p(dy), _p(inp), _p(mean), _p(rstd), _p(gamma), _p(dres), _p(dx), _p(dgamma),
-                                         _p(dbeta), rows, cols, int(bool(unbiased)), dtype, _p(workspace), workspace_bytes,
-                                         _h(stream)))
+    check(lib().ko_layernorm_backward_16(dy, inp, mean, rstd, gamma, dres, dx, dgamma,
+                                         dbeta, rows, cols, int(bool(unbiased)), dtype, workspace, workspace_bytes,
+                                         stream))
 
 
 def token_logprob_workspace_bytes(rows, cols):
@@ -363,27 +374,27 @@ def token_logprob_workspace_bytes(rows, cols):
 def token_logprob(logits, labels, logp, rows, cols, ld=None, scale=1.0, row_stats=None, workspace=None, workspace_bytes=0,
                   stream=None):
     """logp[r] = log softmax(scale logits[r])[labels[r]]; rows with a negative label are not read and get 0."""
-    check(lib().ko_token_logprob_f32(_p(logits), cols if ld is None else ld, _p(labels), scale, _p(logp), _p(row_stats), rows,
-                                     cols, _p(workspace), workspace_bytes, _h(stream)))
+    check(lib().ko_token_logprob_f32(logits, cols if ld is None else ld, labels, scale, logp, row_stats, rows,
+                                     cols, workspace, workspace_bytes, stream))
 
 
 def token_logprob16(logits, labels, logp, rows, cols, ld=None, scale=1.0, row_stats=None, dtype=F16, workspace=None,
                     workspace_bytes=0, stream=None):
-    check(lib().ko_token_logprob_16(_p(logits), cols if ld is None else ld, _p(labels), scale, _p(logp), _p(row_stats), rows,
-                                    cols, dtype, _p(workspace), workspace_bytes, _h(stream)))
+    check(lib().ko_token_logprob_16(logits, cols if ld is None else ld, labels, scale, logp, row_stats, rows,
+                                    cols, dtype, workspace, workspace_bytes, stream))
 
 
 def token_logprob_backward(logits, labels, row_stats, dlogp, dlogits, rows, cols, ld=None, ldd=None, scale=1.0, stream=None):
     """dlogits = dlogp scale (onehot(label) - softmax(scale logits)), row_stats from token_logprob."""
-    check(lib().ko_token_logprob_backward_f32(_p(logits), cols if ld is None else ld, _p(labels), scale, _p(row_stats),
-                                              _p(dlogp), _p(dlogits), cols if ldd is None else ldd, rows, cols, _h(stream)))
+    check(lib().ko_token_logprob_backward_f32(logits, cols if ld is None else ld, labels, scale, row_stats,
+                                              dlogp, dlogits, cols if ldd is None else ldd, rows, cols, stream))
 
 
 def token_logprob_backward16(logits, labels, row_stats, dlogp, dlogits, rows, cols, ld=None, ldd=None, scale=1.0, dtype=F16,
                              stream=None):
-    check(lib().ko_token_logprob_backward_16(_p(logits), cols if ld is None else ld, _p(labels), scale, _p(row_stats),
-                                             _p(dlogp), _p(dlogits), cols if ldd is None else ldd, rows, cols, dtype,
-                                             _h(stream)))
+    check(lib().ko_token_logprob_backward_16(logits, cols if ld is None else ld, labels, scale, row_stats,
+                                             dlogp, dlogits, cols if ldd is None else ldd, rows, cols, dtype,
+                                             stream))
 
 
 def policy_loss(logits, labels, advantage, loss, rows, cols, ld=None, old_logp=None, ref_logp=None, weight=None, scale=1.0,
@@ -391,19 +402,19 @@ def policy_loss(logits, labels, advantage, loss, rows, cols, ld=None, old_logp=N
                 workspace=None, workspace_bytes=0, stream=None):
     """Clipped policy loss with a KL term per row, their sum, and the sum's gradient with respect to the logits; workspace:
     token_logprob_workspace_bytes(rows, cols) bytes, or None."""
-    check(lib().ko_policy_loss_f32(_p(logits), cols if ld is None else ld, _p(labels), _p(old_logp), _p(ref_logp),
-                                   _p(advantage), _p(weight), scale, clip_low, clip_high, kl_coef, _p(logp), _p(kl), _p(loss),
-                                   _p(loss_sum), _p(dlogits), cols if ldd is None else ldd, rows, cols, _p(workspace),
-                                   workspace_bytes, _h(stream)))
+    check(lib().ko_policy_loss_f32(logits, cols if ld is None else ld, labels, old_logp, ref_logp,
+                                   advantage, weight, scale, clip_low, clip_high, kl_coef, logp, kl, loss,
+                                   loss_sum, dlogits, cols if ldd is None else ldd, rows, cols, workspace,
+                                   workspace_bytes, stream))
 
 
 def policy_loss16(logits, labels, advantage, loss, rows, cols, ld=None, old_logp=None, ref_logp=None, weight=None, scale=1.0,
                   clip_low=0.2, clip_high=0.2, kl_coef=0.0, logp=None, kl=None, loss_sum=None, dlogits=None, ldd=None,
                   dtype=F16, workspace=None, workspace_bytes=0, stream=None):
-    check(lib().ko_policy_loss_16(_p(logits), cols if ld is None else ld, _p(labels), _p(old_logp), _p(ref_logp),
-                                  _p(advantage), _p(weight), scale, clip_low, clip_high, kl_coef, _p(logp), _p(kl), _p(loss),
-                                  _p(loss_sum), _p(dlogits), cols if ldd is None else ldd, rows, cols, dtype, _p(workspace),
-                                  workspace_bytes, _h(stream)))
+    check(lib().ko_policy_loss_16(logits, cols if ld is None else ld, labels, old_logp, ref_logp,
+                                  advantage, weight, scale, clip_low, clip_high, kl_coef, logp, kl, loss,
+                                  loss_sum, dlogits, cols if ldd is None else ldd, rows, cols, dtype, workspace,
+                                  workspace_bytes, stream))
 
 
 def preference_loss(logp, ref_logp, offsets, pairs, tokens, pair_loss, labels=None, beta=0.1, label_smoothing=0.0,
@@ -412,8 +423,8 @@ def preference_loss(logp, ref_logp, offsets, pairs, tokens, pair_loss, labels=No
     respect to logp."""
     if pair_weight is None:
         pair_weight = 1.0 / max(1, pairs)
-    check(lib().ko_preference_loss_f32(_p(logp), _p(ref_logp), _p(labels), _p(offsets), pairs, tokens, beta, label_smoothing,
-                                       pair_weight, _p(pair_loss), _p(rewards), _p(dlogp), _p(loss_sum), _h(stream)))
+    check(lib().ko_preference_loss_f32(logp, ref_logp, labels, offsets, pairs, tokens, beta, label_smoothing,
+                                       pair_weight, pair_loss, rewards, dlogp, loss_sum, stream))
 
 
 def sgemm(m, n, k, A, B, D, C=None, alpha=1.0, beta=0.0, stream=None):

@@ -32,290 +32,342 @@ struct Args {
     int64_t rows;
     int cols;
     float inv_n, inv_d;
-    float *partial;  // [workgroups][2][cols], or null: dgamma and dbeta are left to the column kernel
+    float *partial;  // [row workgroups][2][cols], or null: dgamma and dbeta are left to others
     hipStream_t stream;
+    int row_groups;  // workgroups of the launch that walk over rows
 };
 
-// One row's (or one lane group's) loads.
+// dgamma and dbeta of a strip of COLUMNS columns alone, by a workgroup: THREADS / COLUMNS slices of the rows from `first` on, every
+// `step`-th row, side by side, then folded in order.  The sums come back in the first COLUMNS threads.
+template <int IO, int THREADS, int COLUMNS>
+__device__ __forceinline__ void column_strip(const Args<IO> &a, int strip, int64_t split, int64_t splits, float &sum_g, float &sum_b) {
+    constexpr int SLICES = THREADS / COLUMNS;
+    constexpr int UNROLL = 8;
+    __shared__ float sums[2][SLICES][COLUMNS + 1];
+    const int lane = threadIdx.x % COLUMNS;
+    const int slice = threadIdx.x / COLUMNS;
+    const int c = strip * COLUMNS + lane;
+    float sg = 0.0f, sb = 0.0f;
+    if (c < a.cols) {
+        const int64_t step = SLICES * splits;
+        for (int64_t row0 = SLICES * split + slice; row0 < a.rows; row0 += step * UNROLL) {
+            float d[UNROLL], xh[UNROLL];
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u) {
+                const int64_t row = row0 + u * step;
+                d[u] = xh[u] = 0.0f;
+                if (row < a.rows) {
+                    d[u] = Io<IO>::scalar(a.dy + row * a.cols + c);
+                    xh[u] = (Io<IO>::scalar(a.x + row * a.cols + c) - a.mean[row]) * a.rstd[row];
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u) {
+                sg = __builtin_fmaf(d[u], xh[u], sg);
+                sb += d[u];
+            }
+        }
+    }
+    sums[0][slice][lane] = sg;
+    sums[1][slice][lane] = sb;
+    __syncthreads();
+    sum_g = sum_b = 0.0f;
+    if (threadIdx.x >= COLUMNS) return;
+#pragma unroll 8
+    for (int i = 0; i < SLICES; ++i) {
+        sum_g += sums[0][i][lane];
+        sum_b += sums[1][i][lane];
+    }
+}
+
+// A strip over all rows, to the results: the few-rows form.
+constexpr int kStripColumns = 16;
+template <int IO, int THREADS>
+__device__ __forceinline__ void whole_strip(const Args<IO> &a, int strip) {
+    float sum_g, sum_b;
+    column_strip<IO, THREADS, kStripColumns>(a, strip, 0, 1, sum_g, sum_b);
+    const int c = strip * kStripColumns + threadIdx.x;
+    if (threadIdx.x < kStripColumns && c < a.cols) {
+        if (a.dgamma) a.dgamma[c] = sum_g;
+        if (a.dbeta) a.dbeta[c] = sum_b;
+    }
+}
+template <int IO, int THREADS>
+__global__ __launch_bounds__(THREADS) void layernorm_backward_strips_kernel(Args<IO> a) {
+    whole_strip<IO, THREADS>(a, blockIdx.x);
+}
+
+// One batch of rows as a thread loads it.
 template <int IO, int VPL, bool RES>
 struct RowLoads {
     typename Io<IO>::raw dy[VPL], x[VPL], res[RES ? VPL : 1];
     float mean, rstd;
 };
 
-// Where a workgroup's column sums go: its partial row, or the results themselves when it is the only one.
-__device__ __forceinline__ void put_column_sums(float *partial, float *dgamma, float *dbeta, int cols, int column, float sum_g,
-                                                float sum_b) {
-    if (gridDim.x == 1) {
-        if (dgamma) dgamma[column] = sum_g;
-        if (dbeta) dbeta[column] = sum_b;
-    } else {
-        float *mine = partial + static_cast<int64_t>(blockIdx.x) * 2 * cols;
-        mine[column] = sum_g;
-        mine[cols + column] = sum_b;
-    }
-}
+// Four floats at any address of a float.
+typedef float4v float4_any __attribute__((aligned(4)));
 
-// ---- a row in the registers of a group of LPR lanes, WAVES wavefronts per workgroup
+// ---- a row in registers: of LPR lanes of a wavefront (LPR <= 64, 64 / LPR rows per wavefront, kWaves wavefronts per
+// workgroup), or of a workgroup of LPR threads; VPL vectors per thread, VPL = ceil(vectors / LPR).
+// A wavefront or workgroup walks over batches of rows, one row per lane group.  The next batch's loads are issued before
+// the present one's arithmetic (up to 512 threads: a 1024-thread workgroup has 128 registers per thread, which the sums
+// and one row fill; it also converts what it loaded once for the sums and once more for dx), and nothing in the loop is loaded or stored under a condition (see load_whole):
+//   - threads beyond a row's last whole vector take the row's last 16 bytes again; they store what the others store
+//     there, and leave out of the sums the columns that they share with others (FULL: there are none);
+//   - lane groups beyond the last row take the last row again, which is in their own batch, likewise.
 constexpr int kWaves = 4;
-template <int IO, int LPR, int VPL, bool RES>
-__global__ __launch_bounds__(64 * kWaves) void layernorm_backward_wave_kernel(Args<IO> a) {
-    constexpr int E = Io<IO>::E;
-    constexpr int RPW = 64 / LPR;
-    typedef typename Io<IO>::elem Elem;
-    extern __shared__ float column_sums[];  // [2][cols]
-    const int lane = threadIdx.x & 63;
-    const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int sub = lane / LPR;
-    const int l = lane % LPR;
-    const int cols = a.cols;
-    const int nvec = cols / E;
-    const bool whole_lines = rows_are_whole_lines<IO>(cols);
-
-    typename Io<IO>::raw gamma[VPL];
-#pragma unroll
-    for (int k = 0; k < VPL; ++k) {
-        gamma[k] = typename Io<IO>::raw{};
-        if (a.gamma && l + k * LPR < nvec) gamma[k] = Io<IO>::template load_raw<false>(a.gamma + E * (l + k * LPR));
-    }
-    float acc_g[VPL][E], acc_b[VPL][E];
-#pragma unroll
-    for (int k = 0; k < VPL; ++k)
-#pragma unroll
-        for (int e = 0; e < E; ++e) acc_g[k][e] = acc_b[k][e] = 0.0f;
-
-    const uint32_t sub_off = static_cast<uint32_t>(sub) * static_cast<uint32_t>(cols) * sizeof(Elem);
-    auto fetch = [&](RowLoads<IO, VPL, RES> &r, int64_t row0) {
-        const int64_t row = row0 + sub;
-        const bool ok = row < a.rows;
-        const Elem *dy = a.dy + row0 * cols, *x = a.x + row0 * cols;
-        const Elem *res = RES ? a.dres + row0 * cols : nullptr;
-#pragma unroll
-        for (int k = 0; k < VPL; ++k) {
-            const int j = l + k * LPR;
-            r.dy[k] = r.x[k] = typename Io<IO>::raw{};
-            if constexpr (RES) r.res[k] = typename Io<IO>::raw{};
-            if (ok && j < nvec) {
-                const uint32_t at = sub_off + Io<IO>::kBytes * j;
-                r.dy[k] = Io<IO>::template load_raw<true>(byte_offset(dy, at));
-                r.x[k] = Io<IO>::template load_raw<true>(byte_offset(x, at));
-                if constexpr (RES) r.res[k] = Io<IO>::template load_raw<true>(byte_offset(res, at));
-            }
-        }
-        r.mean = ok ? a.mean[row] : 0.0f;
-        r.rstd = ok ? a.rstd[row] : 0.0f;
-    };
-
-    const int64_t stride = static_cast<int64_t>(gridDim.x) * kWaves * RPW;
-    int64_t row0 = (static_cast<int64_t>(blockIdx.x) * kWaves + wv) * RPW;
-    RowLoads<IO, VPL, RES> cur;
-    fetch(cur, row0);
-    for (; row0 < a.rows; row0 += stride) {
-        RowLoads<IO, VPL, RES> next;
-        fetch(next, row0 + stride);
-        float xh[VPL][E], g[VPL][E];
-        float s1 = 0.0f, s2 = 0.0f;
-#pragma unroll
-        for (int k = 0; k < VPL; ++k) {
-            float w[E];
-            Io<IO>::unpack(cur.x[k], xh[k]);
-            Io<IO>::unpack(cur.dy[k], g[k]);
-            Io<IO>::unpack(gamma[k], w);
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                xh[k][e] = (xh[k][e] - cur.mean) * cur.rstd;
-                acc_g[k][e] = __builtin_fmaf(g[k][e], xh[k][e], acc_g[k][e]);
-                acc_b[k][e] += g[k][e];
-                if (a.gamma) g[k][e] *= w[e];
-                s1 += g[k][e];
-                s2 = __builtin_fmaf(g[k][e], xh[k][e], s2);
-            }
-        }
-        s1 = wave::allreduce<LPR, wave::Sum>(s1) * a.inv_n;
-        s2 = wave::allreduce<LPR, wave::Sum>(s2) * a.inv_d;
-        Elem *dst0 = a.dx + row0 * cols;
-        const bool ok = row0 + sub < a.rows;
-#pragma unroll
-        for (int k = 0; k < VPL; ++k) {
-            const int j = l + k * LPR;
-            if (ok && j < nvec) {
-                float o[E], res[E];
-                if constexpr (RES) Io<IO>::unpack(cur.res[k], res);
-#pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    o[e] = cur.rstd * __builtin_fmaf(-xh[k][e], s2, g[k][e] - s1);
-                    if constexpr (RES) o[e] += res[e];
-                }
-                store_row_vec<IO>(whole_lines, dst0, sub_off + Io<IO>::kBytes * j, o);
-            }
-        }
-        cur = next;
-    }
-    if (!a.partial && !(gridDim.x == 1 && (a.dgamma || a.dbeta))) return;
-
-    // the lane groups' sums, then the wavefronts' in wave order
-#pragma unroll
-    for (int k = 0; k < VPL; ++k)
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-#pragma unroll
-            for (int step = LPR; step < 64; step <<= 1) {
-                acc_g[k][e] += __shfl_xor(acc_g[k][e], step, 64);
-                acc_b[k][e] += __shfl_xor(acc_b[k][e], step, 64);
-            }
-        }
-    for (int w = 0; w < kWaves; ++w) {
-        if (w == wv && sub == 0) {
-#pragma unroll
-            for (int k = 0; k < VPL; ++k) {
-                const int j = l + k * LPR;
-                if (j < nvec) {
-#pragma unroll
-                    for (int e = 0; e < E; ++e) {
-                        float *at = column_sums + E * j + e;
-                        at[0] = w == 0 ? acc_g[k][e] : at[0] + acc_g[k][e];
-                        at[cols] = w == 0 ? acc_b[k][e] : at[cols] + acc_b[k][e];
-                    }
-                }
-            }
-        }
-        __syncthreads();
-    }
-    for (int c = threadIdx.x; c < cols; c += 64 * kWaves)
-        put_column_sums(a.partial, a.dgamma, a.dbeta, cols, c, column_sums[c], column_sums[cols + c]);
+template <int LPR>
+constexpr int group_threads() {
+    return LPR > 64 ? LPR : 64 * kWaves;
 }
-
-// ---- a row in the registers of a workgroup.  AHEAD: the next row's loads are issued before this row's arithmetic
-// (up to 512 threads; a 1024-thread workgroup has 128 registers per thread, which the sums and one row fill - it also
-// converts what it loaded once for the sums and once more for dx).
-template <int IO, int THREADS, int VPL, bool RES, bool AHEAD>
-__global__ __launch_bounds__(THREADS) void layernorm_backward_block_kernel(Args<IO> a) {
+template <int IO, int LPR, int VPL, bool RES, bool FULL>
+__global__ __launch_bounds__(group_threads<LPR>(), LPR == 1024 ? 4 : LPR <= 64 && VPL * Io<IO>::E >= 24 ? 1 : 2) void layernorm_backward_rows_kernel(Args<IO> a) {
     constexpr int E = Io<IO>::E;
+    constexpr int THREADS = group_threads<LPR>();
+    constexpr bool BLOCK = LPR > 64;       // a workgroup per row
+    constexpr bool AHEAD = LPR < 1024;
+    constexpr int RPB = BLOCK ? 1 : 64 / LPR;  // rows per batch
     typedef typename Io<IO>::elem Elem;
+    typedef RowLoads<IO, VPL, RES> Loads;
     __shared__ float slots[2][THREADS / 64][2];
+    const int wv = BLOCK ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int sub = BLOCK ? 0 : (threadIdx.x & 63) / LPR;
+    const int l = threadIdx.x % LPR;
     const int cols = a.cols;
-    const int nvec = cols / E;
-    const bool whole_lines = rows_are_whole_lines<IO>(cols);
+    if (static_cast<int>(blockIdx.x) >= a.row_groups) {
+        // few rows: dgamma and dbeta by workgroups of their own in the same launch (see launch_rows)
+        whole_strip<IO, THREADS>(a, static_cast<int>(blockIdx.x) - a.row_groups);
+        return;
+    }
+    const uint32_t row_bytes = static_cast<uint32_t>(cols) * sizeof(Elem);
+
+    // vector k of this thread starts `vec_at(k)` bytes into its row; the last one's first `seen` columns are another
+    // thread's, too
+    uint32_t last_at = Io<IO>::kBytes * (l + (VPL - 1) * LPR);
+    int seen = 0;
+    if constexpr (!FULL) {
+        const uint32_t most = row_bytes - Io<IO>::kBytes;
+        if (last_at > most) {
+            const uint32_t past = (last_at - most) / sizeof(Elem);
+            seen = past < E ? static_cast<int>(past) : E;
+            last_at = most;
+        }
+    }
+    auto vec_at = [&](int k) { return k + 1 < VPL ? Io<IO>::kBytes * static_cast<uint32_t>(l + k * LPR) : last_at; };
 
     typename Io<IO>::raw gamma[VPL];
+    float one[E];
 #pragma unroll
-    for (int k = 0; k < VPL; ++k) {
-        const int j = threadIdx.x + k * THREADS;
-        gamma[k] = typename Io<IO>::raw{};
-        if (a.gamma && j < nvec) gamma[k] = Io<IO>::template load_raw<false>(a.gamma + E * j);
-    }
+    for (int e = 0; e < E; ++e) one[e] = 1.0f;
+#pragma unroll
+    for (int k = 0; k < VPL; ++k) gamma[k] = a.gamma ? load_whole<IO, FULL>(a.gamma, vec_at(k)) : pack<IO>(one);
     float acc_g[VPL][E], acc_b[VPL][E];
 #pragma unroll
     for (int k = 0; k < VPL; ++k)
 #pragma unroll
         for (int e = 0; e < E; ++e) acc_g[k][e] = acc_b[k][e] = 0.0f;
 
-    auto fetch = [&](RowLoads<IO, VPL, RES> &r, int64_t row) {
-        const bool ok = row < a.rows;
-        const Elem *dy = a.dy + row * cols, *x = a.x + row * cols;
-        const Elem *res = RES ? a.dres + row * cols : nullptr;
-#pragma unroll
-        for (int k = 0; k < VPL; ++k) {
-            const int j = threadIdx.x + k * THREADS;
-            r.dy[k] = r.x[k] = typename Io<IO>::raw{};
-            if constexpr (RES) r.res[k] = typename Io<IO>::raw{};
-            if (ok && j < nvec) {
-                const uint32_t at = Io<IO>::kBytes * j;
-                r.dy[k] = Io<IO>::template load_raw<true>(byte_offset(dy, at));
-                r.x[k] = Io<IO>::template load_raw<true>(byte_offset(x, at));
-                if constexpr (RES) r.res[k] = Io<IO>::template load_raw<true>(byte_offset(res, at));
-            }
-        }
-        r.mean = ok ? a.mean[row] : 0.0f;
-        r.rstd = ok ? a.rstd[row] : 0.0f;
+    // batch t of this walker
+    const int64_t walkers = BLOCK ? a.row_groups : static_cast<int64_t>(a.row_groups) * kWaves;
+    const int64_t first = BLOCK ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * kWaves + wv;
+    const int64_t batches = (a.rows + RPB - 1) / RPB;
+    const int64_t n = first < batches ? (batches - first + walkers - 1) / walkers : 0;
+    auto row_of = [&](int64_t t) { return (first + t * walkers) * RPB; };
+    // the lane group's row within the batch at row0, the last row's batch having fewer
+    auto row_in_batch = [&](int64_t row0) {
+        const int64_t left = a.rows - row0;
+        return RPB > 1 && left < RPB && sub >= left ? static_cast<int>(left) - 1 : sub;
     };
 
-    int64_t row = blockIdx.x;
-    int turn = 0;
-    RowLoads<IO, VPL, RES> cur;
-    if constexpr (AHEAD) fetch(cur, row);
-    for (; row < a.rows; row += gridDim.x, turn ^= 1) {
-        RowLoads<IO, VPL, RES> next;
-        if constexpr (AHEAD) fetch(next, row + gridDim.x);
-        else fetch(cur, row);
+    auto fetch = [&](Loads &r, int64_t t) {
+        const int64_t row0 = row_of(t);
+        const int in_batch = row_in_batch(row0);
+        const Elem *dy = a.dy + row0 * cols, *x = a.x + row0 * cols, *res = RES ? a.dres + row0 * cols : nullptr;
+        const uint32_t at = static_cast<uint32_t>(in_batch) * row_bytes;
+#pragma unroll
+        for (int k = 0; k < VPL; ++k) {
+            r.dy[k] = load_whole<IO, FULL>(dy, at + vec_at(k));
+            r.x[k] = load_whole<IO, FULL>(x, at + vec_at(k));
+            if constexpr (RES) r.res[k] = load_whole<IO, FULL>(res, at + vec_at(k));
+        }
+        r.mean = a.mean[row0 + in_batch];
+        r.rstd = a.rstd[row0 + in_batch];
+        asm volatile("" ::: "memory");  // the loads stay ahead of what follows
+    };
+
+    // LAST: the batch may be the one with lane groups beyond the last row
+    // One vector converted: xh and g = dy; then, the column sums taken of them, g times gamma.
+    auto convert = [&](const Loads &cur, int k, float (&xh)[E], float (&g)[E]) {
+        Io<IO>::unpack(cur.x[k], xh);
+        Io<IO>::unpack(cur.dy[k], g);
+#pragma unroll
+        for (int e = 0; e < E; ++e) xh[e] = (xh[e] - cur.mean) * cur.rstd;
+    };
+    auto times_gamma = [&](int k, float (&g)[E]) {
+        if constexpr (!AHEAD) convert_again<IO>(gamma[k]);
+        float w[E];
+        Io<IO>::unpack(gamma[k], w);
+#pragma unroll
+        for (int e = 0; e < E; ++e) g[e] *= w[e];
+    };
+    auto finish = [&](Loads &cur, int64_t t, auto last) {
+        constexpr bool LAST = decltype(last)::value && RPB > 1;
+        const int64_t row0 = row_of(t);
+        const int in_batch = LAST ? row_in_batch(row0) : sub;
+        if constexpr (AHEAD) {
+            // what this batch loaded is looked at from here on only: conversions moved up between the next batch's
+            // addresses would have the wavefront wait for this batch before it asks for the next one
+#pragma unroll
+            for (int k = 0; k < VPL; ++k) asm volatile("" : "+v"(cur.dy[k]), "+v"(cur.x[k]));
+        }
         float xh[AHEAD ? VPL : 1][E], g[AHEAD ? VPL : 1][E];
-        auto convert = [&](int k, float (&xk)[E], float (&gk)[E]) {
-            Io<IO>::unpack(cur.x[k], xk);
-            Io<IO>::unpack(cur.dy[k], gk);
-#pragma unroll
-            for (int e = 0; e < E; ++e) xk[e] = (xk[e] - cur.mean) * cur.rstd;
-        };
-        auto times_gamma = [&](int k, float (&gk)[E]) {
-            if (!a.gamma) return;
-            float w[E];
-            Io<IO>::unpack(gamma[k], w);
-#pragma unroll
-            for (int e = 0; e < E; ++e) gk[e] *= w[e];
-        };
         float s[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int k = 0; k < VPL; ++k) {
             float(&xk)[E] = xh[AHEAD ? k : 0], (&gk)[E] = g[AHEAD ? k : 0];
-            convert(k, xk, gk);
+            convert(cur, k, xk, gk);
+            float up[E];  // dy of the columns that this thread counts
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                acc_g[k][e] = __builtin_fmaf(gk[e], xk[e], acc_g[k][e]);
-                acc_b[k][e] += gk[e];
+                up[e] = gk[e];
+                if constexpr (!FULL) {
+                    if (k + 1 == VPL) up[e] = e >= seen ? up[e] : 0.0f;
+                }
+                if constexpr (LAST) up[e] = in_batch == sub ? up[e] : 0.0f;
+                acc_g[k][e] = __builtin_fmaf(up[e], xk[e], acc_g[k][e]);
+                acc_b[k][e] += up[e];
             }
             times_gamma(k, gk);
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                s[0] += gk[e];
-                s[1] = __builtin_fmaf(gk[e], xk[e], s[1]);
+                float gs = gk[e];
+                if constexpr (!FULL) {
+                    if (k + 1 == VPL) gs = e >= seen ? gs : 0.0f;
+                }
+                s[0] += gs;
+                s[1] = __builtin_fmaf(gs, xk[e], s[1]);
             }
         }
-        block_sum<THREADS / 64, 2>(s, slots[turn]);
+        if constexpr (BLOCK) {
+            block_sum<THREADS / 64, 2>(s, slots[t & 1]);
+        } else {
+            s[0] = wave::allreduce<LPR, wave::Sum>(s[0]);
+            s[1] = wave::allreduce<LPR, wave::Sum>(s[1]);
+        }
         const float s1 = s[0] * a.inv_n, s2 = s[1] * a.inv_d;
-        Elem *dst = a.dx + row * cols;
+        Elem *dx = a.dx + row0 * cols;
+        const uint32_t at = static_cast<uint32_t>(in_batch) * row_bytes;
 #pragma unroll
         for (int k = 0; k < VPL; ++k) {
-            const int j = threadIdx.x + k * THREADS;
-            if (j < nvec) {
-                float o[E], res[E];
-                float(&xk)[E] = xh[AHEAD ? k : 0], (&gk)[E] = g[AHEAD ? k : 0];
-                if constexpr (!AHEAD) {
-                    convert_again<IO>(cur.x[k]);
-                    convert_again<IO>(cur.dy[k]);
-                    convert(k, xk, gk);
-                    times_gamma(k, gk);
-                }
-                if constexpr (RES) Io<IO>::unpack(cur.res[k], res);
+            float o[E], res[E];
+            float(&xk)[E] = xh[AHEAD ? k : 0], (&gk)[E] = g[AHEAD ? k : 0];
+            if constexpr (!AHEAD) {
+                convert_again<IO>(cur.x[k]);
+                convert_again<IO>(cur.dy[k]);
+                convert(cur, k, xk, gk);
+                times_gamma(k, gk);
+            }
+            if constexpr (RES) Io<IO>::unpack(cur.res[k], res);
 #pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    o[e] = cur.rstd * __builtin_fmaf(-xk[e], s2, gk[e] - s1);
-                    if constexpr (RES) o[e] += res[e];
-                }
-                store_row_vec<IO>(whole_lines, dst, Io<IO>::kBytes * j, o);
+            for (int e = 0; e < E; ++e) {
+                o[e] = cur.rstd * __builtin_fmaf(-xk[e], s2, gk[e] - s1);
+                if constexpr (RES) o[e] += res[e];
+            }
+            store_whole<IO, FULL>(dx, at + vec_at(k), o);
+        }
+    };
+    typedef std::integral_constant<bool, false> Whole;
+    typedef std::integral_constant<bool, true> Last;
+
+    // Two sets of registers in turn (moving one into the other would wait for its loads).  The loop is entered the way
+    // it comes round, with one set's loads and the other's stores on their way, so that its waits can be exact.
+    if constexpr (!AHEAD) {
+        Loads only;
+        for (int64_t t = 0; t < n; ++t) {
+            fetch(only, t);
+            finish(only, t, Whole{});
+        }
+    } else if (n > 0) {
+        Loads even, odd;
+        int64_t t = 0;
+        fetch(even, 0);
+        if (n > 1) {
+            fetch(odd, 1);
+            finish(even, 0, Whole{});
+            for (t = 1; t + 2 < n; t += 2) {
+                fetch(even, t + 1);
+                finish(odd, t, Whole{});
+                fetch(odd, t + 2);
+                finish(even, t + 1, Whole{});
+            }
+            if (t + 1 < n) {
+                fetch(even, t + 1);
+                finish(odd, t, Whole{});
+                ++t;
+            } else {
+                even = odd;
             }
         }
-        if constexpr (AHEAD) cur = next;
+        finish(even, t, Last{});
     }
-    if (!a.partial && !(gridDim.x == 1 && (a.dgamma || a.dbeta))) return;
+    // Where this workgroup's column sums go: its partial row, or the results themselves when it is the only one.
+    float *to_g = a.dgamma, *to_b = a.dbeta;
+    if (a.row_groups > 1) {
+        if (!a.partial) return;
+        to_g = a.partial + static_cast<int64_t>(blockIdx.x) * 2 * cols;
+        to_b = to_g + cols;
+    } else if (!to_g && !to_b) {
+        return;
+    }
+    // the columns of vector k that this thread counts, at base + column
+    auto put = [&](float *base, int k, const float (&v)[E]) {
+        float *at = base + vec_at(k) / sizeof(Elem);
+        if (FULL || k + 1 < VPL || seen == 0) {
 #pragma unroll
-    for (int k = 0; k < VPL; ++k) {
-        const int j = threadIdx.x + k * THREADS;
-        if (j < nvec) {
+            for (int e = 0; e < E; e += 4)
+                *reinterpret_cast<float4_any *>(at + e) = float4v{v[e], v[e + 1], v[e + 2], v[e + 3]};
+        } else {
 #pragma unroll
             for (int e = 0; e < E; ++e)
-                put_column_sums(a.partial, a.dgamma, a.dbeta, cols, E * j + e, acc_g[k][e], acc_b[k][e]);
+                if (e >= seen) at[e] = v[e];
+        }
+    };
+    if constexpr (BLOCK) {
+#pragma unroll
+        for (int k = 0; k < VPL; ++k) {
+            if (to_g) put(to_g, k, acc_g[k]);
+            if (to_b) put(to_b, k, acc_b[k]);
+        }
+    } else {
+        // every lane group's sums side by side in LDS, then added in order, column by column
+        constexpr int GROUPS = kWaves * RPB;
+        extern __shared__ float column_sums[];  // [GROUPS][2][cols]
+        float *mine = column_sums + (wv * RPB + sub) * 2 * cols;
+#pragma unroll
+        for (int k = 0; k < VPL; ++k) {
+            put(mine, k, acc_g[k]);
+            put(mine + cols, k, acc_b[k]);
+        }
+        __syncthreads();
+        for (int c = threadIdx.x; c < 2 * cols; c += THREADS) {
+            float sum = 0.0f;
+#pragma unroll 8
+            for (int i = 0; i < GROUPS; ++i) sum += column_sums[i * 2 * cols + c];
+            float *to = c < cols ? to_g : to_b;
+            if (to) to[c < cols ? c : c - cols] = sum;
         }
     }
 }
 
 // ---- rows of any length: the sums first, then a second read; no share of dgamma and dbeta (the column kernel's)
-template <int IO, int THREADS>
+template <int IO, int THREADS, bool RAGGED>
 __global__ __launch_bounds__(THREADS) void layernorm_backward_reread_kernel(Args<IO> a) {
     constexpr int E = Io<IO>::E;
-    constexpr int UNROLL = E == 1 ? 4 : 2;
+    constexpr int UNROLL = 2;
     typedef typename Io<IO>::elem Elem;
     __shared__ float slots[2][THREADS / 64][2];
     const int cols = a.cols;
-    const int nvec = cols / E;
+    const int nvec = row_vectors<IO, RAGGED>(cols);
     const bool whole_lines = rows_are_whole_lines<IO>(cols);
     int turn = 0;
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
@@ -326,12 +378,12 @@ __global__ __launch_bounds__(THREADS) void layernorm_backward_reread_kernel(Args
                 typename Io<IO>::raw rd[UNROLL], rx[UNROLL], rg[UNROLL];
 #pragma unroll
                 for (int u = 0; u < UNROLL; ++u) {
-                    const int64_t j = j0 + u * THREADS;
+                    const int j = j0 + u * THREADS;
                     rd[u] = rx[u] = rg[u] = typename Io<IO>::raw{};
                     if (j < nvec) {
-                        rd[u] = Io<IO>::template load_raw<false>(dy + E * j);
-                        rx[u] = Io<IO>::template load_raw<false>(x + E * j);
-                        if (a.gamma) rg[u] = Io<IO>::template load_raw<false>(a.gamma + E * j);
+                        rd[u] = load_row_vec<IO, RAGGED, false>(dy, 0, j, cols);
+                        rx[u] = load_row_vec<IO, RAGGED, false>(x, 0, j, cols);
+                        if (a.gamma) rg[u] = load_row_vec<IO, RAGGED, false>(a.gamma, 0, j, cols);
                     }
                 }
 #pragma unroll
@@ -363,52 +415,24 @@ __global__ __launch_bounds__(THREADS) void layernorm_backward_reread_kernel(Args
         sweep([&](int j, float (&g)[E], float (&xh)[E]) {
             if (j >= nvec) return;
             float res[E];
-            if (a.dres) Io<IO>::template load<true>(a.dres + row * cols + static_cast<int64_t>(E) * j, res);
+            if (a.dres) Io<IO>::unpack(load_row_vec<IO, RAGGED, true>(a.dres + row * cols, 0, j, cols), res);
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 g[e] = rstd * __builtin_fmaf(-xh[e], s2, g[e] - s1);
                 if (a.dres) g[e] += res[e];
             }
-            store_row_vec<IO>(whole_lines, dst, Io<IO>::kBytes * static_cast<uint32_t>(j), g);
+            store_row_vec_any<IO, RAGGED>(whole_lines, dst, 0, j, cols, g);
         });
     }
 }
 
-// ---- dgamma and dbeta alone: workgroup (strip, split) sums 64 columns over every gridDim.y-th group of four rows
+// ---- dgamma and dbeta alone: workgroup (strip, split) takes 64 columns and every gridDim.y-th group of rows
 template <int IO>
 __global__ __launch_bounds__(256) void layernorm_backward_columns_kernel(Args<IO> a) {
-    __shared__ float sums[2][4][64];
-    const int lane = threadIdx.x & 63;
-    const int slice = threadIdx.x >> 6;
-    const int c = static_cast<int>(blockIdx.x) * 64 + lane;
-    float sg = 0.0f, sb = 0.0f;
-    if (c < a.cols) {
-        constexpr int UNROLL = 4;
-        const int64_t step = int64_t{4} * gridDim.y;
-        for (int64_t row0 = int64_t{4} * blockIdx.y + slice; row0 < a.rows; row0 += step * UNROLL) {
-            float d[UNROLL], xh[UNROLL];
-#pragma unroll
-            for (int u = 0; u < UNROLL; ++u) {
-                const int64_t row = row0 + u * step;
-                d[u] = xh[u] = 0.0f;
-                if (row < a.rows) {
-                    d[u] = Io<IO>::scalar(a.dy + row * a.cols + c);
-                    xh[u] = (Io<IO>::scalar(a.x + row * a.cols + c) - a.mean[row]) * a.rstd[row];
-                }
-            }
-#pragma unroll
-            for (int u = 0; u < UNROLL; ++u) {
-                sg = __builtin_fmaf(d[u], xh[u], sg);
-                sb += d[u];
-            }
-        }
-    }
-    sums[0][slice][lane] = sg;
-    sums[1][slice][lane] = sb;
-    __syncthreads();
-    if (slice != 0 || c >= a.cols) return;
-    sg = (sums[0][0][lane] + sums[0][1][lane]) + (sums[0][2][lane] + sums[0][3][lane]);
-    sb = (sums[1][0][lane] + sums[1][1][lane]) + (sums[1][2][lane] + sums[1][3][lane]);
+    float sg, sb;
+    column_strip<IO, 256, 64>(a, blockIdx.x, blockIdx.y, gridDim.y, sg, sb);
+    const int c = static_cast<int>(blockIdx.x) * 64 + threadIdx.x;
+    if (threadIdx.x >= 64 || c >= a.cols) return;
     if (gridDim.y == 1) {
         if (a.dgamma) a.dgamma[c] = sg;
         if (a.dbeta) a.dbeta[c] = sb;
@@ -430,7 +454,14 @@ __global__ __launch_bounds__(1024) void layernorm_backward_reduce_kernel(const f
     const int64_t c = int64_t{16} * blockIdx.x + lane;
     float s = 0.0f;
     if (c < width) {
-        for (int p = slice; p < groups; p += 64) s += partial[p * width + c];
+        constexpr int UNROLL = 4;
+        for (int p0 = slice; p0 < groups; p0 += 64 * UNROLL) {
+            float v[UNROLL];
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u) v[u] = p0 + 64 * u < groups ? partial[(p0 + 64 * u) * width + c] : 0.0f;
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u) s += v[u];
+        }
     }
     sums[slice][lane] = s;
     __syncthreads();
@@ -457,9 +488,18 @@ __global__ __launch_bounds__(256) void layernorm_backward_zero_kernel(float *dga
 // ---------------------------------------------------------------------------------------------------- dispatch
 // Workgroups that walk over the rows, at most: a function of the sizes alone, so that the workspace can be sized
 // without a device.
-int64_t max_groups(int64_t rows, int64_t cols) {
-    const int64_t most = cols <= 2048 ? 768 : 512;
-    return rows < most ? rows : most;
+constexpr int64_t kUnits = 256;  // compute units of an MI355X
+constexpr int64_t kFewRows = 256;
+constexpr int64_t kMostColumns = 16384;  // of a row that a workgroup's registers hold
+int64_t max_groups(int64_t rows) {
+    return rows < 2 * kUnits ? rows : 2 * kUnits;
+}
+// Groups of rows that the column kernel takes side by side: some 2048 workgroups in all, sixteen rows and more each.
+int64_t column_splits(int64_t rows, int64_t cols) {
+    int64_t splits = 2048 / ((cols + 63) / 64);
+    if (splits > (rows + 15) / 16) splits = (rows + 15) / 16;
+    if (splits > max_groups(rows)) splits = max_groups(rows);
+    return splits < 1 ? 1 : splits;
 }
 
 // `batches` of rows over at most `most` workgroups, as evenly as whole trips allow.
@@ -483,13 +523,7 @@ template <int IO>
 int launch_columns(const Args<IO> &a) {
     if (!a.dgamma && !a.dbeta) return KO_OK;
     const int64_t strips = (a.cols + 63) / 64;
-    int64_t splits = 1;
-    if (a.partial) {
-        splits = 2048 / strips;
-        if (splits > (a.rows + 15) / 16) splits = (a.rows + 15) / 16;
-        if (splits > max_groups(a.rows, a.cols)) splits = max_groups(a.rows, a.cols);
-        if (splits < 1) splits = 1;
-    }
+    const int64_t splits = a.partial ? column_splits(a.rows, a.cols) : 1;
     layernorm_backward_columns_kernel<IO><<<dim3(static_cast<unsigned>(strips), static_cast<unsigned>(splits)), dim3(256), 0,
                                             a.stream>>>(a);
     KO_CHECK_LAUNCH();
@@ -507,77 +541,84 @@ int reduce_last(const Args<IO> &a, int64_t grid) {
     return grid > 1 && a.partial ? launch_reduce(a, grid) : KO_OK;
 }
 
+template <int IO, int LPR, int VPL, bool FULL>
+int launch_rows(Args<IO> a) {
+    constexpr int THREADS = group_threads<LPR>();
+    constexpr int64_t kRows = LPR > 64 ? 1 : kWaves * (64 / LPR);  // per workgroup and trip
+    // One workgroup per compute unit: with the next batch's loads always on their way, more of them only spread the
+    // addresses in flight (65536 x 4096 bf16 with dres: one 363 us, two 388, three 414).  Two where a workgroup's batch is
+    // 8 KB or less (98304 x 1024 fp32: one 5.4 TB/s, two 5.9).
+    const bool light = THREADS * VPL * 16 * (a.dres ? 3 : 2) <= 8192;
+    const int64_t grid = even_grid((a.rows + kRows - 1) / kRows, light ? 2 * kUnits : kUnits);
+    a.row_groups = static_cast<int>(grid);
+    // Few rows: no second launch.  Workgroups of the same launch read the rows once more, from the caches, for dgamma and
+    // dbeta (in a graph, 128 x 768 fp32 5.8 -> 3.2 us, 256 x 4096 bf16 13.1 -> 5.2, 256 x 128 bf16 5.1 -> 4.5; at 512 rows 7.5
+    // against 7.4, 13.9 against 14.8 and 5.1 against 7.1).  Where dx overwrites what they read, they come first, in a launch of
+    // their own, which gives the same bits.
+    int strips = 0;
+    if ((a.dgamma || a.dbeta) && grid > 1 && a.rows <= kFewRows) {
+        a.partial = nullptr;
+        strips = (a.cols + kStripColumns - 1) / kStripColumns;
+        if (a.dx == a.dy || a.dx == a.x) {
+            layernorm_backward_strips_kernel<IO, THREADS><<<dim3(static_cast<unsigned>(strips)), dim3(THREADS), 0, a.stream>>>(a);
+            KO_CHECK_LAUNCH();
+            strips = 0;
+        }
+    } else if (const int st = columns_first(a, grid); st != KO_OK) {
+        return st;
+    }
+    const size_t lds = LPR > 64 ? 0 : static_cast<size_t>(kRows) * 2 * a.cols * sizeof(float);  // 48 KB at most
+    const dim3 g(static_cast<unsigned>(grid + strips)), b(THREADS);
+    if (a.dres) layernorm_backward_rows_kernel<IO, LPR, VPL, true, FULL><<<g, b, lds, a.stream>>>(a);
+    else layernorm_backward_rows_kernel<IO, LPR, VPL, false, FULL><<<g, b, lds, a.stream>>>(a);
+    KO_CHECK_LAUNCH();
+    return reduce_last(a, grid);
+}
+
 template <int IO, int LPR, int VPL>
-int launch_wave(const Args<IO> &a) {
-    constexpr int64_t kRows = kWaves * (64 / LPR);
-    const int64_t grid = even_grid((a.rows + kRows - 1) / kRows, max_groups(a.rows, a.cols));
-    if (const int st = columns_first(a, grid); st != KO_OK) return st;
-    const size_t lds = static_cast<size_t>(2) * a.cols * sizeof(float);
-    const dim3 g(static_cast<unsigned>(grid)), b(64 * kWaves);
-    if (a.dres) layernorm_backward_wave_kernel<IO, LPR, VPL, true><<<g, b, lds, a.stream>>>(a);
-    else layernorm_backward_wave_kernel<IO, LPR, VPL, false><<<g, b, lds, a.stream>>>(a);
-    KO_CHECK_LAUNCH();
-    return reduce_last(a, grid);
+int launch_rows_any(const Args<IO> &a, bool whole) {
+    if (whole && a.cols == LPR * VPL * Io<IO>::E) return launch_rows<IO, LPR, VPL, true>(a);
+    return launch_rows<IO, LPR, VPL, false>(a);
 }
 
-template <int IO, int THREADS, int VPL>
-int launch_block(const Args<IO> &a) {
-    constexpr bool kAhead = THREADS < 1024;
-    const int64_t grid = even_grid(a.rows, max_groups(a.rows, a.cols));
-    if (const int st = columns_first(a, grid); st != KO_OK) return st;
-    const dim3 g(static_cast<unsigned>(grid)), b(THREADS);
-    if (a.dres) layernorm_backward_block_kernel<IO, THREADS, VPL, true, kAhead><<<g, b, 0, a.stream>>>(a);
-    else layernorm_backward_block_kernel<IO, THREADS, VPL, false, kAhead><<<g, b, 0, a.stream>>>(a);
-    KO_CHECK_LAUNCH();
-    return reduce_last(a, grid);
-}
-
-template <int IO>
+template <int IO, int THREADS, bool RAGGED>
 int launch_long(const Args<IO> &a) {
     if (const int st = launch_columns(a); st != KO_OK) return st;  // (dx may overwrite dy or x)
     const int64_t grid = a.rows > 0x7fffffff ? 0x7fffffff : a.rows;
-    layernorm_backward_reread_kernel<IO, 1024><<<dim3(static_cast<unsigned>(grid)), dim3(1024), 0, a.stream>>>(a);
+    layernorm_backward_reread_kernel<IO, THREADS, RAGGED><<<dim3(static_cast<unsigned>(grid)), dim3(THREADS), 0, a.stream>>>(a);
     KO_CHECK_LAUNCH();
     return KO_OK;
 }
 
+// `whole`: rows of whole 16-byte vectors on 16-byte boundaries
 template <int IO>
-int dispatch(const Args<IO> &a) {
-    constexpr int E = Io<IO>::E;
-    const int nvec = a.cols / E;
-    if constexpr (E == 1) {
-        if (nvec <= 16) return launch_wave<IO, 16, 1>(a);
-        if (nvec <= 64) return launch_wave<IO, 64, 1>(a);
-        if (nvec <= 128) return launch_wave<IO, 64, 2>(a);
-        if (nvec <= 256) return launch_wave<IO, 64, 4>(a);
-        if (nvec <= 512) return launch_wave<IO, 64, 8>(a);
-        if (nvec <= 1024) return launch_wave<IO, 64, 16>(a);
-        if (nvec <= 2048) return launch_block<IO, 512, 4>(a);
-        if (nvec <= 4096) return launch_block<IO, 512, 8>(a);
-        if (nvec <= 8192) return launch_block<IO, 1024, 8>(a);
-    } else {
-        int lpr = 0, vpl = 0;
-        if (choose_row_group(nvec, 4, &lpr, &vpl)) {
-#define KO_WAVE(L, V) if (lpr == L && vpl == V) return launch_wave<IO, L, V>(a)
-            KO_WAVE(8, 1); KO_WAVE(8, 2); KO_WAVE(8, 3);
-            KO_WAVE(16, 1); KO_WAVE(16, 2); KO_WAVE(16, 3);
-            KO_WAVE(32, 1); KO_WAVE(32, 2); KO_WAVE(32, 3);
-            KO_WAVE(64, 1); KO_WAVE(64, 2); KO_WAVE(64, 3); KO_WAVE(64, 4);
+int dispatch(const Args<IO> &a, bool whole) {
+    const int nvec = (a.cols + Io<IO>::E - 1) / Io<IO>::E;
+    if (a.cols < Io<IO>::E) return launch_long<IO, 64, true>(a);  // (shorter than a vector)
+    int lpr = 0, vpl = 0;
+    if (choose_row_group(nvec, 3, &lpr, &vpl)) {
+#define KO_WAVE(L, V) if (lpr == L && vpl == V) return launch_rows_any<IO, L, V>(a, whole)
+        KO_WAVE(8, 1); KO_WAVE(8, 2); KO_WAVE(8, 3);
+        KO_WAVE(16, 1); KO_WAVE(16, 2); KO_WAVE(16, 3);
+        KO_WAVE(32, 1); KO_WAVE(32, 2); KO_WAVE(32, 3);
+        KO_WAVE(64, 1); KO_WAVE(64, 2); KO_WAVE(64, 3);
 #undef KO_WAVE
-        }
-        if (nvec <= 512) return launch_block<IO, 256, 2>(a);
-        if (nvec <= 1024) return launch_block<IO, 512, 2>(a);
-        if (nvec <= 2048) return launch_block<IO, 1024, 2>(a);
-        if constexpr (E == 4) {
-            if (nvec <= 4096) return launch_block<IO, 1024, 4>(a);
-        }
     }
-    return launch_long(a);
+    if (nvec <= 256) return launch_rows_any<IO, 256, 1>(a, whole);
+    if (nvec <= 512) return launch_rows_any<IO, 256, 2>(a, whole);
+    if (nvec <= 1024) return launch_rows_any<IO, 512, 2>(a, whole);
+    if (nvec <= 2048) return launch_rows_any<IO, 1024, 2>(a, whole);
+    if constexpr (Io<IO>::E == 4) {
+        if (nvec <= 3072) return launch_rows_any<IO, 1024, 3>(a, whole);
+        if (nvec <= 4096) return launch_rows_any<IO, 1024, 4>(a, whole);
+    }
+    return whole ? launch_long<IO, 1024, false>(a) : launch_long<IO, 1024, true>(a);
 }
 
 size_t workspace_bytes(int64_t rows, int64_t cols) {
     if (rows <= 1 || cols <= 0 || cols > (1 << 30)) return 0;
-    return static_cast<size_t>(max_groups(rows, cols)) * 2 * static_cast<size_t>(cols) * sizeof(float);
+    const int64_t groups = cols <= kMostColumns ? max_groups(rows) : column_splits(rows, cols);
+    return groups > 1 ? static_cast<size_t>(groups) * 2 * static_cast<size_t>(cols) * sizeof(float) : 0;
 }
 
 template <int IO>
@@ -614,16 +655,10 @@ int entry(const void *dy, const void *x, const float *mean, const float *rstd, c
     const float inv_n = 1.0f / static_cast<float>(cols);
     const float inv_d = unbiased ? 1.0f / static_cast<float>(cols - 1) : inv_n;
     float *partial = (dgamma || dbeta) ? static_cast<float *>(workspace) : nullptr;
-    auto run = [&](auto kind) {
-        constexpr int KIND = decltype(kind)::value;
-        const Args<KIND> a{static_cast<const Elem *>(dy), static_cast<const Elem *>(x), mean, rstd,
-                           static_cast<const Elem *>(gamma), static_cast<const Elem *>(dres), static_cast<Elem *>(dx), dgamma,
-                           dbeta, rows, static_cast<int>(cols), inv_n, inv_d, partial, as_stream(stream)};
-        return dispatch<KIND>(a);
-    };
-    // rows that do not start on 16-byte boundaries are walked element by element
-    if (cols % Io<IO>::E != 0 || (rows_at & 15) != 0) return run(std::integral_constant<int, io_by_element(IO)>{});
-    return run(std::integral_constant<int, IO>{});
+    const Args<IO> a{static_cast<const Elem *>(dy), static_cast<const Elem *>(x), mean, rstd, static_cast<const Elem *>(gamma),
+                     static_cast<const Elem *>(dres), static_cast<Elem *>(dx), dgamma, dbeta, rows, static_cast<int>(cols), inv_n,
+                     inv_d, partial, as_stream(stream), 0};
+    return dispatch<IO>(a, cols % Io<IO>::E == 0 && (rows_at & 15) == 0);
 }
 
 }  // namespace

@@ -33,7 +33,7 @@ __device__ __forceinline__ float padding_share(const typename Io<IO>::elem *y, c
 }
 
 // ---- a row in the registers of a group of LPR lanes
-template <int IO, int LPR, int VPL, bool MASKED>
+template <int IO, int LPR, int VPL, bool MASKED, bool RAGGED>
 __global__ __launch_bounds__(64) void softmax_backward_wave_kernel(const typename Io<IO>::elem *y_in,
                                                                    const typename Io<IO>::elem *dy_in,
                                                                    typename Io<IO>::elem *dx_out, int64_t rows, int cols,
@@ -45,12 +45,14 @@ __global__ __launch_bounds__(64) void softmax_backward_wave_kernel(const typenam
     const int lane = threadIdx.x & 63;
     const int sub = lane / LPR;
     const int l = lane % LPR;
-    const int nvec = cols / E;
+    const int nvec = row_vectors<IO, RAGGED>(cols);
     const bool whole_lines = rows_are_whole_lines<IO>(cols);
+    const uint32_t sub_off = static_cast<uint32_t>(sub) * static_cast<uint32_t>(cols) * sizeof(Elem);
     const int64_t stride = static_cast<int64_t>(gridDim.x) * RPW;
     for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * RPW; row0 < rows; row0 += stride) {
         const int64_t row = row0 + sub;
         const bool row_ok = row < rows;
+        const Elem *y0 = y_in + row0 * cols, *dy0 = dy_in + row0 * cols;
         const Elem *y_row = y_in + row * cols, *dy_row = dy_in + row * cols;
         int vlen = cols;
         float beyond = 0.0f;  // y of the masked columns
@@ -72,8 +74,8 @@ __global__ __launch_bounds__(64) void softmax_backward_wave_kernel(const typenam
             yr[k] = typename Io<IO>::raw{};
             dr[k] = typename Io<IO>::raw{};
             if (row_ok && j < nvec && (!MASKED || E * j < vlen)) {
-                yr[k] = Io<IO>::template load_raw<true>(y_row + E * j);
-                dr[k] = Io<IO>::template load_raw<true>(dy_row + E * j);
+                yr[k] = load_row_vec<IO, RAGGED, true>(y0, sub_off, j, cols);
+                dr[k] = load_row_vec<IO, RAGGED, true>(dy0, sub_off, j, cols);
             }
         }
         float y[VPL][E], d[VPL][E];
@@ -95,7 +97,6 @@ __global__ __launch_bounds__(64) void softmax_backward_wave_kernel(const typenam
         }
         t = wave::allreduce<LPR, wave::Sum>(t);
         Elem *dst0 = dx_out + row0 * cols;
-        const uint32_t sub_off = static_cast<uint32_t>(sub) * static_cast<uint32_t>(cols) * sizeof(Elem);
 #pragma unroll
         for (int k = 0; k < VPL; ++k) {
             const int j = l + k * LPR;
@@ -106,14 +107,14 @@ __global__ __launch_bounds__(64) void softmax_backward_wave_kernel(const typenam
                     o[e] = y[k][e] * (d[k][e] - t);
                     if (MASKED && E * j + e >= vlen) o[e] = 0.0f;  // (a NaN t stays with the valid columns)
                 }
-                store_row_vec<IO>(whole_lines, dst0, sub_off + Io<IO>::kBytes * j, o);
+                store_row_vec_any<IO, RAGGED>(whole_lines, dst0, sub_off, j, cols, o);
             }
         }
     }
 }
 
 // ---- a row in the registers of a workgroup
-template <int IO, int THREADS, int VPL, bool MASKED>
+template <int IO, int THREADS, int VPL, bool MASKED, bool RAGGED>
 __global__ __launch_bounds__(THREADS) void softmax_backward_block_kernel(const typename Io<IO>::elem *y_in,
                                                                          const typename Io<IO>::elem *dy_in,
                                                                          typename Io<IO>::elem *dx_out, int64_t rows,
@@ -122,7 +123,7 @@ __global__ __launch_bounds__(THREADS) void softmax_backward_block_kernel(const t
     constexpr int E = Io<IO>::E;
     typedef typename Io<IO>::elem Elem;
     __shared__ float slots[2][THREADS / 64][1];
-    const int nvec = cols / E;
+    const int nvec = row_vectors<IO, RAGGED>(cols);
     const bool whole_lines = rows_are_whole_lines<IO>(cols);
     int turn = 0;
     for (int64_t row = blockIdx.x; row < rows; row += gridDim.x, turn ^= 1) {
@@ -140,8 +141,8 @@ __global__ __launch_bounds__(THREADS) void softmax_backward_block_kernel(const t
             yr[k] = typename Io<IO>::raw{};
             dr[k] = typename Io<IO>::raw{};
             if (j < nvec && (!MASKED || E * j < vlen)) {
-                yr[k] = Io<IO>::template load_raw<true>(byte_offset(y_row, Io<IO>::kBytes * j));
-                dr[k] = Io<IO>::template load_raw<true>(byte_offset(dy_row, Io<IO>::kBytes * j));
+                yr[k] = load_row_vec<IO, RAGGED, true>(y_row, 0, j, cols);
+                dr[k] = load_row_vec<IO, RAGGED, true>(dy_row, 0, j, cols);
             }
         }
         float t[1] = {0.0f};
@@ -173,7 +174,7 @@ __global__ __launch_bounds__(THREADS) void softmax_backward_block_kernel(const t
                     y[e] = y[e] * (d[e] - t[0]);
                     if (MASKED && E * j + e >= vlen) y[e] = 0.0f;
                 }
-                store_row_vec<IO>(whole_lines, dst, Io<IO>::kBytes * j, y);
+                store_row_vec_any<IO, RAGGED>(whole_lines, dst, 0, j, cols, y);
             }
         }
     }
@@ -181,11 +182,11 @@ __global__ __launch_bounds__(THREADS) void softmax_backward_block_kernel(const t
 
 // ---- longer rows: t first, in one or more pieces per row, then a second read
 // One workgroup sums the vectors [lo, hi) of its row.
-template <int IO, int THREADS, bool MASKED>
+template <int IO, int THREADS, bool MASKED, bool RAGGED>
 __device__ __forceinline__ float piece_dot(const typename Io<IO>::elem *y_row, const typename Io<IO>::elem *dy_row, int lo,
-                                           int hi, int vlen) {
+                                           int hi, int vlen, int cols) {
     constexpr int E = Io<IO>::E;
-    constexpr int UNROLL = E == 1 ? 8 : 4;
+    constexpr int UNROLL = 4;
     float t = 0.0f;
     for (int j0 = lo + static_cast<int>(threadIdx.x); j0 < hi; j0 += THREADS * UNROLL) {
         typename Io<IO>::raw yr[UNROLL], dr[UNROLL];
@@ -195,8 +196,8 @@ __device__ __forceinline__ float piece_dot(const typename Io<IO>::elem *y_row, c
             yr[u] = typename Io<IO>::raw{};
             dr[u] = typename Io<IO>::raw{};
             if (j < hi && (!MASKED || E * j < vlen)) {
-                yr[u] = Io<IO>::template load_raw<false>(y_row + static_cast<int64_t>(E) * j);
-                dr[u] = Io<IO>::template load_raw<false>(dy_row + static_cast<int64_t>(E) * j);
+                yr[u] = load_row_vec<IO, RAGGED, false>(y_row, 0, j, cols);
+                dr[u] = load_row_vec<IO, RAGGED, false>(dy_row, 0, j, cols);
             }
         }
 #pragma unroll
@@ -212,12 +213,12 @@ __device__ __forceinline__ float piece_dot(const typename Io<IO>::elem *y_row, c
     return t;
 }
 
-template <int IO, int THREADS, bool MASKED>
+template <int IO, int THREADS, bool MASKED, bool RAGGED>
 __device__ __forceinline__ void piece_apply(const typename Io<IO>::elem *y_row, const typename Io<IO>::elem *dy_row,
-                                            typename Io<IO>::elem *dx_row, int lo, int hi, int vlen, float t,
+                                            typename Io<IO>::elem *dx_row, int lo, int hi, int vlen, int cols, float t,
                                             bool whole_lines) {
     constexpr int E = Io<IO>::E;
-    constexpr int UNROLL = E == 1 ? 8 : 4;
+    constexpr int UNROLL = 4;
     for (int j0 = lo + static_cast<int>(threadIdx.x); j0 < hi; j0 += THREADS * UNROLL) {
         typename Io<IO>::raw yr[UNROLL], dr[UNROLL];
 #pragma unroll
@@ -226,8 +227,8 @@ __device__ __forceinline__ void piece_apply(const typename Io<IO>::elem *y_row, 
             yr[u] = typename Io<IO>::raw{};
             dr[u] = typename Io<IO>::raw{};
             if (j < hi && (!MASKED || E * j < vlen)) {
-                yr[u] = Io<IO>::template load_raw<true>(y_row + static_cast<int64_t>(E) * j);
-                dr[u] = Io<IO>::template load_raw<true>(dy_row + static_cast<int64_t>(E) * j);
+                yr[u] = load_row_vec<IO, RAGGED, true>(y_row, 0, j, cols);
+                dr[u] = load_row_vec<IO, RAGGED, true>(dy_row, 0, j, cols);
             }
         }
 #pragma unroll
@@ -242,13 +243,13 @@ __device__ __forceinline__ void piece_apply(const typename Io<IO>::elem *y_row, 
                 y[e] = y[e] * (d[e] - t);
                 if (MASKED && E * j + e >= vlen) y[e] = 0.0f;
             }
-            store_row_vec<IO>(whole_lines, dx_row, Io<IO>::kBytes * static_cast<uint32_t>(j), y);
+            store_row_vec_any<IO, RAGGED>(whole_lines, dx_row, 0, j, cols, y);
         }
     }
 }
 
 // One workgroup per row, any length.
-template <int IO, int THREADS, bool MASKED>
+template <int IO, int THREADS, bool MASKED, bool RAGGED>
 __global__ __launch_bounds__(THREADS) void softmax_backward_reread_kernel(const typename Io<IO>::elem *y_in,
                                                                           const typename Io<IO>::elem *dy_in,
                                                                           typename Io<IO>::elem *dx_out, int64_t rows,
@@ -256,41 +257,40 @@ __global__ __launch_bounds__(THREADS) void softmax_backward_reread_kernel(const 
                                                                           int64_t rows_per_seq) {
     typedef typename Io<IO>::elem Elem;
     __shared__ float slots[2][THREADS / 64][1];
-    const int nvec = cols / Io<IO>::E;
+    const int nvec = row_vectors<IO, RAGGED>(cols);
     const bool whole_lines = rows_are_whole_lines<IO>(cols);
     int turn = 0;
     for (int64_t row = blockIdx.x; row < rows; row += gridDim.x, turn ^= 1) {
         const Elem *y_row = y_in + row * cols, *dy_row = dy_in + row * cols;
         int vlen = cols;
         if constexpr (MASKED) vlen = clamp_len(valid_len[row / rows_per_seq], cols);
-        float t[1] = {piece_dot<IO, THREADS, MASKED>(y_row, dy_row, 0, nvec, vlen)};
+        float t[1] = {piece_dot<IO, THREADS, MASKED, RAGGED>(y_row, dy_row, 0, nvec, vlen, cols)};
         if constexpr (MASKED) {
             if (vlen > 0 && vlen < cols && Io<IO>::scalar(y_row + vlen) != 0.0f)
                 t[0] += padding_share<IO>(y_row, dy_row, vlen, cols, threadIdx.x, THREADS);
         }
         block_sum<THREADS / 64, 1>(t, slots[turn]);
-        piece_apply<IO, THREADS, MASKED>(y_row, dy_row, dx_out + row * cols, 0, nvec, vlen, t[0], whole_lines);
+        piece_apply<IO, THREADS, MASKED, RAGGED>(y_row, dy_row, dx_out + row * cols, 0, nvec, vlen, cols, t[0], whole_lines);
     }
 }
 
 // A few long rows: workgroup (p, row) takes the row's p-th piece of `piece` vectors; the pieces' sums pass through
 // the workspace and are folded in piece order.
-template <int IO, int THREADS, bool MASKED>
+template <int IO, int THREADS, bool MASKED, bool RAGGED>
 __global__ __launch_bounds__(THREADS) void softmax_backward_pieces_dot_kernel(const typename Io<IO>::elem *y_in,
                                                                               const typename Io<IO>::elem *dy_in, int cols,
                                                                               const int32_t *__restrict__ valid_len,
                                                                               int64_t rows_per_seq, int piece,
                                                                               float *__restrict__ sums) {
-    constexpr int E = Io<IO>::E;
     __shared__ float slots[THREADS / 64][1];
-    const int nvec = cols / E;
+    const int nvec = row_vectors<IO, RAGGED>(cols);
     const int64_t row = blockIdx.y;
     const typename Io<IO>::elem *y_row = y_in + row * cols, *dy_row = dy_in + row * cols;
     int vlen = cols;
     if constexpr (MASKED) vlen = clamp_len(valid_len[row / rows_per_seq], cols);
     const int lo = static_cast<int>(blockIdx.x) * piece;
     const int hi = nvec - lo < piece ? nvec : lo + piece;
-    float t[1] = {piece_dot<IO, THREADS, MASKED>(y_row, dy_row, lo, hi, vlen)};
+    float t[1] = {piece_dot<IO, THREADS, MASKED, RAGGED>(y_row, dy_row, lo, hi, vlen, cols)};
     if constexpr (MASKED) {
         if (vlen > 0 && vlen < cols && Io<IO>::scalar(y_row + vlen) != 0.0f)
             t[0] += padding_share<IO>(y_row, dy_row, vlen, cols, static_cast<int>(blockIdx.x) * THREADS + threadIdx.x,
@@ -300,11 +300,11 @@ __global__ __launch_bounds__(THREADS) void softmax_backward_pieces_dot_kernel(co
     if (threadIdx.x == 0) sums[row * gridDim.x + blockIdx.x] = t[0];
 }
 
-template <int IO, int THREADS, bool MASKED>
+template <int IO, int THREADS, bool MASKED, bool RAGGED>
 __global__ __launch_bounds__(THREADS) void softmax_backward_pieces_apply_kernel(
     const typename Io<IO>::elem *y_in, const typename Io<IO>::elem *dy_in, typename Io<IO>::elem *dx_out, int cols,
     const int32_t *__restrict__ valid_len, int64_t rows_per_seq, int piece, const float *__restrict__ sums) {
-    const int nvec = cols / Io<IO>::E;
+    const int nvec = row_vectors<IO, RAGGED>(cols);
     const int64_t row = blockIdx.y;
     int vlen = cols;
     if constexpr (MASKED) vlen = clamp_len(valid_len[row / rows_per_seq], cols);
@@ -312,7 +312,7 @@ __global__ __launch_bounds__(THREADS) void softmax_backward_pieces_apply_kernel(
     const int hi = nvec - lo < piece ? nvec : lo + piece;
     float t = 0.0f;
     for (unsigned p = 0; p < gridDim.x; ++p) t += sums[row * gridDim.x + p];
-    piece_apply<IO, THREADS, MASKED>(y_in + row * cols, dy_in + row * cols, dx_out + row * cols, lo, hi, vlen, t,
+    piece_apply<IO, THREADS, MASKED, RAGGED>(y_in + row * cols, dy_in + row * cols, dx_out + row * cols, lo, hi, vlen, cols, t,
                                      rows_are_whole_lines<IO>(cols));
 }
 
@@ -330,23 +330,23 @@ struct Args {
     hipStream_t stream;
 };
 
-template <int IO, int LPR, int VPL, bool MASKED>
+template <int IO, int LPR, int VPL, bool MASKED, bool RAGGED>
 int launch_wave(const Args<IO> &a) {
     constexpr int RPW = 64 / LPR;
     int64_t grid = (a.rows + RPW - 1) / RPW;
     if (grid > 0x7fffffff) grid = 0x7fffffff;
     // Residency cap as in the forward kernels (lds_pad_for_residency): a wavefront has y and dy in flight.
     const int lds = lds_pad_for_residency(int64_t{2} * RPW * a.cols * sizeof(typename Io<IO>::elem), (MASKED ? 64 : 40) * 1024);
-    softmax_backward_wave_kernel<IO, LPR, VPL, MASKED><<<dim3(static_cast<unsigned>(grid)), dim3(64), lds, a.stream>>>(
+    softmax_backward_wave_kernel<IO, LPR, VPL, MASKED, RAGGED><<<dim3(static_cast<unsigned>(grid)), dim3(64), lds, a.stream>>>(
         a.y, a.dy, a.dx, a.rows, a.cols, a.valid_len, a.rows_per_seq);
     KO_CHECK_LAUNCH();
     return KO_OK;
 }
 
-template <int IO, int THREADS, int VPL, bool MASKED>
+template <int IO, int THREADS, int VPL, bool MASKED, bool RAGGED>
 int launch_block(const Args<IO> &a) {
     const int64_t grid = a.rows > 0x7fffffff ? 0x7fffffff : a.rows;
-    softmax_backward_block_kernel<IO, THREADS, VPL, MASKED><<<dim3(static_cast<unsigned>(grid)), dim3(THREADS), 0, a.stream>>>(
+    softmax_backward_block_kernel<IO, THREADS, VPL, MASKED, RAGGED><<<dim3(static_cast<unsigned>(grid)), dim3(THREADS), 0, a.stream>>>(
         a.y, a.dy, a.dx, a.rows, a.cols, a.valid_len, a.rows_per_seq);
     KO_CHECK_LAUNCH();
     return KO_OK;
@@ -363,71 +363,54 @@ int pieces_per_row(int64_t rows, int64_t row_bytes) {
     return static_cast<int>(parts);
 }
 
-template <int IO, bool MASKED>
+template <int IO, bool MASKED, bool RAGGED>
 int launch_long(const Args<IO> &a) {
     constexpr int THREADS = 1024;
     const int64_t grid = a.rows > 0x7fffffff ? 0x7fffffff : a.rows;
-    softmax_backward_reread_kernel<IO, THREADS, MASKED><<<dim3(static_cast<unsigned>(grid)), dim3(THREADS), 0, a.stream>>>(
+    softmax_backward_reread_kernel<IO, THREADS, MASKED, RAGGED><<<dim3(static_cast<unsigned>(grid)), dim3(THREADS), 0, a.stream>>>(
         a.y, a.dy, a.dx, a.rows, a.cols, a.valid_len, a.rows_per_seq);
     KO_CHECK_LAUNCH();
     return KO_OK;
 }
 
-template <int IO, bool MASKED>
+template <int IO, bool MASKED, bool RAGGED>
 int launch_pieces(const Args<IO> &a, int parts) {
     constexpr int THREADS = 256;
-    const int nvec = a.cols / Io<IO>::E;
+    const int nvec = (a.cols + Io<IO>::E - 1) / Io<IO>::E;
     const int piece = (nvec + parts - 1) / parts;
     parts = (nvec + piece - 1) / piece;
     const dim3 grid(static_cast<unsigned>(parts), static_cast<unsigned>(a.rows));
-    softmax_backward_pieces_dot_kernel<IO, THREADS, MASKED><<<grid, dim3(THREADS), 0, a.stream>>>(
+    softmax_backward_pieces_dot_kernel<IO, THREADS, MASKED, RAGGED><<<grid, dim3(THREADS), 0, a.stream>>>(
         a.y, a.dy, a.cols, a.valid_len, a.rows_per_seq, piece, a.workspace);
     KO_CHECK_LAUNCH();
-    softmax_backward_pieces_apply_kernel<IO, THREADS, MASKED><<<grid, dim3(THREADS), 0, a.stream>>>(
+    softmax_backward_pieces_apply_kernel<IO, THREADS, MASKED, RAGGED><<<grid, dim3(THREADS), 0, a.stream>>>(
         a.y, a.dy, a.dx, a.cols, a.valid_len, a.rows_per_seq, piece, a.workspace);
     KO_CHECK_LAUNCH();
     return KO_OK;
 }
 
-template <int IO, bool MASKED>
+template <int IO, bool MASKED, bool RAGGED>
 int dispatch(const Args<IO> &a) {
-    constexpr int E = Io<IO>::E;
-    const int nvec = a.cols / E;
+    const int nvec = (a.cols + Io<IO>::E - 1) / Io<IO>::E;
     if (a.workspace != nullptr) {
         const int parts = pieces_per_row(a.rows, static_cast<int64_t>(a.cols) * sizeof(typename Io<IO>::elem));
-        if (parts > 1) return launch_pieces<IO, MASKED>(a, parts);
+        if (parts > 1) return launch_pieces<IO, MASKED, RAGGED>(a, parts);
     }
-    if constexpr (E == 1) {
-        // element by element
-        if (nvec <= 8) return launch_wave<IO, 8, 1, MASKED>(a);
-        if (nvec <= 16) return launch_wave<IO, 16, 1, MASKED>(a);
-        if (nvec <= 32) return launch_wave<IO, 16, 2, MASKED>(a);
-        if (nvec <= 64) return launch_wave<IO, 16, 4, MASKED>(a);
-        if (nvec <= 128) return launch_wave<IO, 64, 2, MASKED>(a);
-        if (nvec <= 256) return launch_wave<IO, 64, 4, MASKED>(a);
-        if (nvec <= 512) return launch_wave<IO, 64, 8, MASKED>(a);
-        if (nvec <= 1024) return launch_wave<IO, 64, 16, MASKED>(a);
-        if (nvec <= 2048) return launch_block<IO, 512, 4, MASKED>(a);
-        if (nvec <= 4096) return launch_block<IO, 512, 8, MASKED>(a);
-        if (nvec <= 8192) return launch_block<IO, 1024, 8, MASKED>(a);
-        if (nvec <= 16384) return launch_block<IO, 1024, 16, MASKED>(a);
-    } else {
-        int lpr = 0, vpl = 0;
-        if (choose_row_group(nvec, 4, &lpr, &vpl)) {
-#define KO_WAVE(L, V) if (lpr == L && vpl == V) return launch_wave<IO, L, V, MASKED>(a)
-            KO_WAVE(8, 1); KO_WAVE(8, 2); KO_WAVE(8, 3);
-            KO_WAVE(16, 1); KO_WAVE(16, 2); KO_WAVE(16, 3);
-            KO_WAVE(32, 1); KO_WAVE(32, 2); KO_WAVE(32, 3);
-            KO_WAVE(64, 1); KO_WAVE(64, 2); KO_WAVE(64, 3); KO_WAVE(64, 4);
+    int lpr = 0, vpl = 0;
+    if (choose_row_group(nvec, 4, &lpr, &vpl)) {
+#define KO_WAVE(L, V) if (lpr == L && vpl == V) return launch_wave<IO, L, V, MASKED, RAGGED>(a)
+        KO_WAVE(8, 1); KO_WAVE(8, 2); KO_WAVE(8, 3);
+        KO_WAVE(16, 1); KO_WAVE(16, 2); KO_WAVE(16, 3);
+        KO_WAVE(32, 1); KO_WAVE(32, 2); KO_WAVE(32, 3);
+        KO_WAVE(64, 1); KO_WAVE(64, 2); KO_WAVE(64, 3); KO_WAVE(64, 4);
 #undef KO_WAVE
-        }
-        if (nvec <= 512) return launch_block<IO, 256, 2, MASKED>(a);
-        if (nvec <= 1024) return launch_block<IO, 512, 2, MASKED>(a);
-        if (nvec <= 2048) return launch_block<IO, 1024, 2, MASKED>(a);
-        if (nvec <= 4096) return launch_block<IO, 1024, 4, MASKED>(a);
-        if (nvec <= 8192) return launch_block<IO, 1024, 8, MASKED>(a);
     }
-    return launch_long<IO, MASKED>(a);
+    if (nvec <= 512) return launch_block<IO, 256, 2, MASKED, RAGGED>(a);
+    if (nvec <= 1024) return launch_block<IO, 512, 2, MASKED, RAGGED>(a);
+    if (nvec <= 2048) return launch_block<IO, 1024, 2, MASKED, RAGGED>(a);
+    if (nvec <= 4096) return launch_block<IO, 1024, 4, MASKED, RAGGED>(a);
+    if (nvec <= 8192) return launch_block<IO, 1024, 8, MASKED, RAGGED>(a);
+    return launch_long<IO, MASKED, RAGGED>(a);
 }
 
 size_t workspace_bytes(int64_t rows, int64_t cols) {
@@ -454,16 +437,11 @@ int entry(const void *y, const void *dy, void *dx, int64_t rows, int64_t cols, c
         return fail(KO_ERR_INVALID_ARGUMENT, "softmax_backward: workspace of %zu bytes, %zu needed", bytes, workspace_bytes(rows, cols));
     if (reinterpret_cast<uintptr_t>(workspace) & 15)
         return fail(KO_ERR_INVALID_ARGUMENT, "softmax_backward: workspace must be 16-byte aligned");
-    const Elem *ye = static_cast<const Elem *>(y), *dye = static_cast<const Elem *>(dy);
-    Elem *dxe = static_cast<Elem *>(dx);
-    float *ws = static_cast<float *>(workspace);
-    if (cols % Io<IO>::E != 0 || (addresses & 15) != 0) {
-        constexpr int BY_ELEMENT = io_by_element(IO);
-        const Args<BY_ELEMENT> a{ye, dye, dxe, rows, static_cast<int>(cols), valid_len, rows_per_seq, ws, as_stream(stream)};
-        return valid_len ? dispatch<BY_ELEMENT, true>(a) : dispatch<BY_ELEMENT, false>(a);
-    }
-    const Args<IO> a{ye, dye, dxe, rows, static_cast<int>(cols), valid_len, rows_per_seq, ws, as_stream(stream)};
-    return valid_len ? dispatch<IO, true>(a) : dispatch<IO, false>(a);
+    const Args<IO> a{static_cast<const Elem *>(y), static_cast<const Elem *>(dy), static_cast<Elem *>(dx), rows,
+                     static_cast<int>(cols), valid_len, rows_per_seq, static_cast<float *>(workspace), as_stream(stream)};
+    if (cols % Io<IO>::E != 0 || (addresses & 15) != 0)
+        return valid_len ? dispatch<IO, true, true>(a) : dispatch<IO, false, true>(a);
+    return valid_len ? dispatch<IO, true, false>(a) : dispatch<IO, false, false>(a);
 }
 
 }  // namespace

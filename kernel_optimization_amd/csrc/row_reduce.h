@@ -21,6 +21,122 @@ __device__ __forceinline__ void convert_again(typename Io<IO>::raw &r) {
     if constexpr (Io<IO>::E > 1) asm volatile("" : "+v"(r));
 }
 
+// ---- vectors of rows that start anywhere
+// A row whose length is no whole number of 16-byte vectors, or a tensor that does not start on a 16-byte boundary, puts
+// rows at any element's address.  Such RAGGED rows are still walked vector by vector, from their first column on: the
+// hardware takes 16-byte accesses at any address (the compiler issues them for under-aligned types), at a fraction of
+// the cost of one access per element; only the row's last vector, where it is not whole, goes element by element.
+template <int IO>
+struct Unaligned {
+    typedef typename Io<IO>::raw type __attribute__((aligned(sizeof(typename Io<IO>::elem))));
+};
+
+// Vectors of a row.
+template <int IO, bool RAGGED>
+__device__ __forceinline__ int row_vectors(int cols) {
+    return RAGGED ? (cols + Io<IO>::E - 1) / Io<IO>::E : cols / Io<IO>::E;
+}
+
+// Vector j (of those that row_vectors counts) of the row at `uniform_base + offset` bytes; what lies past the row's end
+// is 0.
+template <int IO, bool RAGGED, bool NT>
+__device__ __forceinline__ typename Io<IO>::raw load_row_vec(const typename Io<IO>::elem *base, uint32_t offset, int j, int cols) {
+    constexpr int E = Io<IO>::E;
+    typedef typename Io<IO>::raw Raw;
+    const typename Io<IO>::elem *p = byte_offset(base, offset + Io<IO>::kBytes * static_cast<uint32_t>(j));
+    if constexpr (!RAGGED) {
+        return Io<IO>::template load_raw<NT>(p);
+    } else {
+        if (E * (j + 1) <= cols) {
+            typedef typename Unaligned<IO>::type Any;
+            if constexpr (NT) return __builtin_nontemporal_load(reinterpret_cast<const Any *>(p));
+            return *reinterpret_cast<const Any *>(p);
+        }
+        Raw r{};
+        const int n = cols - E * j;
+#pragma unroll
+        for (int e = 0; e < E - 1; ++e) {
+            if constexpr (E == 4) {
+                if (e < n) r[e] = p[e];
+            } else {
+                if (e < n) r[e / 2] |= static_cast<uint32_t>(p[e]) << (16 * (e & 1));
+            }
+        }
+        return r;
+    }
+}
+
+// The values of one vector, rounded to the storage type.
+template <int IO>
+__device__ __forceinline__ typename Io<IO>::raw pack(const float (&v)[Io<IO>::E]) {
+    constexpr int E = Io<IO>::E;
+    if constexpr (IO == IO_F32) {
+        return float4v{v[0], v[1], v[2], v[3]};
+    } else if constexpr (IO == IO_F16) {
+        typename Io<IO>::half8 h;
+#pragma unroll
+        for (int e = 0; e < E; ++e) h[e] = static_cast<_Float16>(v[e]);
+        return __builtin_bit_cast(uint4v, h);
+    } else {
+        typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+        typedef float float2v __attribute__((ext_vector_type(2)));
+        uint4v x;
+#pragma unroll
+        for (int e = 0; e < E / 2; ++e)
+            x[e] = __builtin_bit_cast(uint32_t, __builtin_convertvector(float2v{v[2 * e], v[2 * e + 1]}, bf16x2));
+        return x;
+    }
+}
+
+// Vector j of an output row, counterpart of load_row_vec: whole lines by store_row_vec.
+template <int IO, bool RAGGED>
+__device__ __forceinline__ void store_row_vec_any(bool whole_lines, typename Io<IO>::elem *base, uint32_t offset, int j, int cols,
+                                                  const float (&v)[Io<IO>::E]) {
+    constexpr int E = Io<IO>::E;
+    const uint32_t at = offset + Io<IO>::kBytes * static_cast<uint32_t>(j);
+    if constexpr (!RAGGED) {
+        store_row_vec<IO>(whole_lines, base, at, v);
+    } else {
+        const typename Io<IO>::raw r = pack<IO>(v);
+        typename Io<IO>::elem *p = byte_offset(base, at);
+        if (E * (j + 1) <= cols) {
+            __builtin_nontemporal_store(r, reinterpret_cast<typename Unaligned<IO>::type *>(p));
+            return;
+        }
+        const int n = cols - E * j;
+#pragma unroll
+        for (int e = 0; e < E - 1; ++e) {
+            if constexpr (E == 4) {
+                if (e < n) p[e] = r[e];
+            } else {
+                if (e < n) p[e] = static_cast<uint16_t>(r[e / 2] >> (16 * (e & 1)));
+            }
+        }
+    }
+}
+
+// Whole vectors for kernels that keep loads of later rows in flight: no access is made under a condition, since past a
+// branch the compiler no longer knows how many accesses are on their way and waits for all of them.
+// FULL: rows of whole vectors on 16-byte boundaries; else at any address (`offset` in bytes, a multiple of the element).
+template <int IO, bool FULL>
+__device__ __forceinline__ typename Io<IO>::raw load_whole(const typename Io<IO>::elem *base, uint32_t offset) {
+    if constexpr (FULL) return Io<IO>::template load_raw<true>(byte_offset(base, offset));
+    else return __builtin_nontemporal_load(reinterpret_cast<const typename Unaligned<IO>::type *>(byte_offset(base, offset)));
+}
+template <int IO, bool FULL>
+__device__ __forceinline__ void store_whole(typename Io<IO>::elem *base, uint32_t offset, const float (&v)[Io<IO>::E]) {
+    const typename Io<IO>::raw r = pack<IO>(v);
+    if constexpr (FULL) {
+        // written through at once like stream_store16, but by a builtin, which the compiler counts
+        constexpr int kNt = 2, kSc1 = 16;      // cache policy bits
+        constexpr int kRaw32Bit = 0x00027000;  // resource word 3: raw buffer, 32-bit data
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(uint4v, r),
+                                               __builtin_amdgcn_make_buffer_rsrc(base, 0, -1, kRaw32Bit), offset, 0, kNt | kSc1);
+    } else {
+        __builtin_nontemporal_store(r, reinterpret_cast<typename Unaligned<IO>::type *>(byte_offset(base, offset)));
+    }
+}
+
 // Sum over a workgroup of WAVES wavefronts of N values at once: wave all-reduces, then every thread folds the
 // per-wave partials in wave order (the same bits in every thread).  One barrier: `slot` is not written again before
 // every wave has passed the workgroup's next barrier (callers alternate between two slots).

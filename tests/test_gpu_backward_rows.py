@@ -268,3 +268,29 @@ def test_layernorm_backward_follows_the_forward_call(ko):
             num = (loss(*hi) - loss(*lo)) / (2 * step)
             # the forward gate on mean and rstd (1e-5 of their scale) times sums of six to forty terms of size 1 to 3
             assert abs(num - got[i]) <= 1e-4 * max(1.0, abs(num)), (at, i, num, got[i])
+
+
+# both sides of the forms for few rows (up to 256 of them: one launch), rows of three and four vectors per thread of the largest
+# workgroup, and rows shorter than a vector
+@pytest.mark.parametrize("rows,cols,kind", [(256, 136, "bf16"), (257, 136, "bf16"), (256, 2056, "f32"), (257, 2056, "f32"),
+                                            (40, 9000, "f32"), (300, 12288, "f32"), (40, 12300, "f32"), (3, 16384, "f32"),
+                                            (3, 16400, "f32"), (1025, 5, "f16"), (700, 3, "f32"), (20000, 24, "f32"),
+                                            (3000, 768, "bf16"), (2049, 1536, "f16"), (520, 4096, "bf16")])
+def test_layernorm_backward_borders(ko, rows, cols, kind):
+    case = layernorm_case(rows, cols, kind, 1700 + cols)
+    got = check_layernorm_backward(ko, case, kind)
+    for place in ("dy", "x"):
+        for a, b in zip(run_layernorm_backward(ko, kind=kind, **case, in_place=place), got):
+            np.testing.assert_array_equal(a, b, err_msg=place)
+    check_layernorm_backward(ko, case, kind, workspace=False)
+    check_layernorm_backward(ko, case, kind, skew=4)
+
+
+def test_backward_workspaces_stay_small():
+    """Sizes that a caller can always allocate: 64 MB at most, whatever the shape."""
+    import kernel_optimization_amd as ko
+    for rows in (1, 2, 300, 100000, 1 << 30):
+        for cols in (1, 7, 768, 16384, 16385, 100000, 1 << 30):
+            assert ko.layernorm_backward_workspace_bytes(rows, cols) <= 64 << 20
+            assert ko.softmax_backward_workspace_bytes(rows, cols) <= 64 << 20
+            assert ko.token_logprob_workspace_bytes(rows, cols) <= 64 << 20
