@@ -202,7 +202,7 @@ int ko_layernorm_backward_16(const void *dy, const void *in, const float *mean, 
  * dlogits whose rows lie differently in their 16-byte vectors than the logits' rows is walked element by element.
  * labels: device int32[rows].  A negative label marks a row that takes no part (a prompt's, padding): its logits are
  * never read, its outputs and its gradient are 0.  A label >= cols reads nothing out of place and makes the row's
- * outputs and its gradient NaN.  scale multiplies the logits (1 / temperature), from 1e-30 to 1e30.
+ * outputs and its gradient NaN.  scale multiplies the logits (1 / temperature), from 1e-20 to 1e20.
  * Special values: a NaN or +inf among a row's logits makes its outputs NaN; -inf elements have probability 0.
  * One workspace size serves all of them (see above). */
 size_t ko_token_logprob_workspace_bytes(int64_t rows, int64_t cols);

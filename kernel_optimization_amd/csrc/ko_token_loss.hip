@@ -19,12 +19,25 @@
 #include "row_reduce.h"
 
 #include <cfloat>
+#include <cmath>
 #include <initializer_list>
 
 namespace ko {
 namespace {
 
 constexpr float kLog2e = 0x1.715476p+0f;
+
+// A value that is the same in every lane, in scalar registers: what follows from a row's label stays there, too.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ float uniform(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v)));
+}
+
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+    const uint64_t b = static_cast<uint64_t>(v);
+    const uint64_t hi = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(b >> 32)));
+    return static_cast<int64_t>((hi << 32) | static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(b))));
+}
 
 // ---- a row's columns
 template <int IO>
@@ -56,34 +69,48 @@ __device__ __forceinline__ int single_column(const RowSpan<IO> &s, int i) {
     return i < s.head ? i : s.nvec * Io<IO>::E + i;
 }
 
-// ---- running (maximum, sum of exp(scale (x - maximum))); c = scale log2(e)
+// ---- running (maximum, sum of exp(scale (x - maximum)))
 struct Pair {
     float m, s;
 };
-__device__ __forceinline__ float exp_scaled(float d, float c) { return __builtin_amdgcn_exp2f(d * c); }
+// scale log2(e) in two parts: of one float it would be off by up to 2^-24 of itself, the same way in every exponential of a
+// row, which 100000 of them do not average out (1e-6 in a logp of -13).  lo is positive.
+struct Scale {
+    float hi, lo;
+};
+// exp(scale d).  exp_sum: for sums; exp_scaled: where the result is rounded next.
+__device__ __forceinline__ float exp_sum(float d, Scale c) { return __builtin_amdgcn_exp2f(__builtin_fmaf(d, c.lo, d * c.hi)); }
+__device__ __forceinline__ float exp_scaled(float d, Scale c) { return __builtin_amdgcn_exp2f(d * c.hi); }
 // An empty pair is (-FLT_MAX, 0).
 
-// Adds N values (absent ones: -inf) at once: the sum is rescaled at most once for all of them.
+// Adds N values (absent ones: -inf) at once: the sum is rescaled at most once for all of them, and only where a lane of
+// the wavefront has met a larger value.
 template <int N>
-__device__ __forceinline__ void add_values(Pair &p, const float (&v)[N], float c) {
+__device__ __forceinline__ void add_values(Pair &p, const float (&v)[N], Scale c) {
     float m = v[0];
 #pragma unroll
     for (int i = 1; i < N; ++i) m = fmaxf(m, v[i]);
-    if (m > p.m) {
-        p.s *= exp_scaled(p.m - m, c);
-        p.m = m;
+    if (__any(m > p.m)) {
+        const float top = fmaxf(m, p.m);
+        p.s *= exp_sum(p.m - top, c);
+        p.m = top;
     }
-    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    float s[N < 4 ? N : 4];
 #pragma unroll
-    for (int i = 0; i < N; ++i) s[i % 4] += exp_scaled(v[i] - p.m, c);
-    p.s += (s[0] + s[1]) + (s[2] + s[3]);
+    for (int i = 0; i < N; ++i) {
+        const float e = exp_sum(v[i] - p.m, c);
+        if (i < 4) s[i] = e;
+        else s[i % 4] += e;
+    }
+    if constexpr (N >= 4) p.s += (s[0] + s[1]) + (s[2] + s[3]);
+    else p.s += s[0];
 }
 
 // The pairs of a workgroup's threads, the same bits in every thread.  One barrier; `slot` as in block_sum.
 template <int WAVES>
-__device__ __forceinline__ Pair block_pair(Pair p, Pair *slot, float c) {
+__device__ __forceinline__ Pair block_pair(Pair p, Pair *slot, Scale c) {
     const float m = wave::allreduce<64, wave::Max>(p.m);
-    Pair r{m, wave::allreduce<64, wave::Sum>(p.s * exp_scaled(p.m - m, c))};
+    Pair r{m, wave::allreduce<64, wave::Sum>(p.s * exp_sum(p.m - m, c))};
     if constexpr (WAVES > 1) {
         if ((threadIdx.x & 63) == 0) slot[threadIdx.x >> 6] = r;
         __syncthreads();
@@ -92,7 +119,7 @@ __device__ __forceinline__ Pair block_pair(Pair p, Pair *slot, float c) {
         for (int w = 1; w < WAVES; ++w) top = fmaxf(top, slot[w].m);
         float s = 0.0f;
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) s += slot[w].s * exp_scaled(slot[w].m - top, c);
+        for (int w = 0; w < WAVES; ++w) s += slot[w].s * exp_sum(slot[w].m - top, c);
         r = Pair{top, s};
     }
     return r;
@@ -102,7 +129,7 @@ __device__ __forceinline__ Pair block_pair(Pair p, Pair *slot, float c) {
 // the label's column.
 template <int IO, int THREADS>
 __device__ __forceinline__ Pair thread_pair(const typename Io<IO>::elem *row, const RowSpan<IO> &span, int lo, int hi,
-                                            bool with_singles, int label, float c) {
+                                            bool with_singles, int label, Scale c) {
     constexpr int E = Io<IO>::E;
     constexpr int UNROLL = E == 8 ? 4 : 8;
     Pair p{-FLT_MAX, 0.0f};
@@ -165,10 +192,10 @@ __device__ __forceinline__ double log_in_parts(float t) {
     return __builtin_fma(static_cast<double>(k), 0.69314718055994531, static_cast<double>(logf(f)));
 }
 // From the pair of the other columns and the label's logit.
-__device__ __forceinline__ RowScore score_row(Pair p, float at_label, float scale, float c) {
+__device__ __forceinline__ RowScore score_row(Pair p, float at_label, float scale, Scale c) {
     RowScore r;
     r.top = fmaxf(p.m, at_label);
-    const float s = p.s * exp_scaled(p.m - r.top, c);
+    const float s = p.s * exp_sum(p.m - r.top, c);
     const double z = (static_cast<double>(at_label) - static_cast<double>(r.top)) * static_cast<double>(scale);
     const float e = expf(static_cast<float>(z));
     const float total = s + e;
@@ -191,7 +218,7 @@ __device__ __forceinline__ RowScore nan_score() {
 // The values of one vector, the first of them element `first` of the row's vectors, become their gradient.
 template <int E, class LabelGrad>
 __device__ __forceinline__ void gradient_of(float (&x)[E], int first, bool live, int in_vecs, bool holds_label, float top,
-                                            float a, LabelGrad label_grad, float c) {
+                                            float a, LabelGrad label_grad, Scale c) {
     float at_label = 0.0f;
     if (holds_label) {
 #pragma unroll
@@ -208,13 +235,20 @@ __device__ __forceinline__ void gradient_of(float (&x)[E], int first, bool live,
     }
 }
 
+// One vector at base + offset, counted by the compiler (see store_whole).  LINES: part of whole 64-byte lines.
+template <int IO, bool LINES>
+__device__ __forceinline__ void store_vec(typename Io<IO>::elem *base, uint32_t offset, const float (&v)[Io<IO>::E]) {
+    if constexpr (LINES) store_whole<IO, true>(base, offset, v);
+    else Io<IO>::template store<true>(byte_offset(base, offset), v);
+}
+
 // Gradient of one row's vectors [lo, hi) and, if `with_singles`, its single elements: a exp(scale (x - top)) beside the
 // label, label_grad(x) at the label.  `live` false: zeros, nothing read.  Every thread reads what it overwrites and nothing
 // else, so `out` may be `row`.
 template <int IO, int THREADS, class LabelGrad>
 __device__ __forceinline__ void write_gradient(const typename Io<IO>::elem *row, typename Io<IO>::elem *out,
                                                const RowSpan<IO> &span, int lo, int hi, bool with_singles, bool live,
-                                               int label, float top, float a, LabelGrad label_grad, float c) {
+                                               int label, float top, float a, LabelGrad label_grad, Scale c) {
     constexpr int E = Io<IO>::E;
     constexpr int UNROLL = E == 8 ? 2 : 4;
     typedef typename Io<IO>::elem Elem;
@@ -263,7 +297,8 @@ struct ScoreArgs {
     const Elem *logits;
     int64_t ld;
     const int32_t *labels;
-    float scale, c;
+    float scale;
+    Scale c;
     float *logp;
     float *row_stats;  // [rows][2]: maximum, log sum
     int64_t rows;
@@ -286,7 +321,7 @@ __global__ __launch_bounds__(THREADS) void token_logprob_row_kernel(ScoreArgs<IO
     __shared__ Pair slots[2][THREADS / 64];
     int turn = 0;
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
-        const int label = a.labels[row];
+        const int label = uniform(a.labels[row]);
         RowScore r = nan_score();
         if (label >= 0 && label < a.cols) {
             const typename Io<IO>::elem *src = a.logits + row * a.ld;
@@ -311,12 +346,12 @@ static_assert(sizeof(PieceHeader) == sizeof(Pair), "");
 template <int IO, int THREADS>
 __global__ __launch_bounds__(THREADS) void token_pieces_kernel(const typename Io<IO>::elem *logits, int64_t ld,
                                                                const int32_t *__restrict__ labels,
-                                                               const float *__restrict__ weight, int cols, float c,
+                                                               const float *__restrict__ weight, int cols, Scale c,
                                                                Pair *__restrict__ pairs) {
     __shared__ Pair slot[THREADS / 64];
     const int64_t row = blockIdx.y;
-    const int label = labels[row];
-    if (label < 0 || label >= cols || (weight && weight[row] == 0.0f)) return;
+    const int label = uniform(labels[row]);
+    if (label < 0 || label >= cols || (weight && uniform(weight[row]) == 0.0f)) return;
     const typename Io<IO>::elem *src = logits + row * ld;
     const RowSpan<IO> span = span_of<IO>(src, cols);
     const int parts = static_cast<int>(gridDim.x), part = static_cast<int>(blockIdx.x);
@@ -330,11 +365,11 @@ __global__ __launch_bounds__(THREADS) void token_pieces_kernel(const typename Io
         mine[1 + part] = p;
     }
 }
-__device__ __forceinline__ Pair fold_pieces(const Pair *mine, int parts, float c) {
+__device__ __forceinline__ Pair fold_pieces(const Pair *mine, int parts, Scale c) {
     float m = mine[1].m;
     for (int i = 2; i <= parts; ++i) m = fmaxf(m, mine[i].m);
     float s = 0.0f;
-    for (int i = 1; i <= parts; ++i) s += mine[i].s * exp_scaled(mine[i].m - m, c);
+    for (int i = 1; i <= parts; ++i) s += mine[i].s * exp_sum(mine[i].m - m, c);
     return Pair{m, s};
 }
 
@@ -353,14 +388,14 @@ __global__ __launch_bounds__(64) void token_logprob_fold_kernel(ScoreArgs<IO> a,
 template <int IO, int THREADS>
 __global__ __launch_bounds__(THREADS) void token_logprob_backward_kernel(const typename Io<IO>::elem *logits, int64_t ld,
                                                                          const int32_t *__restrict__ labels, float scale,
-                                                                         float c, const float *__restrict__ row_stats,
+                                                                         Scale c, const float *__restrict__ row_stats,
                                                                          const float *__restrict__ dlogp,
                                                                          typename Io<IO>::elem *dlogits, int64_t ldd,
                                                                          int64_t rows, int cols) {
     typedef typename Io<IO>::elem Elem;
     for (int64_t row = blockIdx.y; row < rows; row += gridDim.y) {
-        const int label = labels[row];
-        float coeff = dlogp[row] * scale;
+        const int label = uniform(labels[row]);
+        float coeff = uniform(dlogp[row]) * scale;
         const bool live = label >= 0 && coeff != 0.0f;
         if (label >= cols) coeff = __builtin_nanf("");
         const Elem *src = logits + row * ld;
@@ -370,8 +405,8 @@ __global__ __launch_bounds__(THREADS) void token_logprob_backward_kernel(const t
         const int piece = (span.nvec + parts - 1) / parts;
         const int lo = part * piece < span.nvec ? part * piece : span.nvec;
         const int hi = span.nvec - lo < piece ? span.nvec : lo + piece;
-        const float top = live ? row_stats[2 * row] : 0.0f;
-        const float logsum = live ? row_stats[2 * row + 1] : 0.0f;
+        const float top = live ? uniform(row_stats[2 * row]) : 0.0f;
+        const float logsum = live ? uniform(row_stats[2 * row + 1]) : 0.0f;
         const float a = -coeff * __builtin_amdgcn_exp2f(-logsum * kLog2e);
         // coeff (1 - p), from p's logarithm: close to 0 that is where p has lost the difference
         const auto label_grad = [&](float x) { return -coeff * expm1f((x - top) * scale - logsum); };
@@ -393,7 +428,9 @@ struct PolicyArgs {
     const float *ref_logp;   // null: no KL term
     const float *advantage;
     const float *weight;     // null: 1
-    float scale, c, clip_low, clip_high, kl_coef;
+    float scale;
+    Scale c;
+    float clip_low, clip_high, kl_coef;
     float *logp;
     float *kl;
     float *loss;
@@ -410,10 +447,14 @@ struct RowGradient {
     bool live;
 };
 
+__device__ __forceinline__ RowGradient uniform_gradient(const RowGradient &g) {
+    return RowGradient{uniform(g.a), uniform(g.label_grad), uniform(g.top), uniform(static_cast<int>(g.live)) != 0};
+}
+
 template <int IO>
 __device__ __forceinline__ bool policy_row_counts(const PolicyArgs<IO> &a, int64_t row, int &label) {
-    label = a.labels[row];
-    return label >= 0 && (!a.weight || a.weight[row] != 0.0f);
+    label = uniform(a.labels[row]);
+    return label >= 0 && (!a.weight || uniform(a.weight[row]) != 0.0f);
 }
 
 // exp(d) - 1 - d, given up = exp(d) - 1: close to 0 the difference cancels, and the series takes over
@@ -431,44 +472,71 @@ __device__ __forceinline__ float kl_of(float d, float up) {
     return s * d * d;
 }
 
-// One thread's work: the row's outputs (if `put`) and its gradient's factors.
+// What a row's loss is made of beside its logits.
+struct PolicyRow {
+    float advantage, weight, old_logp, ref_logp, at_label;
+    int label;
+};
 template <int IO>
-__device__ __forceinline__ RowGradient policy_row(const PolicyArgs<IO> &a, int64_t row, bool counts, const RowScore &r, bool put) {
-    RowGradient g{0.0f, 0.0f, 0.0f, false};
-    double kl = 0.0, loss = 0.0;
-    if (counts) {
-        const double adv = a.advantage[row], w = a.weight ? a.weight[row] : 1.0f;
-        const double ratio = a.old_logp ? expf(static_cast<float>(r.logp - static_cast<double>(a.old_logp[row])))
-                                        : 1.0 + 0.0 * r.logp;
-        const double low = 1.0 - a.clip_low, high = 1.0 + a.clip_high;
-        double kept = ratio, slope = -adv * ratio;
-        if (adv > 0.0 ? ratio > high : ratio < low) {
-            kept = adv > 0.0 ? high : low;
-            slope = 0.0;
-        }
-        if (adv == 0.0) slope = kept = 0.0;  // (no surrogate, however large the ratio)
-        double total = -adv * kept;
-        if (a.ref_logp) {
-            const float d = static_cast<float>(static_cast<double>(a.ref_logp[row]) - r.logp);
-            const float up = expm1f(d);
-            kl = kl_of(d, up);
-            if (a.kl_coef != 0.0f) {
-                total += a.kl_coef * kl;
-                slope -= a.kl_coef * up;
-            }
-        }
-        loss = w * total;
-        const float coeff = static_cast<float>(w * slope * a.scale);
-        // a row whose gradient is 0 is written without a second look at its logits
-        g = RowGradient{-coeff * r.inv_total, coeff * r.rest, r.top, coeff != 0.0f};
-    }
-    if (put) {
-        if (a.logp) a.logp[row] = counts ? static_cast<float>(r.logp) : 0.0f;
-        if (a.kl) a.kl[row] = static_cast<float>(kl);
-        a.loss[row] = static_cast<float>(loss);
-    }
-    return g;
+__device__ __forceinline__ PolicyRow policy_inputs(const PolicyArgs<IO> &a, int64_t row, int label, float at_label) {
+    return PolicyRow{a.advantage[row], a.weight ? a.weight[row] : 1.0f, a.old_logp ? a.old_logp[row] : 0.0f,
+                     a.ref_logp ? a.ref_logp[row] : 0.0f, at_label, label};
 }
+struct PolicyOptions {
+    float scale;
+    Scale c;
+    float clip_low, clip_high, kl_coef;
+    int cols;
+    bool old, ref;
+};
+template <int IO>
+__device__ __forceinline__ PolicyOptions options_of(const PolicyArgs<IO> &a) {
+    return PolicyOptions{a.scale, a.c, a.clip_low, a.clip_high, a.kl_coef, a.cols, a.old_logp != nullptr, a.ref_logp != nullptr};
+}
+struct PolicyResult {
+    float logp, kl, loss;
+    RowGradient gradient;
+};
+// One thread's work for a row that counts: p is the pair of the other columns.
+__device__ __forceinline__ PolicyResult policy_row(const PolicyOptions &o, const PolicyRow &in, Pair p) {
+    const RowScore r = in.label < o.cols ? score_row(p, in.at_label, o.scale, o.c) : nan_score();
+    const double adv = in.advantage, w = in.weight;
+    const double ratio = o.old ? expf(static_cast<float>(r.logp - static_cast<double>(in.old_logp))) : 1.0 + 0.0 * r.logp;
+    const double low = 1.0 - o.clip_low, high = 1.0 + o.clip_high;
+    double kept = ratio, slope = -adv * ratio;
+    if (adv > 0.0 ? ratio > high : ratio < low) {
+        kept = adv > 0.0 ? high : low;
+        slope = 0.0;
+    }
+    if (adv == 0.0) slope = kept = 0.0;  // (no surrogate, however large the ratio)
+    double total = -adv * kept;
+    float kl = 0.0f;
+    if (o.ref) {
+        const float d = static_cast<float>(static_cast<double>(in.ref_logp) - r.logp);
+        const float up = expm1f(d);
+        kl = kl_of(d, up);
+        if (o.kl_coef != 0.0f) {
+            total += static_cast<double>(o.kl_coef) * kl;
+            slope -= static_cast<double>(o.kl_coef) * up;
+        }
+    }
+    const float coeff = static_cast<float>(w * slope * o.scale);
+    // a row whose gradient is 0 is written without a second look at its logits
+    return PolicyResult{static_cast<float>(r.logp), kl, static_cast<float>(w * total),
+                        RowGradient{-coeff * r.inv_total, coeff * r.rest, r.top, coeff != 0.0f}};
+}
+// The same as a call.  Inlined into a loop over rows its constants are loaded once, ahead of the loop, into some fifty
+// registers - of the ones that policy_onchip_kernel holds its row in.
+__device__ __attribute__((noinline)) PolicyResult policy_row_call(const PolicyOptions &o, const PolicyRow &in, Pair p) {
+    return policy_row(o, in, p);
+}
+template <int IO>
+__device__ __forceinline__ void put_policy(const PolicyArgs<IO> &a, int64_t row, const PolicyResult &r) {
+    if (a.logp) a.logp[row] = r.logp;
+    if (a.kl) a.kl[row] = r.kl;
+    a.loss[row] = r.loss;
+}
+__device__ __forceinline__ PolicyResult no_policy() { return PolicyResult{0.0f, 0.0f, 0.0f, RowGradient{0.0f, 0.0f, 0.0f, false}}; }
 
 // One workgroup per row, any length and alignment: the sums, then a second read.
 template <int IO, int THREADS>
@@ -482,20 +550,24 @@ __global__ __launch_bounds__(THREADS) void policy_reread_kernel(PolicyArgs<IO> a
         const typename Io<IO>::elem *src = a.logits + row * a.ld;
         const RowSpan<IO> span = span_of<IO>(src, a.cols);
         if (counts) {
-            RowScore r = nan_score();
+            float at_label = 0.0f;
+            Pair p{-FLT_MAX, 0.0f};
             if (label < a.cols) {
-                const float at_label = Io<IO>::scalar(src + label);
-                const Pair p = block_pair<THREADS / 64>(
-                    thread_pair<IO, THREADS>(src, span, 0, span.nvec, true, label, a.c), slots[turn], a.c);
-                if (threadIdx.x == 0) r = score_row(p, at_label, a.scale, a.c);
+                at_label = Io<IO>::scalar(src + label);
+                p = block_pair<THREADS / 64>(thread_pair<IO, THREADS>(src, span, 0, span.nvec, true, label, a.c), slots[turn],
+                                             a.c);
             }
-            if (threadIdx.x == 0) shared[turn] = policy_row(a, row, true, r, true);
+            if (threadIdx.x == 0) {
+                const PolicyResult r = policy_row(options_of(a), policy_inputs(a, row, label, at_label), p);
+                put_policy(a, row, r);
+                shared[turn] = r.gradient;
+            }
             __syncthreads();
         } else if (threadIdx.x == 0) {
-            policy_row(a, row, false, nan_score(), true);
+            put_policy(a, row, no_policy());
         }
         if (!a.dlogits) continue;
-        const RowGradient g = counts ? shared[turn] : RowGradient{0.0f, 0.0f, 0.0f, false};
+        const RowGradient g = counts ? uniform_gradient(shared[turn]) : RowGradient{0.0f, 0.0f, 0.0f, false};
         const auto label_grad = [&](float) { return g.label_grad; };
         write_gradient<IO, THREADS>(src, a.dlogits + row * a.ldd, span, 0, span.nvec, true, g.live, label, g.top, g.a,
                                     label_grad, a.c);
@@ -511,14 +583,19 @@ __global__ __launch_bounds__(THREADS) void policy_pieces_kernel(PolicyArgs<IO> a
     int label;
     const bool counts = policy_row_counts(a, row, label);
     if (threadIdx.x == 0) {
-        RowScore r = nan_score();
+        PolicyResult r = no_policy();
         const Pair *mine = pairs + row * (1 + parts);
-        if (counts && label < a.cols) r = score_row(fold_pieces(mine, parts, a.c), mine[0].m, a.scale, a.c);
-        shared = policy_row(a, row, counts, r, part == 0);
+        if (counts) {
+            Pair p{-FLT_MAX, 0.0f};
+            if (label < a.cols) p = fold_pieces(mine, parts, a.c);
+            r = policy_row(options_of(a), policy_inputs(a, row, label, label < a.cols ? mine[0].m : 0.0f), p);
+        }
+        if (part == 0) put_policy(a, row, r);
+        shared = r.gradient;
     }
     __syncthreads();
     if (!a.dlogits) return;
-    const RowGradient g = shared;
+    const RowGradient g = uniform_gradient(shared);
     const typename Io<IO>::elem *src = a.logits + row * a.ld;
     const RowSpan<IO> span = span_of<IO>(src, a.cols);
     const int piece = (span.nvec + parts - 1) / parts;
@@ -529,118 +606,156 @@ __global__ __launch_bounds__(THREADS) void policy_pieces_kernel(PolicyArgs<IO> a
                                 a.c);
 }
 
-// One workgroup per row at a time, the row in its registers, VPT vectors per thread: one read, one write.  While a row's
-// gradient is written the next row is loaded into the registers it leaves, so the workgroup always has loads or stores on
-// their way but for the two reductions.
-template <int IO, int THREADS, int VPT>
+// One workgroup per row at a time, the row in its registers, VPT vectors per thread: one read, one write.  A workgroup walks
+// over rows; vector k of a row's gradient goes out, then vector k of the next row comes into the registers that it left, and
+// LAG vectors later that one enters the next row's sum, so that the arithmetic of both rows (sixteen operations per value, four
+// times a quarter-rate exponential among them) runs under the memory's time.  No access in the exchange is made under a
+// condition (see load_whole): threads past the row's last vector take that one again and store what its own thread does.
+// LINES: rows of whole 64-byte lines.
+template <int IO, int THREADS, int VPT, bool LINES>
 __global__ __launch_bounds__(THREADS) void policy_onchip_kernel(PolicyArgs<IO> a) {
     constexpr int E = Io<IO>::E;
+    constexpr int LAG = VPT >= 8 ? 4 : (VPT + 1) / 2;
     typedef typename Io<IO>::elem Elem;
     __shared__ Pair slots[2][THREADS / 64];
     __shared__ RowGradient shared[2];
 
+    // a row as this thread sees it
+    struct Row {
+        int64_t row;
+        int label, label_k, in_vecs;  // label_k: which of the threads' vectors holds the label (VPT: none)
+        RowSpan<IO> span;
+        float single, at_label;
+        const Elem *vecs;
+    };
+    auto enter = [&](int64_t row, int label) {
+        Row w;
+        const Elem *src = a.logits + row * a.ld;
+        w.row = row;
+        w.label = label;
+        w.span = span_of<IO>(src, a.cols);
+        w.in_vecs = label - w.span.head;
+        w.label_k = w.in_vecs >= 0 && w.in_vecs < w.span.nvec * E ? w.in_vecs / E / THREADS : VPT;
+        w.vecs = src + w.span.head;
+        w.single = -INFINITY;
+        w.at_label = 0.0f;
+        if (static_cast<int>(threadIdx.x) < w.span.singles) w.single = Io<IO>::scalar(src + single_column(w.span, threadIdx.x));
+        if (threadIdx.x == 0 && label < a.cols) w.at_label = Io<IO>::scalar(src + label);
+        return w;
+    };
+    // the first row from `row` on that counts (or a.rows); the ones before it get zeros
+    auto next_row = [&](int64_t row, int &label) {
+        for (; row < a.rows; row += gridDim.x) {
+            if (policy_row_counts(a, row, label)) break;
+            if (threadIdx.x == 0) put_policy(a, row, no_policy());
+            Elem *dst = a.dlogits + row * a.ldd;
+            const RowSpan<IO> span = span_of<IO>(dst, a.cols);
+            write_gradient<IO, THREADS>(dst, dst, span, 0, span.nvec, true, false, -1, 0.0f, 0.0f, [](float) { return 0.0f; }, a.c);
+        }
+        return uniform(row);
+    };
+    // vector k of this thread in a row; the dispatch leaves rows of (VPT - 2) THREADS vectors and more to it, so that only
+    // the last two can lie past the row's end.  (Formed from one register at every use, instead of kept for every k.)
+    int thread = threadIdx.x;
+    auto own_vec = [&](int k) {
+        asm volatile("" : "+v"(thread));
+        return thread + k * THREADS;
+    };
+    auto vec_of = [&](const Row &w, int k) {
+        const int j = own_vec(k);
+        return k + 2 < VPT ? j : (j < w.span.nvec ? j : w.span.nvec - 1);
+    };
     typename Io<IO>::raw r[VPT];
-    float single = -INFINITY, at_label = 0.0f;
-    int label;
-    bool counts, reads;
-    RowSpan<IO> span;
-    auto enter = [&](int64_t row) {  // (the row's scalars; rows past the last one count for nothing)
-        counts = false;
-        label = -1;
-        if (row < a.rows) counts = policy_row_counts(a, row, label);
-        reads = counts && label < a.cols;
-        span = span_of<IO>(a.logits + (row < a.rows ? row : 0) * a.ld, a.cols);
-        single = -INFINITY;
-        if (reads) {
-            const Elem *src = a.logits + row * a.ld;
-            if (static_cast<int>(threadIdx.x) < span.singles)
-                single = Io<IO>::scalar(src + single_column(span, threadIdx.x));
-            if (threadIdx.x == 0) at_label = Io<IO>::scalar(src + label);
-        }
+    auto load_vec = [&](const Row &w, int k, uint32_t mask) {
+        r[k] = Io<IO>::template load_raw<true>(byte_offset(w.vecs, Io<IO>::kBytes * static_cast<uint32_t>(vec_of(w, k)) & mask));
+        asm volatile("" ::: "memory");
     };
-    auto load_vec = [&](int64_t row, int k) {
-        const int j = threadIdx.x + k * THREADS;
-        r[k] = typename Io<IO>::raw{};
-        if (reads && j < span.nvec)
-            r[k] = Io<IO>::template load_raw<true>(byte_offset(a.logits + row * a.ld + span.head, Io<IO>::kBytes * j));
+    auto add_vec = [&](const Row &w, int k, Pair &p) {
+        // (in this order: conversions of later vectors moved ahead would take the registers of a second row)
+        asm volatile("" : "+v"(r[k]), "+v"(p.s));
+        const int j = own_vec(k);
+        float x[E];
+        Io<IO>::unpack(r[k], x);
+        if (w.label_k == k) {  // (the same in every lane)
+#pragma unroll
+            for (int e = 0; e < E; ++e) x[e] = E * j + e == w.in_vecs ? -INFINITY : x[e];
+        }
+        if (k + 2 >= VPT) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) x[e] = j < w.span.nvec ? x[e] : -INFINITY;
+        }
+        add_values(p, x, a.c);
     };
-    enter(blockIdx.x);
+    // vector k's gradient, to dst's vectors
+    auto put_vec = [&](const Row &w, const RowGradient &g, Elem *dst, int k) {
+        convert_again<IO>(r[k]);
+        const int j = vec_of(w, k);
+        float x[E];
+        Io<IO>::unpack(r[k], x);
+        // (a row that counts and has no gradient, g.a = 0, has finite statistics: its products are 0)
 #pragma unroll
-    for (int k = 0; k < VPT; ++k) load_vec(blockIdx.x, k);
-
-    int turn = 0;
-    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
-        const int in_vecs = label - span.head;
-        const int label_vec = in_vecs >= 0 ? in_vecs / E : -1;
-        RowGradient g{0.0f, 0.0f, 0.0f, false};
-        if (counts) {
-            RowScore score = nan_score();
-            if (reads) {
-                Pair p{-FLT_MAX, 0.0f};
-                constexpr int GROUP = 32 / E < VPT ? 32 / E : VPT;  // vectors whose sum is rescaled together
-                static_assert(VPT % GROUP == 0, "");
+        for (int e = 0; e < E; ++e) x[e] = g.a * exp_scaled(x[e] - g.top, a.c);
+        if (w.label_k == k) {
 #pragma unroll
-                for (int k0 = 0; k0 < VPT; k0 += GROUP) {
-                    float v[GROUP * E];
-                    // one group after the other: all of them converted at once would be twice the row's registers
-#pragma unroll
-                    for (int u = 0; u < GROUP; ++u) asm volatile("" : "+v"(r[k0 + u]), "+v"(p.s));
-#pragma unroll
-                    for (int u = 0; u < GROUP; ++u) {
-                        const int j = threadIdx.x + (k0 + u) * THREADS;
-                        float x[E];
-                        Io<IO>::unpack(r[k0 + u], x);
-                        if (j >= span.nvec || j == label_vec) {
-#pragma unroll
-                            for (int e = 0; e < E; ++e)
-                                if (j >= span.nvec || E * j + e == in_vecs) x[e] = -INFINITY;
-                        }
-#pragma unroll
-                        for (int e = 0; e < E; ++e) v[u * E + e] = x[e];
-                    }
-                    add_values(p, v, a.c);
-                }
-                const bool one_more = static_cast<int>(threadIdx.x) < span.singles && single_column(span, threadIdx.x) != label;
-                const float v[1] = {one_more ? single : -INFINITY};
-                add_values(p, v, a.c);
-                p = block_pair<THREADS / 64>(p, slots[turn], a.c);
-                if (threadIdx.x == 0) score = score_row(p, at_label, a.scale, a.c);
-            }
-            if (threadIdx.x == 0) shared[turn] = policy_row(a, row, true, score, true);
-            __syncthreads();
-            g = shared[turn];
-        } else if (threadIdx.x == 0) {
-            policy_row(a, row, false, nan_score(), true);
+            for (int e = 0; e < E; ++e) x[e] = E * j + e == w.in_vecs ? g.label_grad : x[e];
         }
-        // this row's gradient out, the next row in
-        const RowSpan<IO> here = span;
-        const int here_label = label;
-        const float here_single = single;
-        const int64_t next = row + gridDim.x;
-        enter(next);
-        Elem *dst = a.dlogits + row * a.ldd;
-        Elem *dst_vecs = dst + here.head;
-        const bool whole_lines = (reinterpret_cast<uintptr_t>(dst_vecs) & 63) == 0;
-        const auto label_grad = [&](float) { return g.label_grad; };
-#pragma unroll
-        for (int k = 0; k < VPT; ++k) {
-            const int j = threadIdx.x + k * THREADS;
-            if (j < here.nvec) {
-                float x[E];
-                convert_again<IO>(r[k]);
-                Io<IO>::unpack(r[k], x);
-                gradient_of(x, E * j, g.live, in_vecs, j == label_vec, g.top, g.a, label_grad, a.c);
-                store_row_vec<IO>(whole_lines, dst_vecs, Io<IO>::kBytes * static_cast<uint32_t>(j), x);
-            }
-            load_vec(next, k);
-        }
-        if (static_cast<int>(threadIdx.x) < here.singles) {
+        store_vec<IO, LINES>(dst, Io<IO>::kBytes * static_cast<uint32_t>(j), x);
+        asm volatile("" ::: "memory");
+    };
+    auto put_single = [&](const Row &w, const RowGradient &g, Elem *dst) {
+        if (static_cast<int>(threadIdx.x) < w.span.singles) {
             constexpr int ONE = io_by_element(IO);
-            const int column = single_column(here, threadIdx.x);
+            const int column = single_column(w.span, threadIdx.x);
             float x[1] = {0.0f};
-            if (g.live) x[0] = column == here_label ? g.label_grad : g.a * exp_scaled(here_single - g.top, a.c);
+            if (g.live) x[0] = column == w.label ? g.label_grad : g.a * exp_scaled(w.single - g.top, a.c);
             Io<ONE>::template store<true>(dst + column, x);
         }
+    };
+
+    int label = -1;
+    int64_t row = next_row(blockIdx.x, label);
+    if (row >= a.rows) return;
+    Row cur = enter(row, label);
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) load_vec(cur, k, ~0u);
+    Pair p{-FLT_MAX, 0.0f};
+#pragma unroll
+    for (int k = 0; k < VPT - LAG; ++k) add_vec(cur, k, p);
+
+    for (int turn = 0;; turn ^= 1) {
+        // the rest of the row's sum, and what it makes of the row
+#pragma unroll
+        for (int k = VPT - LAG; k < VPT; ++k) add_vec(cur, k, p);
+        {
+            const bool one_more = static_cast<int>(threadIdx.x) < cur.span.singles && single_column(cur.span, threadIdx.x) != cur.label;
+            const float v[1] = {one_more ? cur.single : -INFINITY};
+            add_values(p, v, a.c);
+        }
+        p = block_pair<THREADS / 64>(p, slots[turn], a.c);
+        if (threadIdx.x == 0) {
+            const PolicyResult res = policy_row_call(options_of(a), policy_inputs(a, cur.row, cur.label, cur.at_label), p);
+            put_policy(a, cur.row, res);
+            shared[turn] = res.gradient;
+        }
+        row = next_row(cur.row + gridDim.x, label);
+        __syncthreads();
+        const RowGradient g = uniform_gradient(shared[turn]);
+        Elem *dst = a.dlogits + cur.row * a.ldd;
+        put_single(cur, g, dst);
+        // Behind the last row the exchange goes on loading - the same 16 bytes every time - for nothing: a way out of the
+        // loop with the row in registers would have the compiler keep two rows there.
+        const bool more = row < a.rows;
+        const Row next = more ? enter(row, label) : cur;
+        const uint32_t mask = more ? ~0u : 0u;
+        p = Pair{-FLT_MAX, 0.0f};
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) {
+            put_vec(cur, g, dst + cur.span.head, k);
+            load_vec(next, k, mask);
+            if (k >= LAG) add_vec(next, k - LAG, p);
+        }
+        if (!more) return;
+        cur = next;
     }
 }
 
@@ -759,6 +874,15 @@ size_t workspace_bytes(int64_t rows, int64_t cols) {
     return parts > 1 ? static_cast<size_t>(rows) * (1 + parts) * sizeof(Pair) : 0;
 }
 
+Scale two_parts(float scale) {
+    const double c = static_cast<double>(scale) * 1.4426950408889634;
+    float hi = static_cast<float>(c);
+    if (hi > c) hi = nextafterf(hi, 0.0f);
+    // (lo > 0: -inf times either part is -inf)
+    const float lo = static_cast<float>(c - hi);
+    return Scale{hi, lo > 1e-37f ? lo : 1e-37f};
+}
+
 unsigned row_grid(int64_t rows) { return static_cast<unsigned>(rows > 0x7fffffff ? 0x7fffffff : rows); }
 
 // What every entry on rows of logits checks.
@@ -767,7 +891,7 @@ int check_logits(const char *who, const void *logits, int64_t ld, const void *la
     if (rows < 0 || cols <= 0) return fail(KO_ERR_INVALID_ARGUMENT, "%s: rows=%lld cols=%lld", who, (long long)rows, (long long)cols);
     if (cols > (1 << 30)) return fail(KO_ERR_UNSUPPORTED_SHAPE, "%s: cols=%lld too large", who, (long long)cols);
     if (ld < cols) return fail(KO_ERR_INVALID_ARGUMENT, "%s: ld=%lld is less than cols=%lld", who, (long long)ld, (long long)cols);
-    if (!(scale >= 1e-30f && scale <= 1e30f)) return fail(KO_ERR_INVALID_ARGUMENT, "%s: scale=%g", who, static_cast<double>(scale));
+    if (!(scale >= 1e-20f && scale <= 1e20f)) return fail(KO_ERR_INVALID_ARGUMENT, "%s: scale=%g", who, static_cast<double>(scale));
     if (rows > 0 && (!logits || !labels)) return fail(KO_ERR_INVALID_ARGUMENT, "%s: null logits/labels pointer", who);
     if ((reinterpret_cast<uintptr_t>(logits) & (size - 1)) || (reinterpret_cast<uintptr_t>(labels) & 3))
         return fail(KO_ERR_INVALID_ARGUMENT, "%s: logits/labels must be aligned to their element type", who);
@@ -796,7 +920,7 @@ bool rows_lie_alike(const void *logits, int64_t ld, const void *dlogits, int64_t
 
 template <int IO, int THREADS>
 int launch_pieces(const typename Io<IO>::elem *logits, int64_t ld, const int32_t *labels, const float *weight, int64_t rows,
-                  int cols, float c, Pair *pairs, int parts, hipStream_t stream) {
+                  int cols, Scale c, Pair *pairs, int parts, hipStream_t stream) {
     token_pieces_kernel<IO, THREADS><<<dim3(static_cast<unsigned>(parts), static_cast<unsigned>(rows)), dim3(THREADS), 0, stream>>>(
         logits, ld, labels, weight, cols, c, pairs);
     KO_CHECK_LAUNCH();
@@ -812,7 +936,7 @@ int logprob_entry(const void *logits, int64_t ld, const int32_t *labels, float s
     if (const int st = check_floats(who, {logp, row_stats}); st != KO_OK) return st;
     if (rows == 0) return KO_OK;
     if (!logp) return fail(KO_ERR_INVALID_ARGUMENT, "%s: null logp pointer", who);
-    const ScoreArgs<IO> a{static_cast<const Elem *>(logits), ld, labels, scale, scale * kLog2e, logp, row_stats, rows,
+    const ScoreArgs<IO> a{static_cast<const Elem *>(logits), ld, labels, scale, two_parts(scale), logp, row_stats, rows,
                           static_cast<int>(cols), as_stream(stream)};
     const int parts = pieces_per_row(rows, cols);
     if (workspace && parts > 1) {
@@ -841,7 +965,7 @@ int launch_logprob_backward(const void *logits, int64_t ld, const int32_t *label
     const unsigned parts = static_cast<unsigned>((cols + piece - 1) / piece);
     const unsigned grid_rows = static_cast<unsigned>(rows > 65535 ? 65535 : rows);
     token_logprob_backward_kernel<IO, THREADS><<<dim3(parts, grid_rows), dim3(THREADS), 0, stream>>>(
-        static_cast<const Elem *>(logits), ld, labels, scale, scale * kLog2e, row_stats, dlogp, static_cast<Elem *>(dlogits), ldd,
+        static_cast<const Elem *>(logits), ld, labels, scale, two_parts(scale), row_stats, dlogp, static_cast<Elem *>(dlogits), ldd,
         rows, static_cast<int>(cols));
     KO_CHECK_LAUNCH();
     return KO_OK;
@@ -866,10 +990,12 @@ int logprob_backward_entry(const void *logits, int64_t ld, const int32_t *labels
 template <int IO, int THREADS, int VPT>
 int launch_onchip(const PolicyArgs<IO> &a) {
     // as many workgroups as are resident at once walk over the rows
-    constexpr int kPerUnit = THREADS * VPT <= 1024 * 4 ? 4096 / (THREADS * VPT) * 2 : THREADS * VPT <= 1024 * 8 ? 2 : 1;
-    int64_t grid = static_cast<int64_t>(compute_units()) * (kPerUnit * THREADS > 2048 ? 2048 / THREADS : kPerUnit);
+    int64_t grid = static_cast<int64_t>(compute_units()) * (1024 / THREADS);
     if (grid > a.rows) grid = a.rows;
-    policy_onchip_kernel<IO, THREADS, VPT><<<dim3(static_cast<unsigned>(grid)), dim3(THREADS), 0, a.stream>>>(a);
+    const dim3 g(static_cast<unsigned>(grid)), b(THREADS);
+    const bool lines = ((reinterpret_cast<uintptr_t>(a.dlogits) | static_cast<uintptr_t>(a.ldd) * sizeof(typename Io<IO>::elem)) & 63) == 0;
+    if (lines) policy_onchip_kernel<IO, THREADS, VPT, true><<<g, b, 0, a.stream>>>(a);
+    else policy_onchip_kernel<IO, THREADS, VPT, false><<<g, b, 0, a.stream>>>(a);
     KO_CHECK_LAUNCH();
     return KO_OK;
 }
@@ -888,13 +1014,21 @@ int launch_policy(const PolicyArgs<IO> &a, void *workspace) {
         return KO_OK;
     }
     if constexpr (Io<IO>::E > 1) {
+        // (a row has one whole vector at least from 2 E - 1 columns on, wherever it starts)
         const int nvec = a.cols / Io<IO>::E;
-        if (a.dlogits) {
+        if (a.dlogits && a.cols >= 2 * Io<IO>::E) {
+            if (nvec <= 256) return launch_onchip<IO, 256, 1>(a);
             if (nvec <= 512) return launch_onchip<IO, 256, 2>(a);
             if (nvec <= 1024) return launch_onchip<IO, 256, 4>(a);
             if (nvec <= 2048) return launch_onchip<IO, 512, 4>(a);
-            if (nvec <= 4096) return launch_onchip<IO, 1024, 4>(a);
+            if (nvec <= 3072) return launch_onchip<IO, 512, 6>(a);
+            if (nvec <= 4096) return launch_onchip<IO, 512, 8>(a);
+            if (nvec <= 6144) return launch_onchip<IO, 1024, 6>(a);
             if (nvec <= 8192) return launch_onchip<IO, 1024, 8>(a);
+            if (nvec <= 10240) return launch_onchip<IO, 1024, 10>(a);
+            if (nvec <= 12288) return launch_onchip<IO, 1024, 12>(a);
+            if (nvec <= 14336) return launch_onchip<IO, 1024, 14>(a);
+            if (nvec <= 16384) return launch_onchip<IO, 1024, 16>(a);
         }
     }
     const dim3 grid(row_grid(a.rows));
@@ -932,7 +1066,7 @@ int policy_entry(const void *logits, int64_t ld, const int32_t *labels, const fl
     auto run = [&](auto kind) {
         constexpr int KIND = decltype(kind)::value;
         const PolicyArgs<KIND> a{static_cast<const Elem *>(logits), ld, labels, old_logp, ref_logp, advantage, weight, scale,
-                                 scale * kLog2e, clip_low, clip_high, kl_coef, logp, kl, loss, static_cast<Elem *>(dlogits), ldd,
+                                 two_parts(scale), clip_low, clip_high, kl_coef, logp, kl, loss, static_cast<Elem *>(dlogits), ldd,
                                  rows, static_cast<int>(cols), s};
         return launch_policy<KIND>(a, workspace);
     };
