@@ -608,16 +608,22 @@ __global__ __launch_bounds__(THREADS) void policy_pieces_kernel(PolicyArgs<IO> a
 
 // One workgroup per row at a time, the row in its registers, VPT vectors per thread: one read, one write.  A workgroup walks
 // over rows; vector k of a row's gradient goes out, then vector k of the next row comes into the registers that it left, and
-// LAG vectors later that one enters the next row's sum, so that the arithmetic of both rows (sixteen operations per value, four
-// times a quarter-rate exponential among them) runs under the memory's time.  No access in the exchange is made under a
-// condition (see load_whole): threads past the row's last vector take that one again and store what its own thread does.
+// LAG vectors later that one enters the next row's sum, so that the arithmetic of both rows runs under the memory's time.  No
+// access in the exchange is made under a condition (see load_whole): threads past the row's last vector take that one again
+// and store what its own thread does.
+// Arithmetic is what bounds a sum with a running maximum here (a quarter-rate exponential and ten more operations per value
+// in the sum, eight in the gradient, 16 us per row of 128256 where the memory takes 20).  So exponentials are taken against
+// the label's logit instead, known when the row is entered: exp(scale (x - x_l)) = 2^(c x - c x_l) is one fused multiply-add
+// and the exponential, logp = -log1p of their sum.  A label so unlikely that this sum reaches 2^40, or not a number, is summed
+// again from the registers, against the maximum.
 // LINES: rows of whole 64-byte lines.
 template <int IO, int THREADS, int VPT, bool LINES>
 __global__ __launch_bounds__(THREADS) void policy_onchip_kernel(PolicyArgs<IO> a) {
     constexpr int E = Io<IO>::E;
     constexpr int LAG = VPT >= 8 ? 4 : (VPT + 1) / 2;
     typedef typename Io<IO>::elem Elem;
-    __shared__ Pair slots[2][THREADS / 64];
+    __shared__ float sums[2][THREADS / 64][1];
+    __shared__ Pair slots[THREADS / 64];
     __shared__ RowGradient shared[2];
 
     // a row as this thread sees it
@@ -625,7 +631,7 @@ __global__ __launch_bounds__(THREADS) void policy_onchip_kernel(PolicyArgs<IO> a
         int64_t row;
         int label, label_k, in_vecs;  // label_k: which of the threads' vectors holds the label (VPT: none)
         RowSpan<IO> span;
-        float single, at_label;
+        float single, at_label, k;    // k: c.hi times the reference's logit
         const Elem *vecs;
     };
     auto enter = [&](int64_t row, int label) {
@@ -638,9 +644,9 @@ __global__ __launch_bounds__(THREADS) void policy_onchip_kernel(PolicyArgs<IO> a
         w.label_k = w.in_vecs >= 0 && w.in_vecs < w.span.nvec * E ? w.in_vecs / E / THREADS : VPT;
         w.vecs = src + w.span.head;
         w.single = -INFINITY;
-        w.at_label = 0.0f;
         if (static_cast<int>(threadIdx.x) < w.span.singles) w.single = Io<IO>::scalar(src + single_column(w.span, threadIdx.x));
-        if (threadIdx.x == 0 && label < a.cols) w.at_label = Io<IO>::scalar(src + label);
+        w.at_label = label < a.cols ? Io<IO>::scalar(src + label) : 0.0f;
+        w.k = w.at_label * a.c.hi;
         return w;
     };
     // the first row from `row` on that counts (or a.rows); the ones before it get zeros
@@ -670,11 +676,9 @@ __global__ __launch_bounds__(THREADS) void policy_onchip_kernel(PolicyArgs<IO> a
         r[k] = Io<IO>::template load_raw<true>(byte_offset(w.vecs, Io<IO>::kBytes * static_cast<uint32_t>(vec_of(w, k)) & mask));
         asm volatile("" ::: "memory");
     };
-    auto add_vec = [&](const Row &w, int k, Pair &p) {
-        // (in this order: conversions of later vectors moved ahead would take the registers of a second row)
-        asm volatile("" : "+v"(r[k]), "+v"(p.s));
+    // vector k's values, -inf at the label and past the row's end
+    auto others = [&](const Row &w, int k, float (&x)[E]) {
         const int j = own_vec(k);
-        float x[E];
         Io<IO>::unpack(r[k], x);
         if (w.label_k == k) {  // (the same in every lane)
 #pragma unroll
@@ -684,32 +688,42 @@ __global__ __launch_bounds__(THREADS) void policy_onchip_kernel(PolicyArgs<IO> a
 #pragma unroll
             for (int e = 0; e < E; ++e) x[e] = j < w.span.nvec ? x[e] : -INFINITY;
         }
-        add_values(p, x, a.c);
     };
-    // vector k's gradient, to dst's vectors
-    auto put_vec = [&](const Row &w, const RowGradient &g, Elem *dst, int k) {
+    auto other_single = [&](const Row &w) {
+        return static_cast<int>(threadIdx.x) < w.span.singles && single_column(w.span, threadIdx.x) != w.label ? w.single : -INFINITY;
+    };
+    auto power = [&](const Row &w, float x) {
+        return __builtin_amdgcn_exp2f(__builtin_fmaf(x, a.c.lo, __builtin_fmaf(x, a.c.hi, -w.k)));
+    };
+    auto add_vec = [&](const Row &w, int k, float &sum) {
+        // (in this order: conversions of later vectors moved ahead would take the registers of a second row)
+        asm volatile("" : "+v"(r[k]), "+v"(sum));
+        float x[E];
+        others(w, k, x);
+        float s[4];
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const float p = power(w, x[e]);
+            if (e < 4) s[e] = p;
+            else s[e % 4] += p;
+        }
+        sum += (s[0] + s[1]) + (s[2] + s[3]);
+    };
+    // vector k's gradient, to dst's vectors: factor 2^(c x - k)
+    auto put_vec = [&](const Row &w, float factor, float label_grad, Elem *dst, int k) {
         convert_again<IO>(r[k]);
         const int j = vec_of(w, k);
         float x[E];
         Io<IO>::unpack(r[k], x);
-        // (a row that counts and has no gradient, g.a = 0, has finite statistics: its products are 0)
+        // (a row that counts and has no gradient, factor 0, has finite powers: its products are 0)
 #pragma unroll
-        for (int e = 0; e < E; ++e) x[e] = g.a * exp_scaled(x[e] - g.top, a.c);
-        if (w.label_k == k) {
+        for (int e = 0; e < E; ++e) x[e] = factor * __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], a.c.hi, -w.k));
+        if (k + 2 >= VPT || w.label_k == k) {  // (the last vector may come by in the threads past it, too)
 #pragma unroll
-            for (int e = 0; e < E; ++e) x[e] = E * j + e == w.in_vecs ? g.label_grad : x[e];
+            for (int e = 0; e < E; ++e) x[e] = E * j + e == w.in_vecs ? label_grad : x[e];
         }
         store_vec<IO, LINES>(dst, Io<IO>::kBytes * static_cast<uint32_t>(j), x);
         asm volatile("" ::: "memory");
-    };
-    auto put_single = [&](const Row &w, const RowGradient &g, Elem *dst) {
-        if (static_cast<int>(threadIdx.x) < w.span.singles) {
-            constexpr int ONE = io_by_element(IO);
-            const int column = single_column(w.span, threadIdx.x);
-            float x[1] = {0.0f};
-            if (g.live) x[0] = column == w.label ? g.label_grad : g.a * exp_scaled(w.single - g.top, a.c);
-            Io<ONE>::template store<true>(dst + column, x);
-        }
     };
 
     int label = -1;
@@ -718,20 +732,34 @@ __global__ __launch_bounds__(THREADS) void policy_onchip_kernel(PolicyArgs<IO> a
     Row cur = enter(row, label);
 #pragma unroll
     for (int k = 0; k < VPT; ++k) load_vec(cur, k, ~0u);
-    Pair p{-FLT_MAX, 0.0f};
+    float sum = 0.0f;
 #pragma unroll
-    for (int k = 0; k < VPT - LAG; ++k) add_vec(cur, k, p);
+    for (int k = 0; k < VPT - LAG; ++k) add_vec(cur, k, sum);
 
     for (int turn = 0;; turn ^= 1) {
         // the rest of the row's sum, and what it makes of the row
 #pragma unroll
-        for (int k = VPT - LAG; k < VPT; ++k) add_vec(cur, k, p);
-        {
-            const bool one_more = static_cast<int>(threadIdx.x) < cur.span.singles && single_column(cur.span, threadIdx.x) != cur.label;
-            const float v[1] = {one_more ? cur.single : -INFINITY};
+        for (int k = VPT - LAG; k < VPT; ++k) add_vec(cur, k, sum);
+        sum += power(cur, other_single(cur));
+        float total[1] = {sum};
+        block_sum<THREADS / 64, 1>(total, sums[turn]);
+        // 2^(c x_l - k): what k lacks of c times the reference
+        const float lack = __builtin_amdgcn_exp2f(-__builtin_fmaf(cur.at_label, a.c.lo, __builtin_fmaf(cur.at_label, a.c.hi, -cur.k)));
+        Pair p{cur.at_label, total[0] * lack};
+        if (!(uniform(p.s) < 0x1p40f) || cur.label >= a.cols) {
+            // against the maximum: an unlikely label, special values, or logits that c times overflows
+            p = Pair{-FLT_MAX, 0.0f};
+#pragma unroll
+            for (int k = 0; k < VPT; ++k) {
+                asm volatile("" : "+v"(r[k]), "+v"(p.s));
+                float x[E];
+                others(cur, k, x);
+                add_values(p, x, a.c);
+            }
+            const float v[1] = {other_single(cur)};
             add_values(p, v, a.c);
+            p = block_pair<THREADS / 64>(p, slots, a.c);
         }
-        p = block_pair<THREADS / 64>(p, slots[turn], a.c);
         if (threadIdx.x == 0) {
             const PolicyResult res = policy_row_call(options_of(a), policy_inputs(a, cur.row, cur.label, cur.at_label), p);
             put_policy(a, cur.row, res);
@@ -740,19 +768,45 @@ __global__ __launch_bounds__(THREADS) void policy_onchip_kernel(PolicyArgs<IO> a
         row = next_row(cur.row + gridDim.x, label);
         __syncthreads();
         const RowGradient g = uniform_gradient(shared[turn]);
+        if (g.top != cur.at_label || !(fabsf(cur.k) < 1e30f)) {
+            // the reference is the maximum now; one whose multiple by c might overflow is taken off the values
+            cur.k = g.top * a.c.hi;
+            if (!(fabsf(cur.k) < 1e30f)) {
+#pragma unroll
+                for (int k = 0; k < VPT; ++k) {
+                    asm volatile("" : "+v"(r[k]));
+                    float x[E];
+                    Io<IO>::unpack(r[k], x);
+#pragma unroll
+                    for (int e = 0; e < E; ++e) x[e] -= g.top;
+                    r[k] = pack<IO>(x);
+                }
+                cur.single -= g.top;
+                cur.k = 0.0f;
+            }
+        }
+        // (c.lo makes no difference to what is rounded here)
+        const float reference = cur.k == 0.0f ? 0.0f : g.top;
+        const float factor = g.a * __builtin_amdgcn_exp2f(-__builtin_fmaf(reference, a.c.hi, -cur.k));
         Elem *dst = a.dlogits + cur.row * a.ldd;
-        put_single(cur, g, dst);
+        if (static_cast<int>(threadIdx.x) < cur.span.singles) {
+            constexpr int ONE = io_by_element(IO);
+            const int column = single_column(cur.span, threadIdx.x);
+            const float x[1] = {column == cur.label ? g.label_grad
+                                                    : factor * __builtin_amdgcn_exp2f(__builtin_fmaf(cur.single, a.c.hi, -cur.k))};
+            Io<ONE>::template store<true>(dst + column, x);
+        }
         // Behind the last row the exchange goes on loading - the same 16 bytes every time - for nothing: a way out of the
         // loop with the row in registers would have the compiler keep two rows there.
         const bool more = row < a.rows;
         const Row next = more ? enter(row, label) : cur;
         const uint32_t mask = more ? ~0u : 0u;
-        p = Pair{-FLT_MAX, 0.0f};
+        sum = 0.0f;
 #pragma unroll
         for (int k = 0; k < VPT; ++k) {
-            put_vec(cur, g, dst + cur.span.head, k);
+            put_vec(cur, factor, g.label_grad, dst + cur.span.head, k);
             load_vec(next, k, mask);
-            if (k >= LAG) add_vec(next, k - LAG, p);
+            if (k >= LAG) add_vec(next, k - LAG, sum);
         }
         if (!more) return;
         cur = next;

@@ -356,3 +356,57 @@ def test_preference_loss_no_pairs(ko):
     ko.preference_loss(None, None, None, 0, 0, None, loss_sum=total.ptr)
     ko.synchronize()
     assert total.get(np.float32, (1,))[0] == 0.0
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows,cols", [(5, 40), (300, 333), (300, 9001)])
+def test_policy_loss_unlikely_labels_and_lowest_values(ko, rows, cols, kind):
+    """Labels far below the row's maximum, rows of nothing but the type's lowest value, and a label that is -inf."""
+    call = Call(ko, rows, cols, kind, 3600)
+    lowest = {"f32": np.finfo(np.float32).min, "f16": -65504.0, "bf16": -3.3895314e38}[kind]
+    x = call.values.copy()
+    live = np.flatnonzero(call.labels >= 0)
+    r = np.arange(rows)
+    x[live, call.labels[live]] -= np.array([0.0, 20.0, 28.0, 60.0])[live % 4]
+    x[live[0]] = lowest                                       # a uniform distribution
+    x[live[1], :] = lowest                                    # all but two columns masked
+    x[live[1], [call.labels[live[1]], (call.labels[live[1]] + 1) % cols]] = [1.0, 2.0]
+    stored, values = ref.to_storage(x, kind)
+    call.keep.upload(stored)
+    call.values = values
+    call.stored = stored
+    call.scores = ref.Scores(values, call.labels)
+    case = policy_case(call, 11)
+    check_policy(call, run_policy(call, case, 0), case)
+    # the label's own logit is -inf: logp is, too, and with no pull from its reference the gradient is finite
+    x = stored.copy()
+    x[live[2], call.labels[live[2]]] = {"f32": -np.inf, "f16": 0xFC00, "bf16": 0xFF80}[kind]
+    call.keep.upload(x)
+    case["ref"] = None
+    got = run_policy(call, case, 0, kl_coef=0.0)
+    assert got["logp"][live[2]] == -np.inf
+    assert np.isfinite(ref.to_float(np.ascontiguousarray(got["dlogits"]), kind)[live]).all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows,cols", [(7, 19), (300, 333), (300, 2050), (270, 9001), (260, 33000)])
+def test_labels_in_the_first_and_last_columns(ko, rows, cols, kind):
+    """Where rows start off a vector the first and last columns are taken one by one, and where a workgroup has more threads
+    than the row has vectors the last vector is written by several."""
+    call = Call(ko, rows, cols, kind, 3700)
+    at = np.arange(rows) % 18
+    alive = call.labels >= 0
+    call.labels[alive] = np.where(at < 9, at, cols - 1 - (at - 9))[alive]
+    x = np.nan_to_num(call.values, nan=0.0, neginf=-5.0)
+    x = np.where(x < -100.0, -5.0, x)
+    x[np.arange(rows), np.maximum(call.labels, 0)] += 3.0
+    call.stored, call.values = ref.to_storage(x, kind)
+    call.keep.upload(call.stored)
+    call.d_labels.upload(call.labels)
+    call.scores = ref.Scores(call.values, call.labels)
+    case = policy_case(call, 12)
+    check_policy(call, run_policy(call, case, 0), case)
+    call.check_logprob()
+    dlogp = inputs.normal_f32((rows,), 3701)
+    want = call.scores.gradient(dlogp.astype(np.float64), 0.0, 3 * ref.U * np.abs(call.scores.logsum) + 2 * ref.U)
+    call.check_gradient(call.backward(dlogp, 0), want)
