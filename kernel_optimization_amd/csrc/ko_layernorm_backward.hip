@@ -609,7 +609,7 @@ int dispatch(const Args<IO> &a, bool whole) {
     if (nvec <= 1024) return launch_rows_any<IO, 512, 2>(a, whole);
     if (nvec <= 2048) return launch_rows_any<IO, 1024, 2>(a, whole);
     if constexpr (Io<IO>::E == 4) {
-        if (nvec <= 3072) return launch_rows_any<IO, 1024, 3>(a, whole);
+        if (nvec <= 3 * 1024) return launch_rows_any<IO, 1024, 3>(a, whole);
         if (nvec <= 4096) return launch_rows_any<IO, 1024, 4>(a, whole);
     }
     return whole ? launch_long<IO, 1024, false>(a) : launch_long<IO, 1024, true>(a);

@@ -137,6 +137,23 @@ __device__ __forceinline__ void store_whole(typename Io<IO>::elem *base, uint32_
     }
 }
 
+// Buffer accesses of 16 bytes at base + offset, dropped (loads: zeros, nothing is fetched) where offset + 16 passes `bytes`:
+// what takes the place of a condition in such kernels.  `base` and `bytes` are the same in every lane.
+typedef __amdgpu_buffer_rsrc_t Buffer;
+__device__ __forceinline__ Buffer buffer_of(const void *base, uint32_t bytes) {
+    constexpr int kRaw32Bit = 0x00027000;  // resource word 3: raw buffer, 32-bit data
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), 0, bytes, kRaw32Bit);
+}
+template <int IO>
+__device__ __forceinline__ typename Io<IO>::raw buffer_load(Buffer b, uint32_t offset) {
+    return __builtin_bit_cast(typename Io<IO>::raw, __builtin_amdgcn_raw_buffer_load_b128(b, offset, 0, 2 /* nt */));
+}
+// LINES: part of whole 64-byte lines, written through at once (see store_row_vec)
+template <int IO, bool LINES>
+__device__ __forceinline__ void buffer_store(Buffer b, uint32_t offset, const float (&v)[Io<IO>::E]) {
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(uint4v, pack<IO>(v)), b, offset, 0, LINES ? 2 | 16 /* nt sc1 */ : 2);
+}
+
 // Sum over a workgroup of WAVES wavefronts of N values at once: wave all-reduces, then every thread folds the
 // per-wave partials in wave order (the same bits in every thread).  One barrier: `slot` is not written again before
 // every wave has passed the workgroup's next barrier (callers alternate between two slots).

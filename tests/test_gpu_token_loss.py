@@ -410,3 +410,16 @@ def test_labels_in_the_first_and_last_columns(ko, rows, cols, kind):
     dlogp = inputs.normal_f32((rows,), 3701)
     want = call.scores.gradient(dlogp.astype(np.float64), 0.0, 3 * ref.U * np.abs(call.scores.logsum) + 2 * ref.U)
     call.check_gradient(call.backward(dlogp, 0), want)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("vectors", [1, 2, 63, 64, 65, 128, 129, 257, 260, 319, 513, 1025, 1537, 2049, 3 * 1024 + 1, 4097, 5121, 6145,
+                                     8193, 10241, 12289, 14337, 16384, 16385])
+def test_policy_loss_where_one_way_ends_and_the_next_begins(ko, vectors, kind):
+    """Rows of one 16-byte vector more than the last shape of a workgroup takes, whole and with single elements around them."""
+    per = 4 if kind == "f32" else 8
+    for pad, skew, more in ((0, 0, 0), (3, 4, per - 1), (0, 0, -1)):
+        call = Call(ko, 4, vectors * per + more, kind, 3800 + vectors, pad, skew, False)
+        case = policy_case(call, vectors)
+        got = run_policy(call, case, pad)
+        check_policy(call, got, case)
