@@ -8,9 +8,11 @@
 // 1 + S it would be rounded away.  Gradient of c * logp:  dx_j = -c scale exp(scale (x_j - m)) / (S + e) for j != l, and
 // c scale S / (S + e) for the label.
 //
-// Rows.  A row of logits starts anywhere (ld elements after the last one): its columns are a head of up to E - 1
-// elements up to the first 16-byte boundary, whole 16-byte vectors, and a tail.  Head and tail elements are taken one by
-// one by the first threads; the vectors carry the row.  So a vocabulary of 50257 contiguous columns runs on vectors, too.
+// Rows.  A row of logits starts anywhere (ld elements after the last one): its columns are a head up to the first 128-byte
+// boundary, whole 16-byte vectors, and a tail.  Head and tail elements are taken one by one by the first threads; the
+// vectors carry the row, and what they write are whole lines of the caches, which no two workgroups share (1 GiB of rows of
+// 50272 bf16 columns, their odd ones 64 bytes into a line: gradient 383 us with vectors from 64-byte boundaries on).  So a
+// vocabulary of 50257 contiguous columns runs on vectors, too.
 //
 // Bound: memory.  The sums are one pass with a running maximum; the policy loss keeps the whole row in a workgroup's
 // registers between the sum and the gradient, so that the logits are read once and the gradient written once.
@@ -42,7 +44,7 @@ __device__ __forceinline__ int64_t uniform(int64_t v) {
 // ---- a row's columns
 template <int IO>
 struct RowSpan {
-    int head;     // single elements before the first vector
+    int head;     // single elements before the first vector, up to a 128-byte boundary
     int nvec;     // vectors, from column `head` on
     int singles;  // single elements in all: the head, and what is left after the last vector
 };
@@ -55,8 +57,9 @@ __device__ __forceinline__ RowSpan<IO> span_of(const typename Io<IO>::elem *row,
         s.nvec = cols;
         s.singles = 0;
     } else {
-        const int past = static_cast<int>((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(typename Io<IO>::elem));
-        s.head = (E - past) % E;
+        constexpr int LINE = 128 / static_cast<int>(sizeof(typename Io<IO>::elem));
+        const int past = static_cast<int>((reinterpret_cast<uintptr_t>(row) & 127) / sizeof(typename Io<IO>::elem));
+        s.head = (LINE - past) % LINE;
         if (s.head > cols) s.head = cols;
         s.nvec = (cols - s.head) / E;
         s.singles = cols - s.nvec * E;
@@ -67,6 +70,12 @@ __device__ __forceinline__ RowSpan<IO> span_of(const typename Io<IO>::elem *row,
 template <int IO>
 __device__ __forceinline__ int single_column(const RowSpan<IO> &s, int i) {
     return i < s.head ? i : s.nvec * Io<IO>::E + i;
+}
+
+// Where the part-th of `parts` pieces of n vectors begins: pieces are whole 128-byte lines, and the last ones may be empty.
+__device__ __forceinline__ int piece_begin(int n, int parts, int part) {
+    const int64_t at = static_cast<int64_t>(((n + parts - 1) / parts + 7) & ~7) * part;
+    return at < n ? static_cast<int>(at) : n;
 }
 
 // ---- running (maximum, sum of exp(scale (x - maximum)))
@@ -160,10 +169,12 @@ __device__ __forceinline__ Pair thread_pair(const typename Io<IO>::elem *row, co
         }
         add_values(p, v, c);
     }
-    if (with_singles && static_cast<int>(threadIdx.x) < span.singles) {
-        const int column = single_column(span, threadIdx.x);
-        const float v[1] = {column == label ? -INFINITY : Io<IO>::scalar(row + column)};
-        add_values(p, v, c);
+    if (with_singles) {
+        for (int i = threadIdx.x; i < span.singles; i += THREADS) {
+            const int column = single_column(span, i);
+            const float v[1] = {column == label ? -INFINITY : Io<IO>::scalar(row + column)};
+            add_values(p, v, c);
+        }
     }
     return p;
 }
@@ -249,8 +260,6 @@ __device__ __forceinline__ void write_gradient(const typename Io<IO>::elem *row,
     Elem *out_vecs = out + span.head;
     const int in_vecs = label - span.head;
     const int label_vec = in_vecs >= 0 ? in_vecs / E : -1;
-    // whole lines are written through (see store_row_vec)
-    const bool whole_lines = (reinterpret_cast<uintptr_t>(out_vecs) & 63) == 0;
     for (int j0 = lo + static_cast<int>(threadIdx.x); j0 < hi; j0 += THREADS * UNROLL) {
         typename Io<IO>::raw r[UNROLL];
 #pragma unroll
@@ -266,13 +275,13 @@ __device__ __forceinline__ void write_gradient(const typename Io<IO>::elem *row,
             float x[E];
             Io<IO>::unpack(r[u], x);
             gradient_of(x, E * j, live, in_vecs, j == label_vec, top, a, label_grad, c);
-            store_row_vec<IO>(whole_lines, out_vecs, Io<IO>::kBytes * static_cast<uint32_t>(j), x);
+            store_row_vec<IO>(E > 1, out_vecs, Io<IO>::kBytes * static_cast<uint32_t>(j), x);
         }
     }
     if constexpr (E > 1) {
-        if (with_singles && static_cast<int>(threadIdx.x) < span.singles) {
+        for (int i = threadIdx.x; with_singles && i < span.singles; i += THREADS) {
             constexpr int ONE = io_by_element(IO);
-            const int column = single_column(span, threadIdx.x);
+            const int column = single_column(span, i);
             float x[1] = {0.0f};
             if (live) {
                 x[0] = Io<IO>::scalar(row + column);
@@ -308,23 +317,105 @@ __device__ __forceinline__ void put_score(const A &a, int64_t row, bool live, co
     }
 }
 
-// One workgroup per row.
-template <int IO, int THREADS>
+// One workgroup per row, the next batch of U vectors per thread in flight while this one is added up.  As in
+// policy_onchip_kernel the exponentials are taken against the label's logit, and the row's maximum is noted by the way; a label
+// so unlikely that the sum reaches 2^40, or a sum that is not a number, is summed again with a running maximum.
+template <int IO, int THREADS, int U>
 __global__ __launch_bounds__(THREADS) void token_logprob_row_kernel(ScoreArgs<IO> a) {
-    __shared__ Pair slots[2][THREADS / 64];
+    constexpr int E = Io<IO>::E;
+    constexpr int WAVES = THREADS / 64;
+    typedef typename Io<IO>::raw Raw;
+    __shared__ Pair slots[2][WAVES];
+    __shared__ Pair again[WAVES];
     int turn = 0;
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
+        const typename Io<IO>::elem *src = a.logits + row * a.ld;
+        const RowSpan<IO> span = span_of<IO>(src, a.cols);
         const int label = uniform(a.labels[row]);
-        RowScore r = nan_score();
-        if (label >= 0 && label < a.cols) {
-            const typename Io<IO>::elem *src = a.logits + row * a.ld;
-            const float at_label = Io<IO>::scalar(src + label);
-            const RowSpan<IO> span = span_of<IO>(src, a.cols);
-            const Pair p = block_pair<THREADS / 64>(thread_pair<IO, THREADS>(src, span, 0, span.nvec, true, label, a.c),
-                                                    slots[turn], a.c);
-            if (threadIdx.x == 0) r = score_row(p, at_label, a.scale, a.c);
+        if (label < 0 || label >= a.cols) {
+            if (threadIdx.x == 0) put_score(a, row, label >= 0, nan_score());
+            continue;
         }
-        if (threadIdx.x == 0) put_score(a, row, label >= 0, r);
+        // vectors past the row's end read as zeros, without traffic
+        const Buffer from = buffer_of(src + span.head, Io<IO>::kBytes * span.nvec);
+        const float at_label = Io<IO>::scalar(src + label);
+        const float shift = at_label * a.c.hi;
+        const int in_vecs = label - span.head;
+        const int label_vec = in_vecs >= 0 && in_vecs < span.nvec * E ? in_vecs / E : -1;
+        float top = at_label;
+        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        auto load = [&](Raw (&r)[U], int first) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) r[u] = buffer_load<IO>(from, Io<IO>::kBytes * static_cast<uint32_t>(first + u * THREADS));
+        };
+        auto add = [&](Raw (&r)[U], int first) {
+            const int begin = uniform(first - static_cast<int>(threadIdx.x));
+            // in this batch, the same in every lane: the label, or the row's end
+            const bool ragged = begin + U * THREADS > span.nvec || (label_vec >= begin && label_vec < begin + U * THREADS);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                float x[E];
+                Io<IO>::unpack(r[u], x);
+                if (ragged) {
+                    if (begin + u * THREADS >= span.nvec) break;
+                    const int j = first + u * THREADS;
+#pragma unroll
+                    for (int e = 0; e < E; ++e) x[e] = j >= span.nvec || E * j + e == in_vecs ? -INFINITY : x[e];
+                }
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    top = fmaxf(top, x[e]);
+                    s[e % 4] += __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], a.c.lo, __builtin_fmaf(x[e], a.c.hi, -shift)));
+                }
+            }
+        };
+        Raw r[2][U];
+        int j = static_cast<int>(threadIdx.x);
+        load(r[0], j);
+        while (true) {
+            load(r[1], j + U * THREADS);
+            add(r[0], j);
+            j += U * THREADS;
+            if (j - static_cast<int>(threadIdx.x) >= span.nvec) break;
+            load(r[0], j + U * THREADS);
+            add(r[1], j);
+            j += U * THREADS;
+            if (j - static_cast<int>(threadIdx.x) >= span.nvec) break;
+        }
+        for (int i = threadIdx.x; i < span.singles; i += THREADS) {
+            const int column = single_column(span, i);
+            const float x = column == label ? -INFINITY : Io<IO>::scalar(src + column);
+            top = fmaxf(top, x);
+            s[1] += __builtin_amdgcn_exp2f(__builtin_fmaf(x, a.c.lo, __builtin_fmaf(x, a.c.hi, -shift)));
+        }
+        top = wave::allreduce<64, wave::Max>(top);
+        float sum = wave::allreduce<64, wave::Sum>((s[0] + s[1]) + (s[2] + s[3]));
+        if constexpr (WAVES > 1) {
+            if ((threadIdx.x & 63) == 0) slots[turn][threadIdx.x >> 6] = Pair{top, sum};
+            __syncthreads();
+            top = slots[turn][0].m;
+            sum = slots[turn][0].s;
+#pragma unroll
+            for (int w = 1; w < WAVES; ++w) {
+                top = fmaxf(top, slots[turn][w].m);
+                sum += slots[turn][w].s;
+            }
+        }
+        // times 2^-(c x_l - shift): shift is c x_l rounded
+        sum *= __builtin_amdgcn_exp2f(-__builtin_fmaf(at_label, a.c.lo, __builtin_fmaf(at_label, a.c.hi, -shift)));
+        Pair p{at_label, sum};
+        if (!(uniform(sum) < 0x1p40f)) {
+            p = block_pair<WAVES>(thread_pair<IO, THREADS>(src, span, 0, span.nvec, true, label, a.c), again, a.c);
+            top = fmaxf(p.m, at_label);
+            __syncthreads();  // (read before the next row writes them)
+        }
+        if (threadIdx.x == 0) {
+            RowScore score = score_row(p, at_label, a.scale, a.c);
+            // the sum is relative to the label: its logarithm relative to the maximum
+            score.logsum += (static_cast<double>(score.top) - static_cast<double>(top)) * static_cast<double>(a.scale);
+            score.top = top;
+            put_score(a, row, true, score);
+        }
     }
 }
 
@@ -348,9 +439,7 @@ __global__ __launch_bounds__(THREADS) void token_pieces_kernel(const typename Io
     const typename Io<IO>::elem *src = logits + row * ld;
     const RowSpan<IO> span = span_of<IO>(src, cols);
     const int parts = static_cast<int>(gridDim.x), part = static_cast<int>(blockIdx.x);
-    const int piece = (span.nvec + parts - 1) / parts;
-    const int lo = part * piece < span.nvec ? part * piece : span.nvec;
-    const int hi = span.nvec - lo < piece ? span.nvec : lo + piece;
+    const int lo = piece_begin(span.nvec, parts, part), hi = piece_begin(span.nvec, parts, part + 1);
     const Pair p = block_pair<THREADS / 64>(thread_pair<IO, THREADS>(src, span, lo, hi, part == 0, label, c), slot, c);
     if (threadIdx.x == 0) {
         Pair *mine = pairs + row * (1 + parts);
@@ -358,23 +447,26 @@ __global__ __launch_bounds__(THREADS) void token_pieces_kernel(const typename Io
         mine[1 + part] = p;
     }
 }
+// by one wavefront, the same bits in every lane
 __device__ __forceinline__ Pair fold_pieces(const Pair *mine, int parts, Scale c) {
-    float m = mine[1].m;
-    for (int i = 2; i <= parts; ++i) m = fmaxf(m, mine[i].m);
-    float s = 0.0f;
-    for (int i = 1; i <= parts; ++i) s += mine[i].s * exp_sum(mine[i].m - m, c);
-    return Pair{m, s};
+    Pair p{-FLT_MAX, 0.0f};
+    for (int i = 1 + (threadIdx.x & 63); i <= parts; i += 64) {
+        const float m = fmaxf(p.m, mine[i].m);
+        p.s = p.s * exp_sum(p.m - m, c) + mine[i].s * exp_sum(mine[i].m - m, c);
+        p.m = m;
+    }
+    return block_pair<1>(p, nullptr, c);
 }
 
+// One wavefront per row.
 template <int IO>
 __global__ __launch_bounds__(64) void token_logprob_fold_kernel(ScoreArgs<IO> a, const Pair *__restrict__ pairs, int parts) {
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * 64 + threadIdx.x;
-    if (row >= a.rows) return;
-    const int label = a.labels[row];
+    const int64_t row = blockIdx.x;
+    const int label = uniform(a.labels[row]);
     RowScore r = nan_score();
     const Pair *mine = pairs + row * (1 + parts);
     if (label >= 0 && label < a.cols) r = score_row(fold_pieces(mine, parts, a.c), mine[0].m, a.scale, a.c);
-    put_score(a, row, label >= 0, r);
+    if (threadIdx.x == 0) put_score(a, row, label >= 0, r);
 }
 
 // Workgroup (p, row): a piece of the row's gradient.
@@ -395,9 +487,7 @@ __global__ __launch_bounds__(THREADS) void token_logprob_backward_kernel(const t
         Elem *dst = dlogits + row * ldd;
         const RowSpan<IO> span = span_of<IO>(dst, cols);
         const int parts = static_cast<int>(gridDim.x), part = static_cast<int>(blockIdx.x);
-        const int piece = (span.nvec + parts - 1) / parts;
-        const int lo = part * piece < span.nvec ? part * piece : span.nvec;
-        const int hi = span.nvec - lo < piece ? span.nvec : lo + piece;
+        const int lo = piece_begin(span.nvec, parts, part), hi = piece_begin(span.nvec, parts, part + 1);
         const float top = live ? uniform(row_stats[2 * row]) : 0.0f;
         const float logsum = live ? uniform(row_stats[2 * row + 1]) : 0.0f;
         const float a = -coeff * __builtin_amdgcn_exp2f(-logsum * kLog2e);
@@ -536,7 +626,7 @@ __global__ __launch_bounds__(THREADS) void policy_reread_kernel(PolicyArgs<IO> a
         int label;
         const bool counts = policy_row_counts(a, row, label);
         const typename Io<IO>::elem *src = a.logits + row * a.ld;
-        const RowSpan<IO> span = span_of<IO>(src, a.cols);
+        const RowSpan<IO> span = span_of<IO>(a.dlogits ? a.dlogits + row * a.ldd : src, a.cols);
         if (counts) {
             float at_label = 0.0f;
             Pair p{-FLT_MAX, 0.0f};
@@ -570,7 +660,7 @@ __global__ __launch_bounds__(THREADS) void policy_pieces_kernel(PolicyArgs<IO> a
     const int part = static_cast<int>(blockIdx.x);
     int label;
     const bool counts = policy_row_counts(a, row, label);
-    if (threadIdx.x == 0) {
+    if (threadIdx.x < 64) {
         PolicyResult r = no_policy();
         const Pair *mine = pairs + row * (1 + parts);
         if (counts) {
@@ -578,17 +668,17 @@ __global__ __launch_bounds__(THREADS) void policy_pieces_kernel(PolicyArgs<IO> a
             if (label < a.cols) p = fold_pieces(mine, parts, a.c);
             r = policy_row(options_of(a), policy_inputs(a, row, label, label < a.cols ? mine[0].m : 0.0f), p);
         }
-        if (part == 0) put_policy(a, row, r);
-        shared = r.gradient;
+        if (threadIdx.x == 0) {
+            if (part == 0) put_policy(a, row, r);
+            shared = r.gradient;
+        }
     }
     __syncthreads();
     if (!a.dlogits) return;
     const RowGradient g = uniform_gradient(shared);
     const typename Io<IO>::elem *src = a.logits + row * a.ld;
-    const RowSpan<IO> span = span_of<IO>(src, a.cols);
-    const int piece = (span.nvec + parts - 1) / parts;
-    const int lo = part * piece < span.nvec ? part * piece : span.nvec;
-    const int hi = span.nvec - lo < piece ? span.nvec : lo + piece;
+    const RowSpan<IO> span = span_of<IO>(a.dlogits + row * a.ldd, a.cols);
+    const int lo = piece_begin(span.nvec, parts, part), hi = piece_begin(span.nvec, parts, part + 1);
     const auto label_grad = [&](float) { return g.label_grad; };
     write_gradient<IO, THREADS>(src, a.dlogits + row * a.ldd, span, lo, hi, part == 0, g.live, label, g.top, g.a, label_grad,
                                 a.c);
@@ -601,13 +691,15 @@ __global__ __launch_bounds__(THREADS) void policy_pieces_kernel(PolicyArgs<IO> a
 // multiply-add and the exponential, a sum needs no running maximum, and logp = -log1p of it.  (With the maximum the arithmetic
 // of a row of 128256 took 20 us, as long as its memory traffic.)  A label so unlikely that the sum reaches 2^40, or not a
 // number, is summed again from the registers, against the maximum.
-// LINES: rows of whole 64-byte lines.  Rows have columns for more than ABOVE vectors: only a thread's last ones can lie past the
-// row's end.
-template <int IO, int ABOVE, int THREADS, int VPT, bool LINES>
+// Rows have columns for more than ABOVE vectors: only a thread's last ones can lie past the
+// row's end.  REST: rows longer than the registers.  What does not fit is added up before the registers fill, and read a second
+// time for its gradient.
+template <int IO, int ABOVE, int THREADS, int VPT, bool REST = false>
 __global__ __launch_bounds__(THREADS) void policy_onchip_kernel(PolicyArgs<IO> a) {
     constexpr int E = Io<IO>::E;
-    // (a row has at least one vector less than its columns make, so ABOVE of them)
-    constexpr int WHOLE = ABOVE / THREADS;
+    // (up to a 128-byte boundary a row loses less than eight of the vectors that its columns make: it has ABOVE - 7 at least)
+    constexpr int WHOLE = ABOVE < 7 ? 0 : (ABOVE - 7) / THREADS;
+    constexpr int SINGLES = (128 / static_cast<int>(sizeof(typename Io<IO>::elem)) + E - 2 + THREADS - 1) / THREADS;
     typedef typename Io<IO>::elem Elem;
     __shared__ float sums[THREADS / 64][1];
     __shared__ Pair slots[THREADS / 64];
@@ -616,7 +708,7 @@ __global__ __launch_bounds__(THREADS) void policy_onchip_kernel(PolicyArgs<IO> a
     if (row >= a.rows) return;
     const Elem *src = a.logits + row * a.ld;
     Elem *dst = a.dlogits + row * a.ldd;
-    const RowSpan<IO> span = span_of<IO>(src, a.cols);
+    const RowSpan<IO> span = span_of<IO>(dst, a.cols);
     int label;
     if (!policy_row_counts(a, row, label)) {
         if (threadIdx.x == 0) put_policy(a, row, no_policy());
@@ -633,16 +725,49 @@ __global__ __launch_bounds__(THREADS) void policy_onchip_kernel(PolicyArgs<IO> a
         return first + k * Io<IO>::kBytes * THREADS;
     };
     float at_label = label < a.cols ? Io<IO>::scalar(src + label) : 0.0f;
+    float shift = at_label * a.c.hi;
+    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    const int in_vecs = label - span.head;
+    constexpr int BATCH = 8;  // vectors per thread at a time of the rest
+    // the rest's vector at j, with the same exceptions as `others`
+    auto rest_others = [&](const typename Io<IO>::raw &v, int j, float (&x)[E]) {
+        Io<IO>::unpack(v, x);
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[e] = j >= span.nvec || E * j + e == in_vecs ? -INFINITY : x[e];
+    };
+    if constexpr (REST) {
+        for (int j = static_cast<int>(threadIdx.x) + THREADS * VPT; uniform(j) < span.nvec; j += BATCH * THREADS) {
+            typename Io<IO>::raw v[BATCH];
+#pragma unroll
+            for (int u = 0; u < BATCH; ++u) v[u] = buffer_load<IO>(from, Io<IO>::kBytes * static_cast<uint32_t>(j + u * THREADS));
+#pragma unroll
+            for (int u = 0; u < BATCH; ++u) {
+                if (uniform(j + u * THREADS) >= span.nvec) break;
+                float x[E];
+                rest_others(v[u], j + u * THREADS, x);
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    s[e % 4] += __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], a.c.lo, __builtin_fmaf(x[e], a.c.hi, -shift)));
+            }
+        }
+    }
     typename Io<IO>::raw r[VPT];
 #pragma unroll
     for (int k = 0; k < VPT; ++k) r[k] = buffer_load<IO>(from, offset_of(k));
-    float single = -INFINITY;
-    const bool has_single = static_cast<int>(threadIdx.x) < span.singles;
-    if (has_single) single = Io<IO>::scalar(src + single_column(span, threadIdx.x));
+    float single[SINGLES];
+    bool has_single[SINGLES];
+    int column[SINGLES];
+#pragma unroll
+    for (int i = 0; i < SINGLES; ++i) {
+        const int at = static_cast<int>(threadIdx.x) + i * THREADS;
+        has_single[i] = at < span.singles;
+        column[i] = single_column(span, at);
+        single[i] = -INFINITY;
+        if (has_single[i]) single[i] = Io<IO>::scalar(src + column[i]);
+    }
     PolicyRow in{};
     if (threadIdx.x == 0) in = policy_inputs(a, row, label, at_label);
 
-    const int in_vecs = label - span.head;
     // which of the threads' vectors holds the label (VPT: none)
     const int label_k = in_vecs >= 0 && in_vecs < span.nvec * E ? in_vecs / E / THREADS : VPT;
     // vector k's values, -inf at the label and past the row's end
@@ -658,9 +783,7 @@ __global__ __launch_bounds__(THREADS) void policy_onchip_kernel(PolicyArgs<IO> a
             for (int e = 0; e < E; ++e) x[e] = j < span.nvec ? x[e] : -INFINITY;
         }
     };
-    const float other_single = has_single && single_column(span, threadIdx.x) != label ? single : -INFINITY;
-    float shift = at_label * a.c.hi;
-    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    auto other_single = [&](int i) { return has_single[i] && column[i] != label ? single[i] : -INFINITY; };
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
         // (in this order: vectors converted ahead would take the registers of a second row)
@@ -671,7 +794,9 @@ __global__ __launch_bounds__(THREADS) void policy_onchip_kernel(PolicyArgs<IO> a
         for (int e = 0; e < E; ++e)
             s[e % 4] += __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], a.c.lo, __builtin_fmaf(x[e], a.c.hi, -shift)));
     }
-    s[1] += __builtin_amdgcn_exp2f(__builtin_fmaf(other_single, a.c.lo, __builtin_fmaf(other_single, a.c.hi, -shift)));
+#pragma unroll
+    for (int i = 0; i < SINGLES; ++i)
+        s[i % 4] += __builtin_amdgcn_exp2f(__builtin_fmaf(other_single(i), a.c.lo, __builtin_fmaf(other_single(i), a.c.hi, -shift)));
     float total[1] = {(s[0] + s[1]) + (s[2] + s[3])};
     block_sum<THREADS / 64, 1>(total, sums);
     // times 2^-(c x_l - shift): shift is c x_l rounded
@@ -686,8 +811,18 @@ __global__ __launch_bounds__(THREADS) void policy_onchip_kernel(PolicyArgs<IO> a
             others(k, x);
             add_values(p, x, a.c);
         }
-        const float v[1] = {other_single};
-        add_values(p, v, a.c);
+        if constexpr (REST) {
+            for (int j = static_cast<int>(threadIdx.x) + THREADS * VPT; uniform(j) < span.nvec; j += THREADS) {
+                float x[E];
+                rest_others(buffer_load<IO>(from, Io<IO>::kBytes * static_cast<uint32_t>(j)), j, x);
+                add_values(p, x, a.c);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < SINGLES; ++i) {
+            const float v[1] = {other_single(i)};
+            add_values(p, v, a.c);
+        }
         p = block_pair<THREADS / 64>(p, slots, a.c);
     }
     if (threadIdx.x == 0) {
@@ -697,7 +832,7 @@ __global__ __launch_bounds__(THREADS) void policy_onchip_kernel(PolicyArgs<IO> a
     }
     __syncthreads();
     const RowGradient g = uniform_gradient(shared);
-    float reference = g.top;
+    float reference = g.top, less = 0.0f;
     if (g.top != at_label || !(fabsf(shift) < 1e30f)) {
         // the reference is the maximum; one whose multiple by c might overflow is taken off the values
         shift = g.top * a.c.hi;
@@ -711,7 +846,9 @@ __global__ __launch_bounds__(THREADS) void policy_onchip_kernel(PolicyArgs<IO> a
                 for (int e = 0; e < E; ++e) x[e] -= g.top;
                 r[k] = pack<IO>(x);
             }
-            single -= g.top;
+#pragma unroll
+            for (int i = 0; i < SINGLES; ++i) single[i] -= g.top;
+            less = g.top;
             reference = shift = 0.0f;
         }
     }
@@ -730,14 +867,35 @@ __global__ __launch_bounds__(THREADS) void policy_onchip_kernel(PolicyArgs<IO> a
 #pragma unroll
             for (int e = 0; e < E; ++e) x[e] = E * j + e == in_vecs ? g.label_grad : x[e];
         }
-        buffer_store<IO, LINES>(to, offset_of(k), x);
+        buffer_store<IO, true>(to, offset_of(k), x);
     }
-    if (has_single) {
-        constexpr int ONE = io_by_element(IO);
-        const int column = single_column(span, threadIdx.x);
-        const float x[1] = {column == label ? g.label_grad
-                                            : factor * __builtin_amdgcn_exp2f(__builtin_fmaf(single, a.c.hi, -shift))};
-        Io<ONE>::template store<true>(dst + column, x);
+    if constexpr (REST) {
+        for (int j = static_cast<int>(threadIdx.x) + THREADS * VPT; uniform(j) < span.nvec; j += BATCH * THREADS) {
+            typename Io<IO>::raw v[BATCH];
+#pragma unroll
+            for (int u = 0; u < BATCH; ++u) v[u] = buffer_load<IO>(from, Io<IO>::kBytes * static_cast<uint32_t>(j + u * THREADS));
+#pragma unroll
+            for (int u = 0; u < BATCH; ++u) {
+                const int at = j + u * THREADS;
+                if (uniform(at) >= span.nvec) break;
+                float x[E];
+                Io<IO>::unpack(v[u], x);
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    x[e] = E * at + e == in_vecs ? g.label_grad
+                                                 : factor * __builtin_amdgcn_exp2f(__builtin_fmaf(x[e] - less, a.c.hi, -shift));
+                buffer_store<IO, true>(to, Io<IO>::kBytes * static_cast<uint32_t>(at), x);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < SINGLES; ++i) {
+        if (has_single[i]) {
+            constexpr int ONE = io_by_element(IO);
+            const float x[1] = {column[i] == label ? g.label_grad
+                                                   : factor * __builtin_amdgcn_exp2f(__builtin_fmaf(single[i], a.c.hi, -shift))};
+            Io<ONE>::template store<true>(dst + column[i], x);
+        }
     }
 }
 
@@ -841,17 +999,22 @@ __global__ __launch_bounds__(kPreferenceThreads) void preference_kernel(Preferen
 }
 
 // ---------------------------------------------------------------------------------------------------- dispatch
-// Pieces per row of a few rows: a function of the sizes alone, so that the workspace can be sized without a device.
+constexpr int64_t kMaxColumns = 1 << 28;  // bytes of a row are counted in 32 bits
+
+// Pieces per row of a few long rows: a function of the sizes alone, so that the workspace can be sized without a device.  Below
+// 48K columns a workgroup per row takes less time than a second launch (16 rows of 30522 fp32 columns 6.0 us against 7.7, with
+// the policy loss 7.3 against 9.4; 32 rows of 50257 bf16 columns 7.2 against 7.7 and 9.6 against 9.8); 16 rows of 100000 take
+// 8.8 us whole and 7.7 in pieces, the policy loss 12.5 and 9.2.  128 rows are enough workgroups of their own (13 us against 21).
 constexpr int kPieceUnits = 256;  // compute units of an MI355X
 constexpr int64_t kPieceColumns = 4096;
+constexpr int64_t kWholeColumns = 48 << 10;
 int pieces_per_row(int64_t rows, int64_t cols) {
-    if (rows <= 0 || rows * 2 > kPieceUnits) return 1;
-    int64_t parts = 2 * kPieceUnits / rows;
-    if (parts > cols / kPieceColumns) parts = cols / kPieceColumns;
-    return parts < 2 ? 1 : static_cast<int>(parts);
+    if (rows <= 0 || rows * 4 > kPieceUnits || cols <= kWholeColumns) return 1;
+    const int64_t parts = 2 * kPieceUnits / rows;
+    return static_cast<int>(parts < cols / kPieceColumns ? parts : cols / kPieceColumns);
 }
 size_t workspace_bytes(int64_t rows, int64_t cols) {
-    if (rows <= 0 || cols <= 0 || cols > (1 << 30)) return 0;
+    if (rows <= 0 || cols <= 0 || cols > kMaxColumns) return 0;
     const int parts = pieces_per_row(rows, cols);
     return parts > 1 ? static_cast<size_t>(rows) * (1 + parts) * sizeof(Pair) : 0;
 }
@@ -872,7 +1035,7 @@ unsigned row_grid(int64_t rows) { return static_cast<unsigned>(rows > (1 << 21) 
 int check_logits(const char *who, const void *logits, int64_t ld, const void *labels, size_t size, float scale, int64_t rows,
                  int64_t cols, const void *workspace, size_t bytes) {
     if (rows < 0 || cols <= 0) return fail(KO_ERR_INVALID_ARGUMENT, "%s: rows=%lld cols=%lld", who, (long long)rows, (long long)cols);
-    if (cols > (1 << 30)) return fail(KO_ERR_UNSUPPORTED_SHAPE, "%s: cols=%lld too large", who, (long long)cols);
+    if (cols > kMaxColumns) return fail(KO_ERR_UNSUPPORTED_SHAPE, "%s: cols=%lld too large", who, (long long)cols);
     if (ld < cols) return fail(KO_ERR_INVALID_ARGUMENT, "%s: ld=%lld is less than cols=%lld", who, (long long)ld, (long long)cols);
     if (!(scale >= 1e-20f && scale <= 1e20f)) return fail(KO_ERR_INVALID_ARGUMENT, "%s: scale=%g", who, static_cast<double>(scale));
     if (rows > 0 && (!logits || !labels)) return fail(KO_ERR_INVALID_ARGUMENT, "%s: null logits/labels pointer", who);
@@ -926,14 +1089,18 @@ int logprob_entry(const void *logits, int64_t ld, const int32_t *labels, float s
         Pair *pairs = static_cast<Pair *>(workspace);
         if (const int st = launch_pieces<IO, 256>(a.logits, ld, labels, nullptr, rows, a.cols, a.c, pairs, parts, a.stream); st != KO_OK)
             return st;
-        token_logprob_fold_kernel<IO><<<dim3(static_cast<unsigned>((rows + 63) / 64)), dim3(64), 0, a.stream>>>(a, pairs, parts);
+        token_logprob_fold_kernel<IO><<<dim3(static_cast<unsigned>(rows)), dim3(64), 0, a.stream>>>(a, pairs, parts);
         KO_CHECK_LAUNCH();
         return KO_OK;
     }
     const dim3 grid(row_grid(rows));
-    if (cols <= 4096) token_logprob_row_kernel<IO, 256><<<grid, dim3(256), 0, a.stream>>>(a);
-    else if (cols <= 32768 || rows >= 1024) token_logprob_row_kernel<IO, 512><<<grid, dim3(512), 0, a.stream>>>(a);
-    else token_logprob_row_kernel<IO, 1024><<<grid, dim3(1024), 0, a.stream>>>(a);
+    const int nvec = a.cols / Io<IO>::E;
+    if (nvec <= 128) token_logprob_row_kernel<IO, 64, 2><<<grid, dim3(64), 0, a.stream>>>(a);
+    else if (nvec <= 256) token_logprob_row_kernel<IO, 64, 4><<<grid, dim3(64), 0, a.stream>>>(a);
+    else if (nvec <= 512) token_logprob_row_kernel<IO, 128, 4><<<grid, dim3(128), 0, a.stream>>>(a);
+    else if (nvec <= 1024) token_logprob_row_kernel<IO, 256, 4><<<grid, dim3(256), 0, a.stream>>>(a);
+    else if (nvec <= 4096 || rows >= 1024) token_logprob_row_kernel<IO, 512, 4><<<grid, dim3(512), 0, a.stream>>>(a);
+    else token_logprob_row_kernel<IO, 1024, 4><<<grid, dim3(1024), 0, a.stream>>>(a);
     KO_CHECK_LAUNCH();
     return KO_OK;
 }
@@ -970,19 +1137,17 @@ int logprob_backward_entry(const void *logits, int64_t ld, const int32_t *labels
                                                       as_stream(stream));
 }
 
-template <int IO, int ABOVE, int THREADS, int VPT>
+template <int IO, int ABOVE, int THREADS, int VPT, bool REST = false>
 int launch_onchip(const PolicyArgs<IO> &a) {
-    static_assert(ABOVE < THREADS * VPT, "");
+    static_assert(REST ? ABOVE >= THREADS * VPT + 7 : ABOVE < THREADS * VPT, "");
     const int nvec = a.cols / Io<IO>::E;
-    if (nvec <= ABOVE || nvec > THREADS * VPT) return fail(KO_ERR_UNSUPPORTED_SHAPE, "policy_loss: cols=%d", a.cols);
+    if ((ABOVE && nvec <= ABOVE) || (!REST && nvec > THREADS * VPT)) return fail(KO_ERR_UNSUPPORTED_SHAPE, "policy_loss: cols=%d", a.cols);
     // (a grid's threads number less than 2^32 in one dimension)
     const int64_t wide = a.rows < (1 << 20) ? a.rows : (1 << 20);
     const int64_t high = (a.rows + wide - 1) / wide;
     if (high > 65535) return fail(KO_ERR_UNSUPPORTED_SHAPE, "policy_loss: rows=%lld too many", (long long)a.rows);
     const dim3 g(static_cast<unsigned>(wide), static_cast<unsigned>(high)), b(THREADS);
-    const bool lines = ((reinterpret_cast<uintptr_t>(a.dlogits) | static_cast<uintptr_t>(a.ldd) * sizeof(typename Io<IO>::elem)) & 63) == 0;
-    if (lines) policy_onchip_kernel<IO, ABOVE, THREADS, VPT, true><<<g, b, 0, a.stream>>>(a);
-    else policy_onchip_kernel<IO, ABOVE, THREADS, VPT, false><<<g, b, 0, a.stream>>>(a);
+    policy_onchip_kernel<IO, ABOVE, THREADS, VPT, REST><<<g, b, 0, a.stream>>>(a);
     KO_CHECK_LAUNCH();
     return KO_OK;
 }
@@ -1001,9 +1166,8 @@ int launch_policy(const PolicyArgs<IO> &a, void *workspace) {
         return KO_OK;
     }
     if constexpr (Io<IO>::E > 1) {
-        // (a row has one whole vector at least from 2 E - 1 columns on, wherever it starts)
         const int nvec = a.cols / Io<IO>::E;
-        if (a.dlogits && a.cols >= 2 * Io<IO>::E) {
+        if (a.dlogits) {
             // Four vectors per thread, where the rows fit a workgroup that way: 4096 bf16 columns 338 us for 1 GiB of logits
             // against 356 with eight and 372 with two per thread, 1024 columns 393 against 675 with one.  Long rows: 512 threads
             // (two workgroups per compute unit, one of which loads or stores) as far as their registers go, 49152 columns
@@ -1024,6 +1188,7 @@ int launch_policy(const PolicyArgs<IO> &a, void *workspace) {
             if (nvec <= 12 * 1024) return launch_onchip<IO, 10 * 1024, 1024, 12>(a);
             if (nvec <= 14 * 1024) return launch_onchip<IO, 12 * 1024, 1024, 14>(a);
             if (nvec <= 16 * 1024) return launch_onchip<IO, 14 * 1024, 1024, 16>(a);
+            return launch_onchip<IO, 16 * 1024, 1024, 15, true>(a);
         }
     }
     // no gradient, rows that lie differently in the two matrices, a row or two's vectors, and rows longer than the registers
