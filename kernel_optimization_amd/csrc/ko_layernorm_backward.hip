@@ -584,8 +584,7 @@ int launch_rows_any(const Args<IO> &a, bool whole) {
 template <int IO, int THREADS, bool RAGGED>
 int launch_long(const Args<IO> &a) {
     if (const int st = launch_columns(a); st != KO_OK) return st;  // (dx may overwrite dy or x)
-    const int64_t grid = a.rows > 0x7fffffff ? 0x7fffffff : a.rows;
-    layernorm_backward_reread_kernel<IO, THREADS, RAGGED><<<dim3(static_cast<unsigned>(grid)), dim3(THREADS), 0, a.stream>>>(a);
+    layernorm_backward_reread_kernel<IO, THREADS, RAGGED><<<row_grid(a.rows, THREADS), dim3(THREADS), 0, a.stream>>>(a);
     KO_CHECK_LAUNCH();
     return KO_OK;
 }
@@ -616,7 +615,7 @@ int dispatch(const Args<IO> &a, bool whole) {
 }
 
 size_t workspace_bytes(int64_t rows, int64_t cols) {
-    if (rows <= 1 || cols <= 0 || cols > (1 << 30)) return 0;
+    if (rows <= 1 || cols <= 0 || cols > kMaxColumns) return 0;
     const int64_t groups = cols <= kMostColumns ? max_groups(rows) : column_splits(rows, cols);
     return groups > 1 ? static_cast<size_t>(groups) * 2 * static_cast<size_t>(cols) * sizeof(float) : 0;
 }
@@ -628,7 +627,7 @@ int entry(const void *dy, const void *x, const float *mean, const float *rstd, c
     typedef typename Io<IO>::elem Elem;
     if (rows < 0 || cols <= 0)
         return fail(KO_ERR_INVALID_ARGUMENT, "layernorm_backward: rows=%lld cols=%lld", (long long)rows, (long long)cols);
-    if (cols > (1 << 30)) return fail(KO_ERR_UNSUPPORTED_SHAPE, "layernorm_backward: cols=%lld too large", (long long)cols);
+    if (cols > kMaxColumns) return fail(KO_ERR_UNSUPPORTED_SHAPE, "layernorm_backward: cols=%lld too large", (long long)cols);
     if (rows > 0 && (!dy || !x || !mean || !rstd || !dx))
         return fail(KO_ERR_INVALID_ARGUMENT, "layernorm_backward: null dy/in/mean/rstd/dx pointer");
     const uintptr_t rows_at = reinterpret_cast<uintptr_t>(dy) | reinterpret_cast<uintptr_t>(x) |

@@ -319,7 +319,10 @@ __device__ __forceinline__ void put_score(const A &a, int64_t row, bool live, co
 
 // One workgroup per row, the next batch of U vectors per thread in flight while this one is added up.  As in
 // policy_onchip_kernel the exponentials are taken against the label's logit, and the row's maximum is noted by the way; a label
-// so unlikely that the sum reaches 2^40, or a sum that is not a number, is summed again with a running maximum.
+// so unlikely that the sum reaches 2^40, or a sum that is not a number, is summed again with a running maximum.  Bound: memory
+// (1 GiB of bf16 logits: 128256 columns 160 us, 6.7 TB/s, 50257 columns 152 us, 7.1 TB/s, 4096 columns 190 us), the
+// arithmetic close behind: nine instructions' time per value.  A running maximum without loads ahead took 164 us at 32000
+// columns and 329 at 8192.
 template <int IO, int THREADS, int U>
 __global__ __launch_bounds__(THREADS) void token_logprob_row_kernel(ScoreArgs<IO> a) {
     constexpr int E = Io<IO>::E;
@@ -999,15 +1002,13 @@ __global__ __launch_bounds__(kPreferenceThreads) void preference_kernel(Preferen
 }
 
 // ---------------------------------------------------------------------------------------------------- dispatch
-constexpr int64_t kMaxColumns = 1 << 28;  // bytes of a row are counted in 32 bits
-
-// Pieces per row of a few long rows: a function of the sizes alone, so that the workspace can be sized without a device.  Below
-// 48K columns a workgroup per row takes less time than a second launch (16 rows of 30522 fp32 columns 6.0 us against 7.7, with
-// the policy loss 7.3 against 9.4; 32 rows of 50257 bf16 columns 7.2 against 7.7 and 9.6 against 9.8); 16 rows of 100000 take
-// 8.8 us whole and 7.7 in pieces, the policy loss 12.5 and 9.2.  128 rows are enough workgroups of their own (13 us against 21).
+// Pieces per row of a few long rows: a function of the sizes alone, so that the workspace can be sized without a device.  Up to
+// 64K columns a workgroup per row takes less time than a second launch (16 rows of 30522 fp32 columns 6.0 us against 7.7, with
+// the policy loss 7.3 against 9.4; 32 rows of 50257 binary16 columns with their gradient 17.8 against 21.2); 16 rows of 100000
+// take 8.8 us whole and 7.7 in pieces, the policy loss 12.5 and 9.2.  128 rows are enough workgroups of their own (13 us against 21).
 constexpr int kPieceUnits = 256;  // compute units of an MI355X
 constexpr int64_t kPieceColumns = 4096;
-constexpr int64_t kWholeColumns = 48 << 10;
+constexpr int64_t kWholeColumns = 64 << 10;
 int pieces_per_row(int64_t rows, int64_t cols) {
     if (rows <= 0 || rows * 4 > kPieceUnits || cols <= kWholeColumns) return 1;
     const int64_t parts = 2 * kPieceUnits / rows;
@@ -1027,9 +1028,6 @@ Scale two_parts(float scale) {
     const float lo = static_cast<float>(c - hi);
     return Scale{hi, lo > 1e-37f ? lo : 1e-37f};
 }
-
-// One workgroup per row, as far as a grid goes (its threads number less than 2^32 in one dimension).
-unsigned row_grid(int64_t rows) { return static_cast<unsigned>(rows > (1 << 21) ? (1 << 21) : rows); }
 
 // What every entry on rows of logits checks.
 int check_logits(const char *who, const void *logits, int64_t ld, const void *labels, size_t size, float scale, int64_t rows,
@@ -1093,8 +1091,10 @@ int logprob_entry(const void *logits, int64_t ld, const int32_t *labels, float s
         KO_CHECK_LAUNCH();
         return KO_OK;
     }
-    const dim3 grid(row_grid(rows));
+    const dim3 grid = row_grid(rows, 1024);
     const int nvec = a.cols / Io<IO>::E;
+    // rows of few vectors: as many threads as make one batch of them (8192 bf16 columns 187 us for 1 GiB, 208 with 512 threads and
+    // 4096 columns 190 against 383 with 256, half of them idle)
     if (nvec <= 128) token_logprob_row_kernel<IO, 64, 2><<<grid, dim3(64), 0, a.stream>>>(a);
     else if (nvec <= 256) token_logprob_row_kernel<IO, 64, 4><<<grid, dim3(64), 0, a.stream>>>(a);
     else if (nvec <= 512) token_logprob_row_kernel<IO, 128, 4><<<grid, dim3(128), 0, a.stream>>>(a);
@@ -1192,7 +1192,7 @@ int launch_policy(const PolicyArgs<IO> &a, void *workspace) {
         }
     }
     // no gradient, rows that lie differently in the two matrices, a row or two's vectors, and rows longer than the registers
-    const dim3 grid(row_grid(a.rows));
+    const dim3 grid = row_grid(a.rows, 1024);
     if (a.cols <= 4096) policy_reread_kernel<IO, 256><<<grid, dim3(256), 0, a.stream>>>(a);
     else if (a.cols <= 32768) policy_reread_kernel<IO, 512><<<grid, dim3(512), 0, a.stream>>>(a);
     else policy_reread_kernel<IO, 1024><<<grid, dim3(1024), 0, a.stream>>>(a);
@@ -1318,7 +1318,7 @@ KO_EXPORT int ko_preference_loss_f32(const float *logp, const float *ref_logp, c
         return ko::fail(KO_ERR_INVALID_ARGUMENT, "%s: null logp/ref_logp/offsets/pair_loss pointer", who);
     const ko::PreferenceArgs a{logp, ref_logp, labels, offsets, pairs, tokens, beta, label_smoothing, pair_weight, pair_loss,
                                rewards, dlogp};
-    ko::preference_kernel<<<dim3(ko::row_grid(pairs)), dim3(ko::kPreferenceThreads), 0, s>>>(a);
+    ko::preference_kernel<<<ko::row_grid(pairs, ko::kPreferenceThreads), dim3(ko::kPreferenceThreads), 0, s>>>(a);
     KO_CHECK_LAUNCH();
     return loss_sum ? ko::launch_loss_sum(pair_loss, pairs, pair_weight, loss_sum, s) : KO_OK;
 }

@@ -176,6 +176,16 @@ __device__ __forceinline__ void block_sum(float (&v)[N], float (*slot)[N]) {
     }
 }
 
+// Longest row of the kernels that count its bytes in 32 bits.
+constexpr int64_t kMaxColumns = 1 << 28;
+
+// One workgroup per row (or group of rows), as far as a grid goes: its threads number less than 2^32, and the kernels walk on
+// from there.
+inline dim3 row_grid(int64_t groups, int threads) {
+    const int64_t most = 0xffffffffll / threads;
+    return dim3(static_cast<unsigned>(groups < most ? groups : most));
+}
+
 // Lanes per row and vectors per lane for rows of `nvec` vectors held by groups of 8 to 64 lanes: the fewest idle
 // vector slots, among equals the widest group (one load instruction then covers the longest piece of a row).
 // `max_vpl` bounds the vectors per lane for 64 lanes; narrower groups take at most 3.

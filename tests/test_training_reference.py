@@ -147,9 +147,9 @@ def test_token_logprob_refusals():
     _refused(f(BAD, 8, BAD, 1.0, BAD, None, 4, 0, None, 0, None), inv, "cols")
     _refused(f(BAD, 1 << 31, BAD, 1.0, BAD, None, 4, (1 << 30) + 1, None, 0, None), ko.KO_ERR_UNSUPPORTED_SHAPE, "too large")
     _refused(f(BAD + 2, 8, BAD, 1.0, BAD, None, 4, 8, None, 0, None), inv, "aligned")
-    need = ko.token_logprob_workspace_bytes(4, 50257)
+    need = ko.token_logprob_workspace_bytes(4, 100000)
     assert need > 0 and ko.token_logprob_workspace_bytes(4096, 50257) == 0
-    _refused(f(BAD, 50257, BAD, 1.0, BAD, None, 4, 50257, BAD, need - 1, None), inv, "workspace")
+    _refused(f(BAD, 100000, BAD, 1.0, BAD, None, 4, 100000, BAD, need - 1, None), inv, "workspace")
     _refused(h(BAD, 8, BAD, 1.0, BAD, None, 4, 8, 5, None, 0, None), inv, "dtype")
     _refused(b(BAD, 8, BAD, 1.0, None, BAD, BAD, 8, 4, 8, None), inv, "row_stats")
     _refused(b(BAD, 8, BAD, 1.0, BAD, BAD, BAD, 7, 4, 8, None), inv, "ldd")
