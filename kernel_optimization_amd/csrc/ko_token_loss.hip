@@ -1094,13 +1094,13 @@ int logprob_entry(const void *logits, int64_t ld, const int32_t *labels, float s
     const dim3 grid = row_grid(rows, 1024);
     const int nvec = a.cols / Io<IO>::E;
     // rows of few vectors: as many threads as make one batch of them (8192 bf16 columns 187 us for 1 GiB, 208 with 512 threads and
-    // 4096 columns 190 against 383 with 256, half of them idle)
+    // 4096 columns 190 against 383 with 256, half of them idle).  Long rows: 1024 threads took 258 us for 1 GiB of rows of
+    // 50257 bf16 columns, 512 take 152, and 32 such rows 6.7 against 7.2.
     if (nvec <= 128) token_logprob_row_kernel<IO, 64, 2><<<grid, dim3(64), 0, a.stream>>>(a);
     else if (nvec <= 256) token_logprob_row_kernel<IO, 64, 4><<<grid, dim3(64), 0, a.stream>>>(a);
     else if (nvec <= 512) token_logprob_row_kernel<IO, 128, 4><<<grid, dim3(128), 0, a.stream>>>(a);
     else if (nvec <= 1024) token_logprob_row_kernel<IO, 256, 4><<<grid, dim3(256), 0, a.stream>>>(a);
-    else if (nvec <= 4096 || rows >= 1024) token_logprob_row_kernel<IO, 512, 4><<<grid, dim3(512), 0, a.stream>>>(a);
-    else token_logprob_row_kernel<IO, 1024, 4><<<grid, dim3(1024), 0, a.stream>>>(a);
+    else token_logprob_row_kernel<IO, 512, 4><<<grid, dim3(512), 0, a.stream>>>(a);
     KO_CHECK_LAUNCH();
     return KO_OK;
 }

@@ -1,0 +1,315 @@
+"""The training-side operators as a program runs them: one after the other on a stream, in two captured graphs that replay beside
+eager work, on two streams at once, and on matrices whose offsets pass 32 bits."""
+import ctypes
+
+import numpy as np
+import pytest
+
+import training_reference as ref
+from kernel_optimization_amd import inputs
+from test_gpu_streams_and_graphs import _hip_runtime
+
+pytestmark = pytest.mark.gpu
+
+U = ref.U
+
+
+@pytest.mark.parametrize("loss", ["preference", "policy"])
+def test_a_training_step_from_hidden_states_to_their_gradient(ko, loss):
+    """LayerNorm, logits, the loss, and back: the gradients of the hidden states, gamma and beta against the same chain in 64
+    bits.  Each bound carries the one before it through the next operator's derivative."""
+    lens = np.array([30, 17, 25, 56])
+    tokens, hidden, vocab = int(lens.sum()), 64, 333
+    rng = np.random.default_rng(41)
+    x = rng.normal(0.3, 1.5, (tokens, hidden)).astype(np.float32)
+    gamma, beta = rng.normal(1, 0.1, hidden).astype(np.float32), rng.normal(0, 0.1, hidden).astype(np.float32)
+    w = (rng.normal(0, 1, (hidden, vocab)) / 8).astype(np.float32)
+    labels = rng.integers(0, vocab, tokens).astype(np.int32)
+    labels[[3, 40]] = -1
+    dx_, dgamma_, dbeta_ = ko.DeviceBuffer(x.nbytes), ko.DeviceBuffer(4 * hidden), ko.DeviceBuffer(4 * hidden)
+    dev = {k: ko.DeviceBuffer.from_numpy(v) for k, v in dict(x=x, gamma=gamma, beta=beta, w=w, wt=np.ascontiguousarray(w.T),
+                                                             labels=labels).items()}
+    h, mean, rstd, dh = (ko.DeviceBuffer(n) for n in (x.nbytes, 4 * tokens, 4 * tokens, x.nbytes))
+    logits = ko.DeviceBuffer(4 * tokens * vocab)
+    # ---- the same in 64 bits
+    x64, g64, w64 = x.astype(np.float64), gamma.astype(np.float64), w.astype(np.float64)
+    mu = x64.mean(1)
+    inv = 1 / np.sqrt(x64.var(1) + 1e-5)
+    h64 = (x64 - mu[:, None]) * inv[:, None] * g64 + beta
+    # (the forward operator's bounds: mean and rstd within 2 depth roundings of what they are made of)
+    mean_off = (ref.depth(hidden) + 2) * U * np.abs(x64).mean(1)
+    rstd_rel = (ref.depth(hidden) + 8) * U + mean_off * inv
+    h_off = (np.abs(x64 - mu[:, None]) * (rstd_rel + 6 * U)[:, None] + mean_off[:, None]) * inv[:, None] * np.abs(g64) + 2 * U * np.abs(h64)
+    z64 = h64 @ w64
+    z_off = (hidden + 1) * U * (np.abs(h64) @ np.abs(w64)) + h_off @ np.abs(w64)
+    z_most = z_off.max(1)
+    scores = ref.Scores(z64, labels)
+    logp_off = scores.logp_off + 2 * z_most * scores.rest
+    alive = labels >= 0
+
+    ko.layernorm(dev["x"], h, tokens, hidden, mean, rstd, dev["gamma"], dev["beta"], 1e-5)
+    ko.sgemm(tokens, vocab, hidden, h, dev["w"], logits)
+    if loss == "preference":
+        reference = (scores.logp + rng.normal(0, 0.2, tokens)).astype(np.float32)
+        offsets = np.concatenate([[0], np.cumsum(lens)]).astype(np.int32)
+        dev["ref"], dev["offsets"] = ko.DeviceBuffer.from_numpy(reference), ko.DeviceBuffer.from_numpy(offsets)
+        logp, stats, dlogp, pair_loss, total = (ko.DeviceBuffer(n) for n in (4 * tokens, 8 * tokens, 4 * tokens, 8, 4))
+        dlogp.upload(np.zeros(tokens, np.float32))
+        ko.token_logprob(logits, dev["labels"], logp, tokens, vocab, row_stats=stats)
+        ko.preference_loss(logp, dev["ref"], dev["offsets"], 2, tokens, pair_loss, labels=dev["labels"], beta=0.3, dlogp=dlogp,
+                           loss_sum=total)
+        ko.token_logprob_backward(logits, dev["labels"], stats, dlogp, logits, tokens, vocab)   # in place
+        rewards = [0.3 * np.where(alive, scores.logp - reference, 0.0)[a:b].sum() for a, b in zip(offsets, offsets[1:])]
+        rewards_off = [0.3 * np.where(alive, logp_off, 0.0)[a:b].sum() for a, b in zip(offsets, offsets[1:])]
+        coeff, coeff_off = np.zeros(tokens), np.zeros(tokens)
+        want_loss = want_off = 0.0
+        for p in range(2):
+            margin, off = rewards[2 * p] - rewards[2 * p + 1], rewards_off[2 * p] + rewards_off[2 * p + 1]
+            want_loss += 0.5 * np.log1p(np.exp(-margin))
+            want_off += 0.5 * off
+            for side, sign in ((2 * p, -1.0), (2 * p + 1, 1.0)):
+                part = slice(offsets[side], offsets[side + 1])
+                coeff[part] = sign * 0.5 * 0.3 / (1 + np.exp(margin))
+                coeff_off[part] = 0.5 * 0.3 * (off / 4) + 4 * U * np.abs(coeff[part])
+        log_error = 2 * z_most + 3 * U * np.abs(scores.logsum) + 2 * U
+    else:
+        old = (scores.logp + rng.normal(0, 0.05, tokens)).astype(np.float32)   # (inside the clip range)
+        old = np.clip(old, scores.logp - 0.15, scores.logp + 0.15).astype(np.float32)
+        advantage = rng.normal(0, 1, tokens).astype(np.float32)
+        dev["old"], dev["adv"] = ko.DeviceBuffer.from_numpy(old), ko.DeviceBuffer.from_numpy(advantage)
+        row_loss, total = ko.DeviceBuffer(4 * tokens), ko.DeviceBuffer(4)
+        ko.policy_loss(logits, dev["labels"], dev["adv"], row_loss, tokens, vocab, old_logp=dev["old"], loss_sum=total,
+                       dlogits=logits)                                          # in place
+        ratio = np.exp(scores.logp - old)
+        want_loss = float((-ratio * advantage)[alive].sum())
+        want_off = float((np.abs(advantage) * ratio * (logp_off + 8 * U))[alive].sum())
+        coeff = np.where(alive, -advantage * ratio, 0.0)
+        coeff_off = np.abs(coeff) * (logp_off + 8 * U)
+        log_error = 2 * z_most
+    dz, dz_off = scores.gradient(coeff, coeff_off, log_error)
+    # a logit's own error moves its exponential too; the label's entry carries 1 - p
+    dz_off = dz_off + 2 * z_most[:, None] * np.abs(coeff)[:, None] * scores.p
+    ko.sgemm(tokens, hidden, vocab, logits, dev["wt"], dh)
+    dh64 = dz @ w64.T
+    dh_off = (vocab + 1) * U * (np.abs(dz) @ np.abs(w64.T)) + dz_off @ np.abs(w64.T)
+    n = ko.layernorm_backward_workspace_bytes(tokens, hidden)
+    ws = ko.DeviceBuffer(max(n, 16))
+    ko.layernorm_backward(dh, dev["x"], mean, rstd, dx_, tokens, hidden, gamma=dev["gamma"], dgamma=dgamma_, dbeta=dbeta_,
+                          workspace=ws, workspace_bytes=n)
+    ko.synchronize()
+    (dx, dgamma, dbeta), (dx_off, dgamma_off, dbeta_off) = ref.layernorm_backward(dh64, x64, mu, inv, g64)
+    xh = np.abs((x64 - mu[:, None]) * inv[:, None])
+    xh_off = mean_off[:, None] * inv[:, None] + xh * (rstd_rel + 2 * U)[:, None]
+    go, gg = dh_off * np.abs(g64), np.abs(dh64 * g64)
+    c2 = (gg * xh).mean(1, keepdims=True)
+    dx_off += inv[:, None] * (go + go.mean(1, keepdims=True) + xh * (go * xh).mean(1, keepdims=True)
+                              + xh_off * c2 + xh * (gg * xh_off).mean(1, keepdims=True)) + np.abs(dx) * rstd_rel[:, None]
+    dgamma_off += (dh_off * xh + np.abs(dh64) * xh_off).sum(0)
+    dbeta_off += dh_off.sum(0)
+    assert abs(float(total.download(np.float32, (1,))[0]) - want_loss) <= want_off + 4 * U * abs(want_loss)
+    ref.assert_within(dx_.download(np.float32, x.shape), dx, dx_off, "dx")
+    ref.assert_within(dgamma_.download(np.float32, (hidden,)), dgamma, dgamma_off, "dgamma")
+    ref.assert_within(dbeta_.download(np.float32, (hidden,)), dbeta, dbeta_off, "dbeta")
+
+
+def test_softmax_and_its_gradient_follow_each_other(ko):
+    """The masked softmax's own output goes into its gradient, a sequence without a valid column among them."""
+    rows, cols, rps = 96, 200, 24
+    x, dy = inputs.normal_f32((rows, cols), 51, 0.0, 3.0), inputs.normal_f32((rows, cols), 52)
+    lens = np.array([200, 1, 0, 77], np.int32)
+    dx_in, y, ddy, dvl = (ko.DeviceBuffer.from_numpy(v) for v in (x, np.zeros_like(x), dy, lens))
+    ko.softmax(dx_in, y, rows, cols, dvl, rps)
+    ko.softmax_backward(y, ddy, ddy, rows, cols, dvl, rps)   # in place of dy
+    ko.synchronize()
+    got_y = y.download(np.float32, (rows, cols))
+    want, off = ref.softmax_backward(got_y.astype(np.float64), dy.astype(np.float64), lens, rps)
+    got = ddy.download(np.float32, (rows, cols))
+    # (2^-149: masked columns are exactly 0, and 0 / 0 is no comparison)
+    ref.assert_within(got, want, off + U * np.abs(want) + 2.0 ** -149, "dx")
+    # the rows' gradients sum to nothing: y (dy - t) with t = sum y dy
+    assert (np.abs(got.astype(np.float64).sum(1)) <= (2 * off.sum(1) + cols * U * np.abs(want).sum(1)
+                                                      + np.abs(1 - got_y.astype(np.float64).sum(1)) * np.abs(dy).max())).all()
+
+
+class Step:
+    """One training program of every operator, its buffers and workspaces its own; kind f32 or bf16."""
+
+    def __init__(self, ko, kind, seed):
+        self.ko, self.kind = ko, kind
+        self.size = 4 if kind == "f32" else 2
+        self.typed = {} if kind == "f32" else dict(dtype=ko.BF16)
+        self.keep, self.out = [], []
+        rng = np.random.default_rng(seed)
+        ko_shapes = dict(ln=[(700, 768), (100, 768), (33, 20000)], sm=[(384, 512), (3, 200001)],
+                         rows=[(64, 2000), (5, 50257), (4, 140001), (130, 33000)])
+        self.ln, self.sm, self.rows = [], [], []
+        for rows, cols in ko_shapes["ln"]:
+            n = ko.layernorm_backward_workspace_bytes(rows, cols)
+            self.ln.append((rows, cols, self.matrix(rows, cols, rng), self.matrix(rows, cols, rng), self.floats(rng.normal(0, .1, rows)),
+                            self.floats(rng.uniform(.5, 2, rows)), self.matrix(1, cols, rng), self.result(rows * cols * self.size),
+                            self.result(4 * cols), self.result(4 * cols), self.scratch(n), n))
+        for rows, cols in ko_shapes["sm"]:
+            n = ko.softmax_backward_workspace_bytes(rows, cols)
+            self.sm.append((rows, cols, self.matrix(rows, cols, rng), self.matrix(rows, cols, rng),
+                            self.ints(rng.integers(0, cols + 1, rows)), self.result(rows * cols * self.size), self.scratch(n), n))
+        for rows, cols in ko_shapes["rows"]:
+            n = ko.token_logprob_workspace_bytes(rows, cols)
+            labels = rng.integers(0, cols, rows)
+            labels[0] = -1
+            self.rows.append((rows, cols, self.matrix(rows, cols, rng), self.ints(labels), self.scratch(n), n,
+                              [self.floats(rng.normal(0, 1, rows)) for _ in range(4)],
+                              [self.result(4 * rows) for _ in range(5)], self.result(8 * rows),
+                              [self.result(rows * cols * self.size) for _ in range(2)], self.result(4),
+                              self.ints(np.linspace(0, rows, 5))))
+
+    def matrix(self, rows, cols, rng):
+        return self.buffer(ref.to_storage(rng.normal(0, 1, (rows, cols)).astype(np.float32), self.kind)[0])
+
+    def buffer(self, a):
+        self.keep.append(self.ko.DeviceBuffer.from_numpy(np.ascontiguousarray(a)))
+        return self.keep[-1]
+
+    def floats(self, a):
+        return self.buffer(np.asarray(a, np.float32))
+
+    def ints(self, a):
+        return self.buffer(np.asarray(a).astype(np.int32))
+
+    def scratch(self, n):
+        return self.buffer(np.full(max(n, 16), 0xFF, np.uint8))
+
+    def result(self, n):
+        self.out.append((self.scratch(n), n))
+        return self.out[-1][0]
+
+    def op(self, name):
+        return getattr(self.ko, name + ("" if self.kind == "f32" else "16"))
+
+    def run(self, stream):
+        for rows, cols, dy, x, mean, rstd, gamma, dx, dgamma, dbeta, ws, n in self.ln:
+            self.op("layernorm_backward")(dy, x, mean, rstd, dx, rows, cols, gamma=gamma, dgamma=dgamma, dbeta=dbeta, workspace=ws,
+                                          workspace_bytes=n, stream=stream, **self.typed)
+        for rows, cols, y, dy, lens, dx, ws, n in self.sm:
+            self.op("softmax_backward")(y, dy, dx, rows, cols, lens, 1, workspace=ws, workspace_bytes=n, stream=stream, **self.typed)
+        for rows, cols, x, labels, ws, n, (a, b, c, d), (logp, kl, loss, dlogp, pair), stats, (g1, g2), total, offsets in self.rows:
+            work = dict(workspace=ws, workspace_bytes=n, stream=stream, **self.typed)
+            self.op("token_logprob")(x, labels, logp, rows, cols, row_stats=stats, **work)
+            self.ko.preference_loss(logp, a, offsets, 2, rows, pair, labels=labels, dlogp=dlogp, stream=stream)
+            self.op("token_logprob_backward")(x, labels, stats, dlogp, g1, rows, cols, stream=stream, **self.typed)
+            self.op("policy_loss")(x, labels, b, loss, rows, cols, old_logp=logp, ref_logp=c, weight=d, kl_coef=0.1, kl=kl,
+                                   loss_sum=total, dlogits=g2, **work)
+
+    def clear(self):
+        for buf, n in self.out:
+            buf.upload(np.full(n, 0xFF, np.uint8))
+
+    def results(self):
+        return [buf.download(np.uint8, (n,)) for buf, n in self.out]
+
+
+def test_two_graphs_with_their_own_workspaces_beside_eager_work(ko):
+    """Captured on streams that ran nothing before, replayed at the same time, several times over, with eager calls of the same
+    operators on the default stream and on the graphs' streams in between."""
+    hip = _hip_runtime()
+    steps = [Step(ko, "f32", 61), Step(ko, "bf16", 62)]
+    want = []
+    for s in steps:
+        s.run(None)
+        ko.synchronize()
+        want.append(s.results())
+        assert any(r.any() for r in want[-1])
+    eager = Step(ko, "bf16", 63)
+    eager.run(None)
+    ko.synchronize()
+    eager_want = eager.results()
+    streams, graphs, execs = [ko.Stream(), ko.Stream()], [], []
+    try:
+        for s, stream in zip(steps, streams):
+            graph, graph_exec = ctypes.c_void_p(), ctypes.c_void_p()
+            assert hip.hipStreamBeginCapture(stream.handle, 0) == 0
+            try:
+                s.run(stream)
+            finally:
+                rc = hip.hipStreamEndCapture(stream.handle, ctypes.byref(graph))
+            assert rc == 0 and graph.value
+            graphs.append(graph)
+            assert hip.hipGraphInstantiate(ctypes.byref(graph_exec), graph, None, None, 0) == 0
+            execs.append(graph_exec)
+        for replay in range(4):
+            for s in steps + [eager]:
+                s.clear()
+            ko.synchronize()
+            for graph_exec, stream in zip(execs, streams):
+                assert hip.hipGraphLaunch(graph_exec, stream.handle) == 0
+            eager.run([None, streams[0], None, streams[1]][replay])
+            for stream in streams:
+                stream.synchronize()
+            ko.synchronize()
+            for s, w in zip(steps + [eager], want + [eager_want]):
+                for i, (got, expected) in enumerate(zip(s.results(), w)):
+                    np.testing.assert_array_equal(got, expected, err_msg="replay %d, %s result %d" % (replay, s.kind, i))
+    finally:
+        for graph_exec in execs:
+            hip.hipGraphExecDestroy(graph_exec)
+        for graph in graphs:
+            hip.hipGraphDestroy(graph)
+
+
+def test_two_streams_at_once(ko):
+    steps = [Step(ko, "bf16", 71), Step(ko, "f32", 72)]
+    want = []
+    for s in steps:
+        s.run(None)
+        ko.synchronize()
+        want.append(s.results())
+        s.clear()
+    ko.synchronize()
+    streams = [ko.Stream(), ko.Stream()]
+    for _ in range(3):
+        for s, stream in zip(steps, streams):
+            s.run(stream)
+    for stream in streams:
+        stream.synchronize()
+    for s, w in zip(steps, want):
+        for i, (got, expected) in enumerate(zip(s.results(), w)):
+            np.testing.assert_array_equal(got, expected, err_msg="%s result %d" % (s.kind, i))
+
+
+def test_matrices_beyond_32_bits(ko):
+    """66000 rows of 33000 bf16 columns, 2.2e9 elements and 4.36e9 bytes: the last rows have the bits that a call on them alone
+    gives, into a matrix that starts at the same place in a cache line (where rows start decides how their sums are split)."""
+    rows, cols, last = 66000, 33000, 300
+    size = rows * cols * 2
+    skip = (rows - last) * cols * 2
+    a, b, d = ko.DeviceBuffer(size), ko.DeviceBuffer(size), ko.DeviceBuffer(size)
+    small = ko.DeviceBuffer(last * cols * 2 + 256)
+    lies = skip % 128
+    ko.fill_uniform_16(a, rows * cols, 81, dtype=ko.BF16)
+    ko.fill_uniform_16(b, rows * cols, 82, dtype=ko.BF16)
+    rng = np.random.default_rng(83)
+    labels = rng.integers(0, cols, rows).astype(np.int32)
+    floats = [rng.normal(0, 1, rows).astype(np.float32) for _ in range(2)] + [rng.uniform(0.5, 2, rows).astype(np.float32)]
+    dl, (df, dm, dr) = ko.DeviceBuffer.from_numpy(labels), (ko.DeviceBuffer.from_numpy(v) for v in floats)
+    f = 4 * (rows - last)
+    typed = dict(dtype=ko.BF16)
+
+    def same(name, run):
+        run(a.ptr, b.ptr, d.ptr, 0, rows)
+        whole, alone = ko.DeviceBuffer(last * cols * 2), ko.DeviceBuffer(last * cols * 2)
+        ko.copy_f32(d.ptr + skip, whole, last * cols // 2)
+        run(a.ptr + skip, b.ptr + skip, small.ptr + lies, f, last)
+        ko.copy_f32(small.ptr + lies, alone, last * cols // 2)
+        ko.synchronize()
+        got, want = whole.download(np.uint16, (last, cols)), alone.download(np.uint16, (last, cols))
+        assert want.any()
+        np.testing.assert_array_equal(got, want, err_msg=name)
+
+    same("layernorm", lambda x, y, o, at, n: ko.layernorm_backward16(y, x, dm.ptr + at, dr.ptr + at, o, n, cols, **typed))
+    same("softmax", lambda x, y, o, at, n: ko.softmax_backward16(x, y, o, n, cols, **typed))
+    logp, stats, loss = ko.DeviceBuffer(4 * rows), ko.DeviceBuffer(8 * rows), ko.DeviceBuffer(4 * rows)
+
+    def scores(x, y, o, at, n):
+        ko.token_logprob16(x, dl.ptr + at, logp.ptr + at, n, cols, row_stats=stats.ptr + 2 * at, **typed)
+        ko.token_logprob_backward16(x, dl.ptr + at, stats.ptr + 2 * at, df.ptr + at, o, n, cols, **typed)
+    same("token_logprob", scores)
+    same("policy", lambda x, y, o, at, n: ko.policy_loss16(x, dl.ptr + at, df.ptr + at, loss.ptr + at, n, cols, dlogits=o, **typed))
