@@ -115,23 +115,48 @@ __device__ __forceinline__ void add_values(Pair &p, const float (&v)[N], Scale c
     else p.s += s[0];
 }
 
+// A row's or a piece's pair: its sum in 64 bits.  What a thread sums in 32 bits is off by its own roundings, which average out
+// over a thousand threads; the last steps of a tree would not, and a KL term takes the difference of two such numbers.
+struct Total {
+    float m;
+    double s;
+};
+__device__ __forceinline__ double wave_sum(double v) {
+#pragma unroll
+    for (int step = 1; step < 64; step <<= 1) v += __shfl_xor(v, step, 64);
+    return v;
+}
+// Sum over a wavefront, the same bits in every lane: sixteen lanes in 32 bits, the four sums of those in 64.
+__device__ __forceinline__ double wave_total(float v) {
+    const int row = __builtin_bit_cast(int, wave::allreduce<16, wave::Sum>(v));
+    auto of = [&](int lane) { return static_cast<double>(__builtin_bit_cast(float, __builtin_amdgcn_readlane(row, lane))); };
+    return (of(0) + of(16)) + (of(32) + of(48));
+}
+
 // The pairs of a workgroup's threads, the same bits in every thread.  One barrier; `slot` as in block_sum.
 template <int WAVES>
-__device__ __forceinline__ Pair block_pair(Pair p, Pair *slot, Scale c) {
+__device__ __forceinline__ Total block_pair(Pair p, Total *slot, Scale c) {
     const float m = wave::allreduce<64, wave::Max>(p.m);
-    Pair r{m, wave::allreduce<64, wave::Sum>(p.s * exp_sum(p.m - m, c))};
+    Total r{m, wave_total(p.s * exp_sum(p.m - m, c))};
     if constexpr (WAVES > 1) {
         if ((threadIdx.x & 63) == 0) slot[threadIdx.x >> 6] = r;
         __syncthreads();
         float top = slot[0].m;
 #pragma unroll
         for (int w = 1; w < WAVES; ++w) top = fmaxf(top, slot[w].m);
-        float s = 0.0f;
+        double s = 0.0;
 #pragma unroll
         for (int w = 0; w < WAVES; ++w) s += slot[w].s * exp_sum(slot[w].m - top, c);
-        r = Pair{top, s};
+        r = Total{top, s};
     }
     return r;
+}
+
+// From a sum of 2^(c x_j - shift) to one of exp(scale (x_j - x_l)): shift is c x_l rounded, and the factor is 1 or next to it
+// unless x_l is large.
+__device__ __forceinline__ double to_label(double sum, float at_label, float shift, Scale c) {
+    const float rest = __builtin_fmaf(at_label, c.lo, __builtin_fmaf(at_label, c.hi, -shift));
+    return sum + sum * expm1f(-0.69314718f * rest);
 }
 
 // A thread's share of the pair over the vectors [lo, hi) and, if `with_singles`, the single elements of a row, without
@@ -192,33 +217,34 @@ struct RowScore {
     float rest;      // S / (S + e): what the label's probability leaves
 };
 // log(t) of a positive t, within 3e-8 absolute
-__device__ __forceinline__ double log_in_parts(float t) {
-    if (!(t < INFINITY)) return t;
+__device__ __forceinline__ double log_in_parts(double t) {
+    if (!(t < 1e30)) return t;
     int k;
-    float f = frexpf(t, &k);
+    float f = frexpf(static_cast<float>(t), &k);
+    const float rest = static_cast<float>(t - static_cast<double>(static_cast<float>(t))) / static_cast<float>(t);
     if (f < 0.70710678f) {
         f *= 2.0f;
         --k;
     }
-    return __builtin_fma(static_cast<double>(k), 0.69314718055994531, static_cast<double>(logf(f)));
+    return __builtin_fma(static_cast<double>(k), 0.69314718055994531, static_cast<double>(logf(f)) + rest);
 }
 // From the pair of the other columns and the label's logit.
-__device__ __forceinline__ RowScore score_row(Pair p, float at_label, float scale, Scale c) {
+__device__ __forceinline__ RowScore score_row(Total p, float at_label, float scale, Scale c) {
     RowScore r;
     r.top = fmaxf(p.m, at_label);
-    const float s = p.s * exp_sum(p.m - r.top, c);
+    const double s = p.s * exp_sum(p.m - r.top, c);
     const double z = (static_cast<double>(at_label) - static_cast<double>(r.top)) * static_cast<double>(scale);
     const float e = expf(static_cast<float>(z));
-    const float total = s + e;
+    const double total = s + e;
     if (s <= e) {  // a likely label: relative to a logarithm close to 0
-        r.logp = -log1pf(s / e);
+        r.logp = -log1pf(static_cast<float>(s) / e);
         r.logsum = z - r.logp;
     } else {
         r.logsum = log_in_parts(total);
         r.logp = z - r.logsum;
     }
-    r.inv_total = 1.0f / total;
-    r.rest = s / total;
+    r.inv_total = 1.0f / static_cast<float>(total);
+    r.rest = static_cast<float>(s) * r.inv_total;
     return r;
 }
 __device__ __forceinline__ RowScore nan_score() {
@@ -320,16 +346,17 @@ __device__ __forceinline__ void put_score(const A &a, int64_t row, bool live, co
 // One workgroup per row, the next batch of U vectors per thread in flight while this one is added up.  As in
 // policy_onchip_kernel the exponentials are taken against the label's logit, and the row's maximum is noted by the way; a label
 // so unlikely that the sum reaches 2^40, or a sum that is not a number, is summed again with a running maximum.  Bound: memory
-// (1 GiB of bf16 logits: 128256 columns 160 us, 6.7 TB/s, 50257 columns 152 us, 7.1 TB/s, 4096 columns 190 us), the
-// arithmetic close behind: nine instructions' time per value.  A running maximum without loads ahead took 164 us at 32000
+// (1 GiB of bf16 logits: 128256 columns 160 us, 6.7 TB/s, 50257 columns 154 us, 7.0 TB/s, 4096 columns 200 us; the
+// arithmetic close behind: nine instructions' time per value; six wavefronts per SIMD, which the compiler has to be told: with five
+// 8192 columns take 216 us, with six 195).  A running maximum without loads ahead took 164 us at 32000
 // columns and 329 at 8192.
 template <int IO, int THREADS, int U>
-__global__ __launch_bounds__(THREADS) void token_logprob_row_kernel(ScoreArgs<IO> a) {
+__global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(6))) void token_logprob_row_kernel(ScoreArgs<IO> a) {
     constexpr int E = Io<IO>::E;
     constexpr int WAVES = THREADS / 64;
     typedef typename Io<IO>::raw Raw;
-    __shared__ Pair slots[2][WAVES];
-    __shared__ Pair again[WAVES];
+    __shared__ Total slots[2][WAVES];
+    __shared__ Total again[WAVES];
     int turn = 0;
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
         const typename Io<IO>::elem *src = a.logits + row * a.ld;
@@ -392,9 +419,9 @@ __global__ __launch_bounds__(THREADS) void token_logprob_row_kernel(ScoreArgs<IO
             s[1] += __builtin_amdgcn_exp2f(__builtin_fmaf(x, a.c.lo, __builtin_fmaf(x, a.c.hi, -shift)));
         }
         top = wave::allreduce<64, wave::Max>(top);
-        float sum = wave::allreduce<64, wave::Sum>((s[0] + s[1]) + (s[2] + s[3]));
+        double sum = wave_total((s[0] + s[1]) + (s[2] + s[3]));
         if constexpr (WAVES > 1) {
-            if ((threadIdx.x & 63) == 0) slots[turn][threadIdx.x >> 6] = Pair{top, sum};
+            if ((threadIdx.x & 63) == 0) slots[turn][threadIdx.x >> 6] = Total{top, sum};
             __syncthreads();
             top = slots[turn][0].m;
             sum = slots[turn][0].s;
@@ -404,10 +431,8 @@ __global__ __launch_bounds__(THREADS) void token_logprob_row_kernel(ScoreArgs<IO
                 sum += slots[turn][w].s;
             }
         }
-        // times 2^-(c x_l - shift): shift is c x_l rounded
-        sum *= __builtin_amdgcn_exp2f(-__builtin_fmaf(at_label, a.c.lo, __builtin_fmaf(at_label, a.c.hi, -shift)));
-        Pair p{at_label, sum};
-        if (!(uniform(sum) < 0x1p40f)) {
+        Total p{at_label, to_label(sum, at_label, shift, a.c)};
+        if (!(uniform(static_cast<float>(p.s)) < 0x1p40f)) {
             p = block_pair<WAVES>(thread_pair<IO, THREADS>(src, span, 0, span.nvec, true, label, a.c), again, a.c);
             top = fmaxf(p.m, at_label);
             __syncthreads();  // (read before the next row writes them)
@@ -424,18 +449,13 @@ __global__ __launch_bounds__(THREADS) void token_logprob_row_kernel(ScoreArgs<IO
 
 // A few rows: workgroup (p, row) takes the row's p-th piece; pieces' pairs and the label's logit pass through the
 // workspace.
-struct PieceHeader {
-    float at_label;
-    float unused;
-};
-static_assert(sizeof(PieceHeader) == sizeof(Pair), "");
-// layout: Pair [rows][1 + parts], the first slot of a row being its header
+// layout: Total [rows][1 + parts]; the first of a row holds the label's logit
 template <int IO, int THREADS>
 __global__ __launch_bounds__(THREADS) void token_pieces_kernel(const typename Io<IO>::elem *logits, int64_t ld,
                                                                const int32_t *__restrict__ labels,
                                                                const float *__restrict__ weight, int cols, Scale c,
-                                                               Pair *__restrict__ pairs) {
-    __shared__ Pair slot[THREADS / 64];
+                                                               Total *__restrict__ pairs) {
+    __shared__ Total slot[THREADS / 64];
     const int64_t row = blockIdx.y;
     const int label = uniform(labels[row]);
     if (label < 0 || label >= cols || (weight && uniform(weight[row]) == 0.0f)) return;
@@ -443,31 +463,30 @@ __global__ __launch_bounds__(THREADS) void token_pieces_kernel(const typename Io
     const RowSpan<IO> span = span_of<IO>(src, cols);
     const int parts = static_cast<int>(gridDim.x), part = static_cast<int>(blockIdx.x);
     const int lo = piece_begin(span.nvec, parts, part), hi = piece_begin(span.nvec, parts, part + 1);
-    const Pair p = block_pair<THREADS / 64>(thread_pair<IO, THREADS>(src, span, lo, hi, part == 0, label, c), slot, c);
+    const Total p = block_pair<THREADS / 64>(thread_pair<IO, THREADS>(src, span, lo, hi, part == 0, label, c), slot, c);
     if (threadIdx.x == 0) {
-        Pair *mine = pairs + row * (1 + parts);
-        if (part == 0) mine[0] = Pair{Io<IO>::scalar(src + label), 0.0f};
+        Total *mine = pairs + row * (1 + parts);
+        if (part == 0) mine[0] = Total{Io<IO>::scalar(src + label), 0.0};
         mine[1 + part] = p;
     }
 }
 // by one wavefront, the same bits in every lane
-__device__ __forceinline__ Pair fold_pieces(const Pair *mine, int parts, Scale c) {
-    Pair p{-FLT_MAX, 0.0f};
-    for (int i = 1 + (threadIdx.x & 63); i <= parts; i += 64) {
-        const float m = fmaxf(p.m, mine[i].m);
-        p.s = p.s * exp_sum(p.m - m, c) + mine[i].s * exp_sum(mine[i].m - m, c);
-        p.m = m;
-    }
-    return block_pair<1>(p, nullptr, c);
+__device__ __forceinline__ Total fold_pieces(const Total *mine, int parts, Scale c) {
+    float m = -FLT_MAX;
+    for (int i = 1 + (threadIdx.x & 63); i <= parts; i += 64) m = fmaxf(m, mine[i].m);
+    m = wave::allreduce<64, wave::Max>(m);
+    double s = 0.0;
+    for (int i = 1 + (threadIdx.x & 63); i <= parts; i += 64) s += mine[i].s * exp_sum(mine[i].m - m, c);
+    return Total{m, wave_sum(s)};
 }
 
 // One wavefront per row.
 template <int IO>
-__global__ __launch_bounds__(64) void token_logprob_fold_kernel(ScoreArgs<IO> a, const Pair *__restrict__ pairs, int parts) {
+__global__ __launch_bounds__(64) void token_logprob_fold_kernel(ScoreArgs<IO> a, const Total *__restrict__ pairs, int parts) {
     const int64_t row = blockIdx.x;
     const int label = uniform(a.labels[row]);
     RowScore r = nan_score();
-    const Pair *mine = pairs + row * (1 + parts);
+    const Total *mine = pairs + row * (1 + parts);
     if (label >= 0 && label < a.cols) r = score_row(fold_pieces(mine, parts, a.c), mine[0].m, a.scale, a.c);
     if (threadIdx.x == 0) put_score(a, row, label >= 0, r);
 }
@@ -584,7 +603,7 @@ struct PolicyResult {
     RowGradient gradient;
 };
 // One thread's work for a row that counts: p is the pair of the other columns.
-__device__ __forceinline__ PolicyResult policy_row(const PolicyOptions &o, const PolicyRow &in, Pair p) {
+__device__ __forceinline__ PolicyResult policy_row(const PolicyOptions &o, const PolicyRow &in, Total p) {
     const RowScore r = in.label < o.cols ? score_row(p, in.at_label, o.scale, o.c) : nan_score();
     const double adv = in.advantage, w = in.weight;
     const double ratio = o.old ? expf(static_cast<float>(r.logp - static_cast<double>(in.old_logp))) : 1.0 + 0.0 * r.logp;
@@ -622,7 +641,7 @@ __device__ __forceinline__ PolicyResult no_policy() { return PolicyResult{0.0f, 
 // One workgroup per row, any length and alignment: the sums, then a second read.
 template <int IO, int THREADS>
 __global__ __launch_bounds__(THREADS) void policy_reread_kernel(PolicyArgs<IO> a) {
-    __shared__ Pair slots[2][THREADS / 64];
+    __shared__ Total slots[2][THREADS / 64];
     __shared__ RowGradient shared[2];
     int turn = 0;
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
@@ -632,7 +651,7 @@ __global__ __launch_bounds__(THREADS) void policy_reread_kernel(PolicyArgs<IO> a
         const RowSpan<IO> span = span_of<IO>(a.dlogits ? a.dlogits + row * a.ldd : src, a.cols);
         if (counts) {
             float at_label = 0.0f;
-            Pair p{-FLT_MAX, 0.0f};
+            Total p{-FLT_MAX, 0.0};
             if (label < a.cols) {
                 at_label = Io<IO>::scalar(src + label);
                 p = block_pair<THREADS / 64>(thread_pair<IO, THREADS>(src, span, 0, span.nvec, true, label, a.c), slots[turn],
@@ -657,7 +676,7 @@ __global__ __launch_bounds__(THREADS) void policy_reread_kernel(PolicyArgs<IO> a
 
 // A few rows, after token_pieces_kernel: workgroup (p, row) folds the row's pairs and writes the p-th piece.
 template <int IO, int THREADS>
-__global__ __launch_bounds__(THREADS) void policy_pieces_kernel(PolicyArgs<IO> a, const Pair *__restrict__ pairs, int parts) {
+__global__ __launch_bounds__(THREADS) void policy_pieces_kernel(PolicyArgs<IO> a, const Total *__restrict__ pairs, int parts) {
     __shared__ RowGradient shared;
     const int64_t row = blockIdx.y;
     const int part = static_cast<int>(blockIdx.x);
@@ -665,9 +684,9 @@ __global__ __launch_bounds__(THREADS) void policy_pieces_kernel(PolicyArgs<IO> a
     const bool counts = policy_row_counts(a, row, label);
     if (threadIdx.x < 64) {
         PolicyResult r = no_policy();
-        const Pair *mine = pairs + row * (1 + parts);
+        const Total *mine = pairs + row * (1 + parts);
         if (counts) {
-            Pair p{-FLT_MAX, 0.0f};
+            Total p{-FLT_MAX, 0.0};
             if (label < a.cols) p = fold_pieces(mine, parts, a.c);
             r = policy_row(options_of(a), policy_inputs(a, row, label, label < a.cols ? mine[0].m : 0.0f), p);
         }
@@ -704,8 +723,8 @@ __global__ __launch_bounds__(THREADS) void policy_onchip_kernel(PolicyArgs<IO> a
     constexpr int WHOLE = ABOVE < 7 ? 0 : (ABOVE - 7) / THREADS;
     constexpr int SINGLES = (128 / static_cast<int>(sizeof(typename Io<IO>::elem)) + E - 2 + THREADS - 1) / THREADS;
     typedef typename Io<IO>::elem Elem;
-    __shared__ float sums[THREADS / 64][1];
-    __shared__ Pair slots[THREADS / 64];
+    __shared__ double sums[THREADS / 64];
+    __shared__ Total slots[THREADS / 64];
     __shared__ RowGradient shared;
     const int64_t row = blockIdx.x + static_cast<int64_t>(blockIdx.y) * gridDim.x;
     if (row >= a.rows) return;
@@ -800,13 +819,18 @@ __global__ __launch_bounds__(THREADS) void policy_onchip_kernel(PolicyArgs<IO> a
 #pragma unroll
     for (int i = 0; i < SINGLES; ++i)
         s[i % 4] += __builtin_amdgcn_exp2f(__builtin_fmaf(other_single(i), a.c.lo, __builtin_fmaf(other_single(i), a.c.hi, -shift)));
-    float total[1] = {(s[0] + s[1]) + (s[2] + s[3])};
-    block_sum<THREADS / 64, 1>(total, sums);
-    // times 2^-(c x_l - shift): shift is c x_l rounded
-    Pair p{at_label, total[0] * __builtin_amdgcn_exp2f(-__builtin_fmaf(at_label, a.c.lo, __builtin_fmaf(at_label, a.c.hi, -shift)))};
-    if (!(uniform(p.s) < 0x1p40f) || label >= a.cols) {
+    double total = wave_total((s[0] + s[1]) + (s[2] + s[3]));
+    if constexpr (THREADS > 64) {
+        if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = total;
+        __syncthreads();
+        total = 0.0;
+#pragma unroll
+        for (int w = 0; w < THREADS / 64; ++w) total += sums[w];
+    }
+    Total all{at_label, to_label(total, at_label, shift, a.c)};
+    if (!(uniform(static_cast<float>(all.s)) < 0x1p40f) || label >= a.cols) {
         // against the maximum: an unlikely label, special values, or logits that c times overflows
-        p = Pair{-FLT_MAX, 0.0f};
+        Pair p{-FLT_MAX, 0.0f};
 #pragma unroll
         for (int k = 0; k < VPT; ++k) {
             asm volatile("" : "+v"(r[k]), "+v"(p.s));
@@ -826,10 +850,10 @@ __global__ __launch_bounds__(THREADS) void policy_onchip_kernel(PolicyArgs<IO> a
             const float v[1] = {other_single(i)};
             add_values(p, v, a.c);
         }
-        p = block_pair<THREADS / 64>(p, slots, a.c);
+        all = block_pair<THREADS / 64>(p, slots, a.c);
     }
     if (threadIdx.x == 0) {
-        const PolicyResult res = policy_row(options_of(a), in, p);
+        const PolicyResult res = policy_row(options_of(a), in, all);
         put_policy(a, row, res);
         shared = res.gradient;
     }
@@ -903,12 +927,6 @@ __global__ __launch_bounds__(THREADS) void policy_onchip_kernel(PolicyArgs<IO> a
 }
 
 // ------------------------------------------------------------------------------------------------------- sums
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-    for (int step = 1; step < 64; step <<= 1) v += __shfl_xor(v, step, 64);
-    return v;
-}
-
 // out[0] = factor * sum of n values, in 64 bits and in a fixed order: one workgroup.
 __global__ __launch_bounds__(1024) void loss_sum_kernel(const float *__restrict__ values, int64_t n, float factor, float *out) {
     __shared__ double sums[16];
@@ -1017,7 +1035,7 @@ int pieces_per_row(int64_t rows, int64_t cols) {
 size_t workspace_bytes(int64_t rows, int64_t cols) {
     if (rows <= 0 || cols <= 0 || cols > kMaxColumns) return 0;
     const int parts = pieces_per_row(rows, cols);
-    return parts > 1 ? static_cast<size_t>(rows) * (1 + parts) * sizeof(Pair) : 0;
+    return parts > 1 ? static_cast<size_t>(rows) * (1 + parts) * sizeof(Total) : 0;
 }
 
 Scale two_parts(float scale) {
@@ -1064,7 +1082,7 @@ bool rows_lie_alike(const void *logits, int64_t ld, const void *dlogits, int64_t
 
 template <int IO, int THREADS>
 int launch_pieces(const typename Io<IO>::elem *logits, int64_t ld, const int32_t *labels, const float *weight, int64_t rows,
-                  int cols, Scale c, Pair *pairs, int parts, hipStream_t stream) {
+                  int cols, Scale c, Total *pairs, int parts, hipStream_t stream) {
     token_pieces_kernel<IO, THREADS><<<dim3(static_cast<unsigned>(parts), static_cast<unsigned>(rows)), dim3(THREADS), 0, stream>>>(
         logits, ld, labels, weight, cols, c, pairs);
     KO_CHECK_LAUNCH();
@@ -1084,7 +1102,7 @@ int logprob_entry(const void *logits, int64_t ld, const int32_t *labels, float s
                           static_cast<int>(cols), as_stream(stream)};
     const int parts = pieces_per_row(rows, cols);
     if (workspace && parts > 1) {
-        Pair *pairs = static_cast<Pair *>(workspace);
+        Total *pairs = static_cast<Total *>(workspace);
         if (const int st = launch_pieces<IO, 256>(a.logits, ld, labels, nullptr, rows, a.cols, a.c, pairs, parts, a.stream); st != KO_OK)
             return st;
         token_logprob_fold_kernel<IO><<<dim3(static_cast<unsigned>(rows)), dim3(64), 0, a.stream>>>(a, pairs, parts);
@@ -1156,7 +1174,7 @@ template <int IO>
 int launch_policy(const PolicyArgs<IO> &a, void *workspace) {
     const int parts = pieces_per_row(a.rows, a.cols);
     if (workspace && parts > 1) {
-        Pair *pairs = static_cast<Pair *>(workspace);
+        Total *pairs = static_cast<Total *>(workspace);
         if (const int st = launch_pieces<IO, 256>(a.logits, a.ld, a.labels, a.weight, a.rows, a.cols, a.c, pairs, parts, a.stream);
             st != KO_OK)
             return st;
