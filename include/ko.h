@@ -160,7 +160,7 @@ int ko_layernorm_16(const void *in, void *out, float *mean, float *rstd, const v
                     int policy, ko_stream_t stream);
 
 /* ---- gradients of the row operators ------------------------------------------------------------------------
- * The reference has forward operators only; these are what training through them needs.  Conventions:
+ * The reference has forward operators only; these are what training through them needs.  Conventions (cols up to 2^28 in all):
  * Workspace: calls that can use device memory for partial results take it from the caller - `workspace` points to at
  * least the number of bytes that the operator's *_workspace_bytes function returns for the call's sizes (a function of
  * the sizes alone; 0: none is needed), 16-byte aligned; its contents need no preparation and mean nothing after the
@@ -185,9 +185,8 @@ int ko_softmax_backward_16(const void *y, const void *dy, void *dx, int64_t rows
  *      dx = rstd (g - sum(g) / cols - xh sum(g xh) / D) + dres,   dgamma = sum_rows dy xh,   dbeta = sum_rows dy.
  * gamma NULL: 1.  dres (NULL: 0): the gradient that reaches `in` beside the norm, a residual branch's.  dgamma, dbeta:
  * fp32 in every entry, each NULL if not wanted; rows == 0 sets them to 0.  dx may be dy, in or dres.
- * Any cols; multiples of 4 (16-bit: 8) on 16-byte aligned tensors are the fast case, others are walked element by
- * element.  Rows longer than 16384 columns (8192 element by element) are read twice and dgamma / dbeta
- * take another pass. */
+ * Any cols up to 2^28 and element-aligned address run on 16-byte accesses, rows shorter than 16 bytes element by element.
+ * Rows longer than 16384 columns are read twice and dgamma / dbeta take another pass. */
 size_t ko_layernorm_backward_workspace_bytes(int64_t rows, int64_t cols);
 int ko_layernorm_backward_f32(const float *dy, const float *in, const float *mean, const float *rstd, const float *gamma,
                               const float *dres, float *dx, float *dgamma, float *dbeta, int64_t rows, int64_t cols,
@@ -198,8 +197,10 @@ int ko_layernorm_backward_16(const void *dy, const void *in, const float *mean, 
 
 /* ---- losses over rows of logits --------------------------------------------------------------------------------
  * logits: [rows] rows of cols elements, ld >= cols elements from one row to the next (what lies between is never read
- * or, in dlogits with its ldd, written).  Any cols, ld and element-aligned address run on 16-byte vectors; a
- * dlogits whose rows lie differently in their 16-byte vectors than the logits' rows is walked element by element.
+ * or, in dlogits with its ldd, written).  cols up to 2^28; any cols, ld and element-aligned address run on 16-byte vectors; a
+ * dlogits whose rows lie differently in their 16-byte vectors than the logits' rows is walked element by element.  How a row's
+ * sum is split depends on its length, on where it starts in a 128-byte line and, from 65537 columns on with a workspace, on the
+ * number of rows; on nothing else.
  * labels: device int32[rows].  A negative label marks a row that takes no part (a prompt's, padding): its logits are
  * never read, its outputs and its gradient are 0.  A label >= cols reads nothing out of place and makes the row's
  * outputs and its gradient NaN.  scale multiplies the logits (1 / temperature), from 1e-20 to 1e20.
@@ -227,8 +228,8 @@ int ko_token_logprob_backward_16(const void *logits, int64_t ld, const int32_t *
  *      ratio = exp(logp - old_logp),  s = min(ratio A, clip(ratio, 1 - clip_low, 1 + clip_high) A),  A = advantage[r],
  *      kl = exp(d) - 1 - d,  d = ref_logp - logp,  loss = weight (-s + kl_coef kl),
  * loss_sum = sum_r loss[r] (NULL if not wanted), dlogits = d loss_sum / d logits (NULL if not wanted; may be logits with
- * ldd = ld).  At a border of the clip range the gradient is the unclipped side's.  old_logp NULL: ratio 1, the policy that sampled is the one that trains.  ref_logp NULL:
- * no KL term.  weight NULL: 1; a row whose weight is 0 is treated as one without a label.  logp, kl (unweighted): [rows],
+ * ldd = ld).  At a border of the clip range the gradient is the unclipped side's.  old_logp NULL: ratio 1, the policy
+ * that sampled is the one that trains.  ref_logp NULL: no KL term.  weight NULL: 1; a row whose weight is 0 is treated as one without a label.  logp, kl (unweighted): [rows],
  * NULL if not wanted; loss: [rows].  clip_low in [0, 1], clip_high >= 0. */
 int ko_policy_loss_f32(const float *logits, int64_t ld, const int32_t *labels, const float *old_logp, const float *ref_logp,
                        const float *advantage, const float *weight, float scale, float clip_low, float clip_high, float kl_coef,

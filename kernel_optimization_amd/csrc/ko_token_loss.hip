@@ -927,11 +927,31 @@ __global__ __launch_bounds__(THREADS) void policy_onchip_kernel(PolicyArgs<IO> a
 }
 
 // ------------------------------------------------------------------------------------------------------- sums
-// out[0] = factor * sum of n values, in 64 bits and in a fixed order: one workgroup.
+// out[0] = factor * sum of n values, in 64 bits and in a fixed order: one workgroup, with sixteen loads per thread in flight
+// (a row's logits take longer than its loss here).
 __global__ __launch_bounds__(1024) void loss_sum_kernel(const float *__restrict__ values, int64_t n, float factor, float *out) {
     __shared__ double sums[16];
     double s = 0.0;
-    for (int64_t i = threadIdx.x; i < n; i += 1024) s += values[i];
+    if (n == 0) {  // the sum over no rows
+        if (threadIdx.x == 0) out[0] = 0.0f;
+        return;
+    }
+    constexpr int UNROLL = 16;
+    int64_t i = threadIdx.x;
+    for (; i - threadIdx.x + 1024 * UNROLL <= n; i += 1024 * UNROLL) {
+        float v[UNROLL];
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) v[u] = values[i + u * 1024];
+        double two[2] = {0.0, 0.0};
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) two[u & 1] += v[u];
+        s += two[0] + two[1];
+    }
+    float v[UNROLL];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) v[u] = values[i + u * 1024 < n ? i + u * 1024 : n - 1];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) s += i + u * 1024 < n ? v[u] : 0.0f;
     s = wave_sum(s);
     if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = s;
     __syncthreads();
@@ -1063,10 +1083,13 @@ int check_logits(const char *who, const void *logits, int64_t ld, const void *la
         return fail(KO_ERR_INVALID_ARGUMENT, "%s: workspace must be 16-byte aligned", who);
     return KO_OK;
 }
-int check_gradient(const char *who, const void *dlogits, int64_t ldd, size_t size, int64_t cols) {
+int check_gradient(const char *who, const void *dlogits, int64_t ldd, const void *logits, int64_t ld, size_t size, int64_t rows,
+                   int64_t cols) {
     if (ldd < cols) return fail(KO_ERR_INVALID_ARGUMENT, "%s: ldd=%lld is less than cols=%lld", who, (long long)ldd, (long long)cols);
     if (reinterpret_cast<uintptr_t>(dlogits) & (size - 1))
         return fail(KO_ERR_INVALID_ARGUMENT, "%s: dlogits must be aligned to its element type", who);
+    if (dlogits && dlogits == logits && rows > 1 && ldd != ld)  // a row's gradient would fall on other rows' logits
+        return fail(KO_ERR_INVALID_ARGUMENT, "%s: dlogits is logits, but ldd=%lld is not ld=%lld", who, (long long)ldd, (long long)ld);
     return KO_OK;
 }
 int check_floats(const char *who, std::initializer_list<const void *> pointers) {
@@ -1145,7 +1168,7 @@ int logprob_backward_entry(const void *logits, int64_t ld, const int32_t *labels
     constexpr size_t kSize = sizeof(typename Io<IO>::elem);
     static const char *const who = "token_logprob_backward";
     if (const int st = check_logits(who, logits, ld, labels, kSize, scale, rows, cols, nullptr, 0); st != KO_OK) return st;
-    if (const int st = check_gradient(who, dlogits, ldd, kSize, cols); st != KO_OK) return st;
+    if (const int st = check_gradient(who, dlogits, ldd, logits, ld, kSize, rows, cols); st != KO_OK) return st;
     if (const int st = check_floats(who, {row_stats, dlogp}); st != KO_OK) return st;
     if (rows == 0) return KO_OK;
     if (!row_stats || !dlogp || !dlogits) return fail(KO_ERR_INVALID_ARGUMENT, "%s: null row_stats/dlogp/dlogits pointer", who);
@@ -1233,7 +1256,7 @@ int policy_entry(const void *logits, int64_t ld, const int32_t *labels, const fl
     static const char *const who = "policy_loss";
     if (const int st = check_logits(who, logits, ld, labels, sizeof(Elem), scale, rows, cols, workspace, bytes); st != KO_OK) return st;
     if (dlogits) {
-        if (const int st = check_gradient(who, dlogits, ldd, sizeof(Elem), cols); st != KO_OK) return st;
+        if (const int st = check_gradient(who, dlogits, ldd, logits, ld, sizeof(Elem), rows, cols); st != KO_OK) return st;
     }
     if (const int st = check_floats(who, {old_logp, ref_logp, advantage, weight, logp, kl, loss, loss_sum}); st != KO_OK) return st;
     if (!(clip_low >= 0.0f && clip_low <= 1.0f) || !(clip_high >= 0.0f && clip_high < INFINITY))

@@ -187,3 +187,11 @@ def test_policy_and_preference_refusals():
     _refused(preference(beta=float("nan")), inv, "beta")
     _refused(preference(eps=1.5), inv, "label_smoothing")
     assert preference(pairs=0) == ko.KO_OK
+
+
+def test_gradients_over_logits_of_another_row_stride_are_refused():
+    """In place the rows have to lie alike: with another stride a row's gradient falls on logits that are still to be read."""
+    backward, policy = ko.lib().ko_token_logprob_backward_f32, ko.lib().ko_policy_loss_f32
+    _refused(backward(BAD, 12, BAD, 1.0, BAD, BAD, BAD, 8, 4, 8, None), ko.KO_ERR_INVALID_ARGUMENT, "ldd")
+    _refused(policy(BAD, 8, BAD, None, None, BAD, None, 1.0, 0.2, 0.2, 0.0, None, None, BAD, None, BAD, 12, 4, 8, None, 0, None),
+             ko.KO_ERR_INVALID_ARGUMENT, "ldd")
