@@ -249,6 +249,11 @@ __global__ __launch_bounds__(group_threads<LPR>(), LPR == 1024 ? 4 : LPR <= 64 &
             }
         }
         if constexpr (BLOCK) {
+            if constexpr (RES && !FULL) {
+                // dx may be dres, and a row's last 16 bytes are several threads': all of them have read before one writes
+#pragma unroll
+                for (int k = 0; k < VPL; ++k) asm volatile("" : "+v"(cur.res[k]));
+            }
             block_sum<THREADS / 64, 2>(s, slots[t & 1]);
         } else {
             s[0] = wave::allreduce<LPR, wave::Sum>(s[0]);

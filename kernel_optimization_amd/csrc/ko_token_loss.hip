@@ -357,8 +357,8 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(6))) vo
     typedef typename Io<IO>::raw Raw;
     __shared__ Total slots[2][WAVES];
     __shared__ Total again[WAVES];
-    int turn = 0;
-    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
+    int turn = 0;  // (alternates between the rows that use the slots: rows without a label pass no barrier)
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const typename Io<IO>::elem *src = a.logits + row * a.ld;
         const RowSpan<IO> span = span_of<IO>(src, a.cols);
         const int label = uniform(a.labels[row]);
@@ -430,6 +430,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(6))) vo
                 top = fmaxf(top, slots[turn][w].m);
                 sum += slots[turn][w].s;
             }
+            turn ^= 1;
         }
         Total p{at_label, to_label(sum, at_label, shift, a.c)};
         if (!(uniform(static_cast<float>(p.s)) < 0x1p40f)) {
@@ -643,13 +644,14 @@ template <int IO, int THREADS>
 __global__ __launch_bounds__(THREADS) void policy_reread_kernel(PolicyArgs<IO> a) {
     __shared__ Total slots[2][THREADS / 64];
     __shared__ RowGradient shared[2];
-    int turn = 0;
-    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
+    int turn = 1;  // (alternates between the rows that count: others pass no barrier)
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         int label;
         const bool counts = policy_row_counts(a, row, label);
         const typename Io<IO>::elem *src = a.logits + row * a.ld;
         const RowSpan<IO> span = span_of<IO>(a.dlogits ? a.dlogits + row * a.ldd : src, a.cols);
         if (counts) {
+            turn ^= 1;
             float at_label = 0.0f;
             Total p{-FLT_MAX, 0.0};
             if (label < a.cols) {

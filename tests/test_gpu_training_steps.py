@@ -313,3 +313,29 @@ def test_matrices_beyond_32_bits(ko):
         ko.token_logprob_backward16(x, dl.ptr + at, stats.ptr + 2 * at, df.ptr + at, o, n, cols, **typed)
     same("token_logprob", scores)
     same("policy", lambda x, y, o, at, n: ko.policy_loss16(x, dl.ptr + at, df.ptr + at, loss.ptr + at, n, cols, dlogits=o, **typed))
+
+
+def test_more_rows_than_a_grid_has_workgroups(ko):
+    """4.3 million short rows: workgroups walk on to rows behind the grid's last, some of them without a label or with one beyond
+    the vocabulary."""
+    rows, cols = 4300003, 8
+    rng = np.random.default_rng(91)
+    x = rng.normal(0, 1, (rows, cols)).astype(np.float32)
+    labels = rng.integers(0, cols, rows).astype(np.int32)
+    labels[1::3] = -1
+    labels[2::7] = cols
+    advantage = rng.normal(0, 1, rows).astype(np.float32)
+    dx, dl, da = (ko.DeviceBuffer.from_numpy(v) for v in (x, labels, advantage))
+    logp, loss, total = ko.DeviceBuffer(4 * rows), ko.DeviceBuffer(4 * rows), ko.DeviceBuffer(4)
+    scores = ref.Scores(x.astype(np.float64), np.where(labels == cols, 0, labels))
+    beyond, dead = labels == cols, labels < 0
+    counted = ~(beyond | dead)
+    for run in (lambda: ko.token_logprob(dx, dl, logp, rows, cols),
+                lambda: ko.policy_loss(dx, dl, da, loss, rows, cols, logp=logp, loss_sum=total)):
+        logp.upload(np.full(rows, 7, np.float32))
+        run()
+        ko.synchronize()
+        got = logp.download(np.float32, (rows,))
+        assert np.isnan(got[beyond]).all() and (got[dead] == 0).all()
+        ref.assert_within(got[counted], scores.logp[counted], scores.logp_off[counted], "logp")
+    np.testing.assert_array_equal(loss.download(np.float32, (rows,))[counted], -advantage[counted])   # ratio 1
