@@ -423,3 +423,10 @@ def test_policy_loss_where_one_way_ends_and_the_next_begins(ko, vectors, kind):
         case = policy_case(call, vectors)
         got = run_policy(call, case, pad)
         check_policy(call, got, case)
+
+
+@pytest.mark.parametrize("lens", [[3, 2] * 2 + [0, 9], [70, 300] * 4, [0, 1] + [200, 150] * 4, [33, 64] * 16, [31, 1] * 17, [4000, 4184],
+                                  [4000, 4185], [513, 511] * 8, [8000, 1, 0, 0, 1, 0]])
+def test_preference_loss_of_few_and_more_pairs(ko, lens):
+    """Both sides of the border between one workgroup for every pair and one for each."""
+    test_preference_loss(ko, lens, 0.1)
