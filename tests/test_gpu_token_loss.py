@@ -430,3 +430,18 @@ def test_policy_loss_where_one_way_ends_and_the_next_begins(ko, vectors, kind):
 def test_preference_loss_of_few_and_more_pairs(ko, lens):
     """Both sides of the border between one workgroup for every pair and one for each."""
     test_preference_loss(ko, lens, 0.1)
+
+
+# rows longer than the registers of a workgroup (16384 vectors): in pieces, and one workgroup each
+@pytest.mark.parametrize("rows", [5, 65])
+@pytest.mark.parametrize("kind,cols", [("f32", 70001), ("bf16", 140001)])
+def test_rows_longer_than_the_registers(ko, rows, kind, cols):
+    test_policy_loss_unlikely_labels_and_lowest_values(ko, rows, cols, kind)
+    test_labels_in_the_first_and_last_columns(ko, rows, cols, kind)
+
+
+@pytest.mark.parametrize("rows,cols", [(5, 70001), (65, 70001)])
+def test_special_rows_longer_than_the_registers(ko, rows, cols):
+    test_policy_loss_weight_zero_rows_are_not_read(ko, rows, cols)
+    test_labels_beyond_the_vocabulary_and_nan_logits(ko, rows, cols)
+    test_policy_loss_options(ko, rows, cols)
