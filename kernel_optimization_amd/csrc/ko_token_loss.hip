@@ -343,6 +343,44 @@ __device__ __forceinline__ void put_score(const A &a, int64_t row, bool live, co
     }
 }
 
+// One vector's share of a row's sum and maximum.  `ragged`: it may hold the label or lie past the row's end.
+template <int IO>
+__device__ __forceinline__ void add_vector(const typename Io<IO>::raw &r, int j, bool ragged, int nvec, int in_vecs, float shift,
+                                           Scale c, float (&s)[4], float &top) {
+    constexpr int E = Io<IO>::E;
+    float x[E];
+    Io<IO>::unpack(r, x);
+    if (ragged) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[e] = j >= nvec || E * j + e == in_vecs ? -INFINITY : x[e];
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        top = fmaxf(top, x[e]);
+        s[e % 4] += __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], c.lo, __builtin_fmaf(x[e], c.hi, -shift)));
+    }
+}
+// A thread's single elements.
+template <int IO, int THREADS>
+__device__ __forceinline__ void add_singles(const typename Io<IO>::elem *src, const RowSpan<IO> &span, int label, float shift, Scale c,
+                                            float (&s)[4], float &top) {
+    for (int i = threadIdx.x; i < span.singles; i += THREADS) {
+        const int column = single_column(span, i);
+        const float x = column == label ? -INFINITY : Io<IO>::scalar(src + column);
+        top = fmaxf(top, x);
+        s[1] += __builtin_amdgcn_exp2f(__builtin_fmaf(x, c.lo, __builtin_fmaf(x, c.hi, -shift)));
+    }
+}
+// The score of a row from its label's logit, the sum relative to that and the row's maximum.
+template <class A>
+__device__ __forceinline__ RowScore label_score(const A &a, Total p, float at_label, float top) {
+    RowScore score = score_row(p, at_label, a.scale, a.c);
+    // the sum is relative to the label: its logarithm relative to the maximum
+    score.logsum += (static_cast<double>(score.top) - static_cast<double>(top)) * static_cast<double>(a.scale);
+    score.top = top;
+    return score;
+}
+
 // One workgroup per row, the next batch of U vectors per thread in flight while this one is added up.  As in
 // policy_onchip_kernel the exponentials are taken against the label's logit, and the row's maximum is noted by the way; a label
 // so unlikely that the sum reaches 2^40, or a sum that is not a number, is summed again with a running maximum.  Bound: memory
@@ -384,19 +422,8 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(6))) vo
             const bool ragged = begin + U * THREADS > span.nvec || (label_vec >= begin && label_vec < begin + U * THREADS);
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                float x[E];
-                Io<IO>::unpack(r[u], x);
-                if (ragged) {
-                    if (begin + u * THREADS >= span.nvec) break;
-                    const int j = first + u * THREADS;
-#pragma unroll
-                    for (int e = 0; e < E; ++e) x[e] = j >= span.nvec || E * j + e == in_vecs ? -INFINITY : x[e];
-                }
-#pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    top = fmaxf(top, x[e]);
-                    s[e % 4] += __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], a.c.lo, __builtin_fmaf(x[e], a.c.hi, -shift)));
-                }
+                if (ragged && begin + u * THREADS >= span.nvec) break;
+                add_vector<IO>(r[u], first + u * THREADS, ragged, span.nvec, in_vecs, shift, a.c, s, top);
             }
         };
         Raw r[2][U];
@@ -412,12 +439,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(6))) vo
             j += U * THREADS;
             if (j - static_cast<int>(threadIdx.x) >= span.nvec) break;
         }
-        for (int i = threadIdx.x; i < span.singles; i += THREADS) {
-            const int column = single_column(span, i);
-            const float x = column == label ? -INFINITY : Io<IO>::scalar(src + column);
-            top = fmaxf(top, x);
-            s[1] += __builtin_amdgcn_exp2f(__builtin_fmaf(x, a.c.lo, __builtin_fmaf(x, a.c.hi, -shift)));
-        }
+        add_singles<IO, THREADS>(src, span, label, shift, a.c, s, top);
         top = wave::allreduce<64, wave::Max>(top);
         double sum = wave_total((s[0] + s[1]) + (s[2] + s[3]));
         if constexpr (WAVES > 1) {
@@ -438,13 +460,77 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(6))) vo
             top = fmaxf(p.m, at_label);
             __syncthreads();  // (read before the next row writes them)
         }
-        if (threadIdx.x == 0) {
-            RowScore score = score_row(p, at_label, a.scale, a.c);
-            // the sum is relative to the label: its logarithm relative to the maximum
-            score.logsum += (static_cast<double>(score.top) - static_cast<double>(top)) * static_cast<double>(a.scale);
-            score.top = top;
-            put_score(a, row, true, score);
+        if (threadIdx.x == 0) put_score(a, row, true, label_score(a, p, at_label, top));
+    }
+}
+
+// Short rows, of U 64 vectors at most: a wavefront takes kShortRows of them, and the arithmetic of a row's score - several times
+// that of its sum, in one lane - is done for all of them at once, a row per lane (1 GiB of bf16 rows: 512 columns 227 us, 1024
+// columns 197; a row per wavefront 471 and 281; four rows 252 and 206, sixteen 238 and, for want of registers, 257).
+constexpr int kShortRows = 8;
+template <int IO, int U>
+__global__ __launch_bounds__(64) void token_logprob_short_kernel(ScoreArgs<IO> a) {
+    typedef typename Io<IO>::elem Elem;
+    const int lane = threadIdx.x;
+    auto of = [&](float v, int i) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), i)); };
+    for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * kShortRows; row0 < a.rows; row0 += static_cast<int64_t>(gridDim.x) * kShortRows) {
+        const int n = a.rows - row0 < kShortRows ? static_cast<int>(a.rows - row0) : kShortRows;
+        const int my_label = lane < n ? a.labels[row0 + lane] : -1;
+        const bool reads = my_label >= 0 && my_label < a.cols;
+        const float my_at = reads ? Io<IO>::scalar(a.logits + (row0 + lane) * a.ld + my_label) : 0.0f;
+        Total mine{my_at, 0.0};
+        float my_top = my_at;
+        typename Io<IO>::raw r[kShortRows][U];
+        // rows without a label are not read: their buffers are empty
+#pragma unroll
+        for (int i = 0; i < kShortRows; ++i) {
+            const Elem *src = a.logits + (row0 + i) * a.ld;
+            const RowSpan<IO> span = span_of<IO>(src, a.cols);
+            const int label = __builtin_amdgcn_readlane(my_label, i);
+            const Buffer from = buffer_of(src + span.head, label >= 0 && label < a.cols ? Io<IO>::kBytes * span.nvec : 0);
+#pragma unroll
+            for (int u = 0; u < U; ++u) r[i][u] = buffer_load<IO>(from, Io<IO>::kBytes * static_cast<uint32_t>(lane + u * 64));
         }
+#pragma unroll
+        for (int i = 0; i < kShortRows; ++i) {
+            const int label = __builtin_amdgcn_readlane(my_label, i);
+            if (label < 0 || label >= a.cols) continue;
+            const Elem *src = a.logits + (row0 + i) * a.ld;
+            const RowSpan<IO> span = span_of<IO>(src, a.cols);
+            const int in_vecs = label - span.head;
+            const float at_label = of(my_at, i);
+            const float shift = at_label * a.c.hi;
+            float top = at_label;
+            float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (u * 64 >= span.nvec) break;
+                add_vector<IO>(r[i][u], lane + u * 64, true, span.nvec, in_vecs, shift, a.c, s, top);
+            }
+            add_singles<IO, 64>(src, span, label, shift, a.c, s, top);
+            top = wave::allreduce<64, wave::Max>(top);
+            const double sum = wave_total((s[0] + s[1]) + (s[2] + s[3]));
+            if (lane == i) {
+                mine.s = sum;
+                my_top = top;
+            }
+        }
+        mine.s = to_label(mine.s, my_at, my_at * a.c.hi, a.c);
+        // unlikely labels, special values: against the maximum, a row at a time
+        uint64_t again = __ballot(reads && !(static_cast<float>(mine.s) < 0x1p40f));
+        while (again) {
+            const int i = __builtin_ctzll(again);
+            again &= again - 1;
+            const Elem *src = a.logits + (row0 + i) * a.ld;
+            const RowSpan<IO> span = span_of<IO>(src, a.cols);
+            const Total p = block_pair<1>(thread_pair<IO, 64>(src, span, 0, span.nvec, true, __builtin_amdgcn_readlane(my_label, i), a.c),
+                                          nullptr, a.c);
+            if (lane == i) {
+                mine = p;
+                my_top = fmaxf(p.m, my_at);
+            }
+        }
+        if (lane < n) put_score(a, row0 + lane, my_label >= 0, reads ? label_score(a, mine, my_at, my_top) : nan_score());
     }
 }
 
@@ -706,6 +792,90 @@ __global__ __launch_bounds__(THREADS) void policy_pieces_kernel(PolicyArgs<IO> a
     const auto label_grad = [&](float) { return g.label_grad; };
     write_gradient<IO, THREADS>(src, a.dlogits + row * a.ldd, span, lo, hi, part == 0, g.live, label, g.top, g.a, label_grad,
                                 a.c);
+}
+
+// Short rows, of 64 vectors at most, as in token_logprob_short_kernel: the rows stay in the registers of a wavefront, the losses
+// are worked out a row per lane, and each row's gradient follows (1 GiB of bf16 logits in rows of 512 columns 386 us, 5.6 TB/s; a
+// wavefront per row 545).
+template <int IO>
+__global__ __launch_bounds__(64) void policy_short_kernel(PolicyArgs<IO> a) {
+    constexpr int E = Io<IO>::E;
+    typedef typename Io<IO>::elem Elem;
+    const int lane = threadIdx.x;
+    const int64_t row0 = (blockIdx.x + static_cast<int64_t>(blockIdx.y) * gridDim.x) * kShortRows;
+    if (row0 >= a.rows) return;
+    const int n = a.rows - row0 < kShortRows ? static_cast<int>(a.rows - row0) : kShortRows;
+    auto of = [&](float v, int i) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), i)); };
+    const int my_label = lane < n ? a.labels[row0 + lane] : -1;
+    const bool counts = my_label >= 0 && (!a.weight || a.weight[row0 + lane] != 0.0f);
+    const bool reads = counts && my_label < a.cols;
+    const uint64_t reading = __ballot(reads);
+    const float my_at = reads ? Io<IO>::scalar(a.logits + (row0 + lane) * a.ld + my_label) : 0.0f;
+    PolicyRow in{};
+    if (counts) in = policy_inputs(a, row0 + lane, my_label, my_at);
+    Total mine{my_at, 0.0};
+    typename Io<IO>::raw r[kShortRows];
+#pragma unroll
+    for (int i = 0; i < kShortRows; ++i) {  // (rows that are not read have empty buffers)
+        const RowSpan<IO> span = span_of<IO>(a.dlogits + (row0 + i) * a.ldd, a.cols);
+        const Buffer from = buffer_of(a.logits + (row0 + i) * a.ld + span.head, reading >> i & 1 ? Io<IO>::kBytes * span.nvec : 0);
+        r[i] = buffer_load<IO>(from, Io<IO>::kBytes * static_cast<uint32_t>(lane));
+    }
+#pragma unroll
+    for (int i = 0; i < kShortRows; ++i) {
+        if (!(reading >> i & 1)) continue;
+        const Elem *src = a.logits + (row0 + i) * a.ld;
+        const RowSpan<IO> span = span_of<IO>(a.dlogits + (row0 + i) * a.ldd, a.cols);
+        const int label = __builtin_amdgcn_readlane(my_label, i);
+        const float shift = of(my_at, i) * a.c.hi;
+        float top = 0.0f;
+        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        add_vector<IO>(r[i], lane, true, span.nvec, label - span.head, shift, a.c, s, top);
+        add_singles<IO, 64>(src, span, label, shift, a.c, s, top);
+        const double sum = wave_total((s[0] + s[1]) + (s[2] + s[3]));
+        if (lane == i) mine.s = sum;
+    }
+    mine.s = to_label(mine.s, my_at, my_at * a.c.hi, a.c);
+    uint64_t again = __ballot(reads && !(static_cast<float>(mine.s) < 0x1p40f));
+    while (again) {
+        const int i = __builtin_ctzll(again);
+        again &= again - 1;
+        const Elem *src = a.logits + (row0 + i) * a.ld;
+        const RowSpan<IO> span = span_of<IO>(a.dlogits + (row0 + i) * a.ldd, a.cols);
+        const Total p = block_pair<1>(thread_pair<IO, 64>(src, span, 0, span.nvec, true, __builtin_amdgcn_readlane(my_label, i), a.c),
+                                      nullptr, a.c);
+        if (lane == i) mine = p;
+    }
+    const PolicyResult res = counts ? policy_row(options_of(a), in, mine) : no_policy();
+    if (lane < n) put_policy(a, row0 + lane, res);
+#pragma unroll
+    for (int i = 0; i < kShortRows; ++i) {
+        if (i >= n) break;
+        const Elem *src = a.logits + (row0 + i) * a.ld;
+        Elem *dst = a.dlogits + (row0 + i) * a.ldd;
+        const RowSpan<IO> span = span_of<IO>(dst, a.cols);
+        const int label = __builtin_amdgcn_readlane(my_label, i);
+        const float factor = of(res.gradient.a, i), at_label = of(res.gradient.label_grad, i), top = of(res.gradient.top, i);
+        const bool live = __builtin_amdgcn_readlane(static_cast<int>(res.gradient.live), i) != 0;
+        const int in_vecs = label - span.head;
+        convert_again<IO>(r[i]);
+        float x[E];
+        Io<IO>::unpack(r[i], x);
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            x[e] = !live ? 0.0f : E * lane + e == in_vecs ? at_label : factor * exp_scaled(x[e] - top, a.c);
+        buffer_store<IO, true>(buffer_of(dst + span.head, Io<IO>::kBytes * span.nvec), Io<IO>::kBytes * static_cast<uint32_t>(lane), x);
+        for (int j = lane; j < span.singles; j += 64) {
+            constexpr int ONE = io_by_element(IO);
+            const int column = single_column(span, j);
+            float v[1] = {0.0f};
+            if (live) {
+                v[0] = Io<IO>::scalar(src + column);
+                v[0] = column == label ? at_label : factor * exp_scaled(v[0] - top, a.c);
+            }
+            Io<ONE>::template store<true>(dst + column, v);
+        }
+    }
 }
 
 // A row in the registers of a workgroup, VPT vectors per thread, one workgroup per row: one read, one write.  (Workgroups that
@@ -1196,8 +1366,11 @@ int logprob_entry(const void *logits, int64_t ld, const int32_t *labels, float s
     // rows of few vectors: as many threads as make one batch of them (8192 bf16 columns 187 us for 1 GiB, 208 with 512 threads and
     // 4096 columns 190 against 383 with 256, half of them idle).  Long rows: 1024 threads took 258 us for 1 GiB of rows of
     // 50257 bf16 columns, 512 take 152, and 32 such rows 6.7 against 7.2.
-    if (nvec <= 128) token_logprob_row_kernel<IO, 64, 2><<<grid, dim3(64), 0, a.stream>>>(a);
-    else if (nvec <= 256) token_logprob_row_kernel<IO, 64, 4><<<grid, dim3(64), 0, a.stream>>>(a);
+    if (nvec <= 128) {
+        const dim3 g = row_grid((rows + kShortRows - 1) / kShortRows, 64);
+        if (nvec <= 64) token_logprob_short_kernel<IO, 1><<<g, dim3(64), 0, a.stream>>>(a);
+        else token_logprob_short_kernel<IO, 2><<<g, dim3(64), 0, a.stream>>>(a);
+    } else if (nvec <= 256) token_logprob_row_kernel<IO, 64, 4><<<grid, dim3(64), 0, a.stream>>>(a);
     else if (nvec <= 512) token_logprob_row_kernel<IO, 128, 4><<<grid, dim3(128), 0, a.stream>>>(a);
     else if (nvec <= 1024) token_logprob_row_kernel<IO, 256, 4><<<grid, dim3(256), 0, a.stream>>>(a);
     else token_logprob_row_kernel<IO, 512, 4><<<grid, dim3(512), 0, a.stream>>>(a);
@@ -1245,13 +1418,24 @@ template <int IO, int ABOVE, int THREADS, int VPT, bool REST = false>
 int launch_onchip(const PolicyArgs<IO> &a) {
     static_assert(REST ? ABOVE >= THREADS * VPT + 7 : ABOVE < THREADS * VPT, "");
     const int nvec = a.cols / Io<IO>::E;
-    if ((ABOVE && nvec <= ABOVE) || (!REST && nvec > THREADS * VPT)) return fail(KO_ERR_UNSUPPORTED_SHAPE, "policy_loss: cols=%d", a.cols);
+    if (nvec <= ABOVE || (!REST && nvec > THREADS * VPT)) return fail(KO_ERR_UNSUPPORTED_SHAPE, "policy_loss: cols=%d", a.cols);
     // (a grid's threads number less than 2^32 in one dimension)
     const int64_t wide = a.rows < (1 << 20) ? a.rows : (1 << 20);
     const int64_t high = (a.rows + wide - 1) / wide;
     if (high > 65535) return fail(KO_ERR_UNSUPPORTED_SHAPE, "policy_loss: rows=%lld too many", (long long)a.rows);
     const dim3 g(static_cast<unsigned>(wide), static_cast<unsigned>(high)), b(THREADS);
     policy_onchip_kernel<IO, ABOVE, THREADS, VPT, REST><<<g, b, 0, a.stream>>>(a);
+    KO_CHECK_LAUNCH();
+    return KO_OK;
+}
+
+template <int IO>
+int launch_short(const PolicyArgs<IO> &a) {
+    const int64_t groups = (a.rows + kShortRows - 1) / kShortRows;
+    const int64_t wide = groups < (1 << 20) ? groups : (1 << 20);
+    const int64_t high = (groups + wide - 1) / wide;
+    if (high > 65535) return fail(KO_ERR_UNSUPPORTED_SHAPE, "policy_loss: rows=%lld too many", (long long)a.rows);
+    policy_short_kernel<IO><<<dim3(static_cast<unsigned>(wide), static_cast<unsigned>(high)), dim3(64), 0, a.stream>>>(a);
     KO_CHECK_LAUNCH();
     return KO_OK;
 }
@@ -1276,7 +1460,7 @@ int launch_policy(const PolicyArgs<IO> &a, void *workspace) {
             // against 356 with eight and 372 with two per thread, 1024 columns 393 against 675 with one.  Long rows: 512 threads
             // (two workgroups per compute unit, one of which loads or stores) as far as their registers go, 49152 columns
             // 369 us against 412 with 1024 threads; three per thread where that is the number (24576 columns, 349 against 370).
-            if (nvec <= 64) return launch_onchip<IO, 0, 64, 1>(a);
+            if (nvec <= 64) return launch_short<IO>(a);
             if (nvec <= 128) return launch_onchip<IO, 64, 64, 2>(a);
             if (nvec <= 256) return launch_onchip<IO, 128, 64, 4>(a);
             if (nvec <= 512) return launch_onchip<IO, 256, 128, 4>(a);

@@ -445,3 +445,21 @@ def test_special_rows_longer_than_the_registers(ko, rows, cols):
     test_policy_loss_weight_zero_rows_are_not_read(ko, rows, cols)
     test_labels_beyond_the_vocabulary_and_nan_logits(ko, rows, cols)
     test_policy_loss_options(ko, rows, cols)
+
+
+# several short rows per wavefront: every number of them at the end, every kind of row among the others
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows,cols", [(1, 40), (7, 256), (8, 257), (9, 512), (17, 100), (1003, 500), (23, 1000), (64, 1030), (5000, 90)])
+def test_short_rows(ko, rows, cols, kind):
+    test_token_logprob_and_its_gradient(ko, rows, cols, kind)
+    test_policy_loss(ko, rows, cols, kind)
+    if rows > 20:
+        test_policy_loss_unlikely_labels_and_lowest_values(ko, rows, cols, kind)
+        test_labels_in_the_first_and_last_columns(ko, rows, cols, kind)
+
+
+@pytest.mark.parametrize("rows,cols", [(30, 90), (30, 250), (30, 509)])
+def test_special_short_rows(ko, rows, cols):
+    test_policy_loss_weight_zero_rows_are_not_read(ko, rows, cols)
+    test_labels_beyond_the_vocabulary_and_nan_logits(ko, rows, cols)
+    test_policy_loss_options(ko, rows, cols)
