@@ -199,8 +199,8 @@ int ko_layernorm_backward_16(const void *dy, const void *in, const float *mean, 
  * logits: [rows] rows of cols elements, ld >= cols elements from one row to the next (what lies between is never read
  * or, in dlogits with its ldd, written).  cols up to 2^28; any cols, ld and element-aligned address run on 16-byte vectors; a
  * dlogits whose rows lie differently in their 16-byte vectors than the logits' rows is walked element by element.  How a row's
- * sum is split depends on its length, on where it starts in a 128-byte line and, from 65537 columns on with a workspace, on the
- * number of rows; on nothing else.
+ * sum is split depends on its length, on where it starts in a 128-byte line and, from 65537 columns on with a workspace and in
+ * the policy loss up to 512 (fp32: 256) columns, on the number of rows; on nothing else.
  * labels: device int32[rows].  A negative label marks a row that takes no part (a prompt's, padding): its logits are
  * never read, its outputs and its gradient are 0.  A label >= cols reads nothing out of place and makes the row's
  * outputs and its gradient NaN.  scale multiplies the logits (1 / temperature), from 1e-20 to 1e20.

@@ -464,10 +464,14 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(6))) vo
     }
 }
 
-// Short rows, of U 64 vectors at most: a wavefront takes kShortRows of them, and the arithmetic of a row's score - several times
+// Many short rows, of U 64 vectors at most: a wavefront takes kShortRows of them, and the arithmetic of a row's score - several times
 // that of its sum, in one lane - is done for all of them at once, a row per lane (1 GiB of bf16 rows: 512 columns 227 us, 1024
 // columns 197; a row per wavefront 471 and 281; four rows 252 and 206, sixteen 238 and, for want of registers, 257).
 constexpr int kShortRows = 8;
+// Fewer rows are better off with a wavefront each: eight rows in turn take 2 to 4 us longer than one (64 rows of 512 bf16
+// columns: log-probabilities 5.7 us against 3.9, policy loss 8.2 against 4.3), which pays from here on, for the policy loss from
+// twice as many.
+constexpr int64_t kManyRows = 16384;
 template <int IO, int U>
 __global__ __launch_bounds__(64) void token_logprob_short_kernel(ScoreArgs<IO> a) {
     typedef typename Io<IO>::elem Elem;
@@ -794,7 +798,7 @@ __global__ __launch_bounds__(THREADS) void policy_pieces_kernel(PolicyArgs<IO> a
                                 a.c);
 }
 
-// Short rows, of 64 vectors at most, as in token_logprob_short_kernel: the rows stay in the registers of a wavefront, the losses
+// Many short rows, of 64 vectors at most, as in token_logprob_short_kernel: the rows stay in the registers of a wavefront, the losses
 // are worked out a row per lane, and each row's gradient follows (1 GiB of bf16 logits in rows of 512 columns 386 us, 5.6 TB/s; a
 // wavefront per row 545).
 template <int IO>
@@ -1366,11 +1370,12 @@ int logprob_entry(const void *logits, int64_t ld, const int32_t *labels, float s
     // rows of few vectors: as many threads as make one batch of them (8192 bf16 columns 187 us for 1 GiB, 208 with 512 threads and
     // 4096 columns 190 against 383 with 256, half of them idle).  Long rows: 1024 threads took 258 us for 1 GiB of rows of
     // 50257 bf16 columns, 512 take 152, and 32 such rows 6.7 against 7.2.
-    if (nvec <= 128) {
+    if (nvec <= 128 && rows >= kManyRows) {
         const dim3 g = row_grid((rows + kShortRows - 1) / kShortRows, 64);
         if (nvec <= 64) token_logprob_short_kernel<IO, 1><<<g, dim3(64), 0, a.stream>>>(a);
         else token_logprob_short_kernel<IO, 2><<<g, dim3(64), 0, a.stream>>>(a);
-    } else if (nvec <= 256) token_logprob_row_kernel<IO, 64, 4><<<grid, dim3(64), 0, a.stream>>>(a);
+    } else if (nvec <= 128) token_logprob_row_kernel<IO, 64, 2><<<grid, dim3(64), 0, a.stream>>>(a);
+    else if (nvec <= 256) token_logprob_row_kernel<IO, 64, 4><<<grid, dim3(64), 0, a.stream>>>(a);
     else if (nvec <= 512) token_logprob_row_kernel<IO, 128, 4><<<grid, dim3(128), 0, a.stream>>>(a);
     else if (nvec <= 1024) token_logprob_row_kernel<IO, 256, 4><<<grid, dim3(256), 0, a.stream>>>(a);
     else token_logprob_row_kernel<IO, 512, 4><<<grid, dim3(512), 0, a.stream>>>(a);
@@ -1418,7 +1423,7 @@ template <int IO, int ABOVE, int THREADS, int VPT, bool REST = false>
 int launch_onchip(const PolicyArgs<IO> &a) {
     static_assert(REST ? ABOVE >= THREADS * VPT + 7 : ABOVE < THREADS * VPT, "");
     const int nvec = a.cols / Io<IO>::E;
-    if (nvec <= ABOVE || (!REST && nvec > THREADS * VPT)) return fail(KO_ERR_UNSUPPORTED_SHAPE, "policy_loss: cols=%d", a.cols);
+    if ((ABOVE && nvec <= ABOVE) || (!REST && nvec > THREADS * VPT)) return fail(KO_ERR_UNSUPPORTED_SHAPE, "policy_loss: cols=%d", a.cols);
     // (a grid's threads number less than 2^32 in one dimension)
     const int64_t wide = a.rows < (1 << 20) ? a.rows : (1 << 20);
     const int64_t high = (a.rows + wide - 1) / wide;
@@ -1460,7 +1465,8 @@ int launch_policy(const PolicyArgs<IO> &a, void *workspace) {
             // against 356 with eight and 372 with two per thread, 1024 columns 393 against 675 with one.  Long rows: 512 threads
             // (two workgroups per compute unit, one of which loads or stores) as far as their registers go, 49152 columns
             // 369 us against 412 with 1024 threads; three per thread where that is the number (24576 columns, 349 against 370).
-            if (nvec <= 64) return launch_short<IO>(a);
+            if (nvec <= 64 && a.rows >= 2 * kManyRows) return launch_short<IO>(a);
+            if (nvec <= 64) return launch_onchip<IO, 0, 64, 1>(a);
             if (nvec <= 128) return launch_onchip<IO, 64, 64, 2>(a);
             if (nvec <= 256) return launch_onchip<IO, 128, 64, 4>(a);
             if (nvec <= 512) return launch_onchip<IO, 256, 128, 4>(a);

@@ -463,3 +463,20 @@ def test_special_short_rows(ko, rows, cols):
     test_policy_loss_weight_zero_rows_are_not_read(ko, rows, cols)
     test_labels_beyond_the_vocabulary_and_nan_logits(ko, rows, cols)
     test_policy_loss_options(ko, rows, cols)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows,cols", [(16384, 130), (16391, 40), (32768, 64), (33003, 65), (33001, 250)])
+def test_many_short_rows(ko, rows, cols, kind):
+    """Eight rows per wavefront, the log-probabilities' from 16384 rows on, the policy loss's from 32768."""
+    test_token_logprob_and_its_gradient(ko, rows, cols, kind)
+    test_policy_loss(ko, rows, cols, kind)
+    test_policy_loss_unlikely_labels_and_lowest_values(ko, rows, cols, kind)
+    test_labels_in_the_first_and_last_columns(ko, rows, cols, kind)
+
+
+@pytest.mark.parametrize("rows,cols", [(33001, 90), (16400, 509)])
+def test_special_ones_among_many_short_rows(ko, rows, cols):
+    test_policy_loss_weight_zero_rows_are_not_read(ko, rows, cols)
+    test_labels_beyond_the_vocabulary_and_nan_logits(ko, rows, cols)
+    test_policy_loss_options(ko, rows, cols)
