@@ -205,10 +205,10 @@ __device__ __forceinline__ Pair thread_pair(const typename Io<IO>::elem *row, co
 }
 
 // ---- a row's scalars
-// Logarithms here are of the size of 10 and get subtracted from each other: in fp32 they would carry an error of 5e-7,
-// ten times that of the sums.  So they are 64-bit numbers, put together from fp32 functions of arguments whose result is
-// small (64-bit functions would take as long as 1.5 us per row and, their constants kept in registers, a hundred
-// registers of kernels that need them for the row).
+// Logarithms here are of the size of 10 and get subtracted from each other, and a KL term takes such a difference squared: in
+// fp32 they would carry an error of 5e-7, ten times that of the sums.  So they are 64-bit numbers, by a short series; the rest
+// are fp32 functions (64-bit ones from the library would take as long as 1.5 us per row and, their constants kept in registers,
+// a hundred registers of kernels that need them for the row).
 struct RowScore {
     double logp;     // log probability of the label
     double logsum;   // log sum_j exp(scale (x_j - top)), the label included
@@ -216,17 +216,28 @@ struct RowScore {
     float inv_total; // 1 / (S + e)
     float rest;      // S / (S + e): what the label's probability leaves
 };
-// log(t) of a positive t, within 3e-8 absolute
+// log(t) of a positive t, within 1e-12 absolute: t = 2^k f, f within sqrt(2) of 1, log f = 2 atanh(u), u = (f - 1) / (f + 1),
+// |u| < 0.172, by its series up to u^13.
 __device__ __forceinline__ double log_in_parts(double t) {
     if (!(t < 1e30)) return t;
     int k;
-    float f = frexpf(static_cast<float>(t), &k);
-    const float rest = static_cast<float>(t - static_cast<double>(static_cast<float>(t))) / static_cast<float>(t);
-    if (f < 0.70710678f) {
-        f *= 2.0f;
+    (void)frexpf(static_cast<float>(t), &k);
+    double f = ldexp(t, -k);
+    if (f < 0.70710678) {
+        f *= 2.0;
         --k;
     }
-    return __builtin_fma(static_cast<double>(k), 0.69314718055994531, static_cast<double>(logf(f)) + rest);
+    // the reciprocal in 32 bits and one Newton step
+    double r = 1.0f / static_cast<float>(f + 1.0);
+    r = __builtin_fma(r, __builtin_fma(-(f + 1.0), r, 1.0), r);
+    const double u = (f - 1.0) * r, w = u * u;
+    double p = __builtin_fma(w, 1.0 / 13.0, 1.0 / 11.0);
+    p = __builtin_fma(w, p, 1.0 / 9.0);
+    p = __builtin_fma(w, p, 1.0 / 7.0);
+    p = __builtin_fma(w, p, 1.0 / 5.0);
+    p = __builtin_fma(w, p, 1.0 / 3.0);
+    p = __builtin_fma(w, p, 1.0);
+    return __builtin_fma(static_cast<double>(k), 0.69314718055994531, 2.0 * u * p);
 }
 // From the pair of the other columns and the label's logit.
 __device__ __forceinline__ RowScore score_row(Total p, float at_label, float scale, Scale c) {
@@ -237,7 +248,8 @@ __device__ __forceinline__ RowScore score_row(Total p, float at_label, float sca
     const float e = expf(static_cast<float>(z));
     const double total = s + e;
     if (s <= e) {  // a likely label: relative to a logarithm close to 0
-        r.logp = -log1pf(static_cast<float>(s) / e);
+        // (e is 1 here: no other column reaches the label's; or 0, in a row of nothing but -inf: NaN)
+        r.logp = !(e > 0.0f) ? __builtin_nan("") : s < 0.03125 ? -log1pf(static_cast<float>(s)) : -log_in_parts(1.0 + s);
         r.logsum = z - r.logp;
     } else {
         r.logsum = log_in_parts(total);
