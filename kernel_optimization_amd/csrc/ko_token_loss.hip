@@ -396,9 +396,9 @@ __device__ __forceinline__ RowScore label_score(const A &a, Total p, float at_la
 // One workgroup per row, the next batch of U vectors per thread in flight while this one is added up.  As in
 // policy_onchip_kernel the exponentials are taken against the label's logit, and the row's maximum is noted by the way; a label
 // so unlikely that the sum reaches 2^40, or a sum that is not a number, is summed again with a running maximum.  Bound: memory
-// (1 GiB of bf16 logits: 128256 columns 160 us, 6.7 TB/s, 50257 columns 154 us, 7.0 TB/s, 4096 columns 200 us; the
+// (1 GiB of bf16 logits: 128256 columns 160 us, 6.7 TB/s, 50257 columns 153 us, 7.0 TB/s, 4096 columns 206 us; the
 // arithmetic close behind: nine instructions' time per value; six wavefronts per SIMD, which the compiler has to be told: with five
-// 8192 columns take 216 us, with six 195).  A running maximum without loads ahead took 164 us at 32000
+// 8192 columns took 216 us, with six 195).  A running maximum without loads ahead took 164 us at 32000
 // columns and 329 at 8192.
 template <int IO, int THREADS, int U>
 __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(6))) void token_logprob_row_kernel(ScoreArgs<IO> a) {
@@ -477,8 +477,9 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(6))) vo
 }
 
 // Many short rows, of U 64 vectors at most: a wavefront takes kShortRows of them, and the arithmetic of a row's score - several times
-// that of its sum, in one lane - is done for all of them at once, a row per lane (1 GiB of bf16 rows: 512 columns 227 us, 1024
-// columns 197; a row per wavefront 471 and 281; four rows 252 and 206, sixteen 238 and, for want of registers, 257).
+// that of its sum, in one lane - is done for all of them at once, a row per lane (1 GiB of bf16 rows: 512 columns 242 us, 1024
+// columns 201; when tried, eight rows 227 and 197, a row per wavefront 471 and 281, four rows 252 and 206, sixteen 238 and, for
+// want of registers, 257).
 constexpr int kShortRows = 8;
 // Fewer rows are better off with a wavefront each: eight rows in turn take 2 to 4 us longer than one (64 rows of 512 bf16
 // columns: log-probabilities 5.7 us against 3.9, policy loss 8.2 against 4.3), which pays from here on, for the policy loss from
@@ -811,7 +812,7 @@ __global__ __launch_bounds__(THREADS) void policy_pieces_kernel(PolicyArgs<IO> a
 }
 
 // Many short rows, of 64 vectors at most, as in token_logprob_short_kernel: the rows stay in the registers of a wavefront, the losses
-// are worked out a row per lane, and each row's gradient follows (1 GiB of bf16 logits in rows of 512 columns 386 us, 5.6 TB/s; a
+// are worked out a row per lane, and each row's gradient follows (1 GiB of bf16 logits in rows of 512 columns 390 us, 5.5 TB/s; a
 // wavefront per row 545).
 template <int IO>
 __global__ __launch_bounds__(64) void policy_short_kernel(PolicyArgs<IO> a) {
