@@ -881,7 +881,7 @@ __global__ __launch_bounds__(64) void policy_short_kernel(PolicyArgs<IO> a) {
 #pragma unroll
         for (int e = 0; e < E; ++e)
             x[e] = !live ? 0.0f : E * lane + e == in_vecs ? at_label : factor * exp_scaled(x[e] - top, a.c);
-        buffer_store<IO, true>(buffer_of(dst + span.head, Io<IO>::kBytes * span.nvec), Io<IO>::kBytes * static_cast<uint32_t>(lane), x);
+        buffer_store<IO>(buffer_of(dst + span.head, Io<IO>::kBytes * span.nvec), Io<IO>::kBytes * static_cast<uint32_t>(lane), x);
         for (int j = lane; j < span.singles; j += 64) {
             constexpr int ONE = io_by_element(IO);
             const int column = single_column(span, j);
@@ -1083,7 +1083,7 @@ __global__ __launch_bounds__(THREADS) void policy_onchip_kernel(PolicyArgs<IO> a
 #pragma unroll
             for (int e = 0; e < E; ++e) x[e] = E * j + e == in_vecs ? g.label_grad : x[e];
         }
-        buffer_store<IO, true>(to, offset_of(k), x);
+        buffer_store<IO>(to, offset_of(k), x);
     }
     if constexpr (REST) {
         for (int j = static_cast<int>(threadIdx.x) + THREADS * VPT; uniform(j) < span.nvec; j += BATCH * THREADS) {
@@ -1100,7 +1100,7 @@ __global__ __launch_bounds__(THREADS) void policy_onchip_kernel(PolicyArgs<IO> a
                 for (int e = 0; e < E; ++e)
                     x[e] = E * at + e == in_vecs ? g.label_grad
                                                  : factor * __builtin_amdgcn_exp2f(__builtin_fmaf(x[e] - less, a.c.hi, -shift));
-                buffer_store<IO, true>(to, Io<IO>::kBytes * static_cast<uint32_t>(at), x);
+                buffer_store<IO>(to, Io<IO>::kBytes * static_cast<uint32_t>(at), x);
             }
         }
     }

@@ -148,10 +148,10 @@ template <int IO>
 __device__ __forceinline__ typename Io<IO>::raw buffer_load(Buffer b, uint32_t offset) {
     return __builtin_bit_cast(typename Io<IO>::raw, __builtin_amdgcn_raw_buffer_load_b128(b, offset, 0, 2 /* nt */));
 }
-// LINES: part of whole 64-byte lines, written through at once (see store_row_vec)
-template <int IO, bool LINES>
+// For vectors that make whole 64-byte lines, written through at once (see store_row_vec).
+template <int IO>
 __device__ __forceinline__ void buffer_store(Buffer b, uint32_t offset, const float (&v)[Io<IO>::E]) {
-    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(uint4v, pack<IO>(v)), b, offset, 0, LINES ? 2 | 16 /* nt sc1 */ : 2);
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(uint4v, pack<IO>(v)), b, offset, 0, 2 | 16 /* nt sc1 */);
 }
 
 // Sum over a workgroup of WAVES wavefronts of N values at once: wave all-reduces, then every thread folds the
