@@ -152,10 +152,13 @@ __device__ __forceinline__ Total block_pair(Pair p, Total *slot, Scale c) {
     return r;
 }
 
-// From a sum of 2^(c x_j - shift) to one of exp(scale (x_j - x_l)): shift is c x_l rounded, and the factor is 1 or next to it
-// unless x_l is large.
+// From a sum of 2^(c x_j - shift) to one of exp(scale (x_j - x_l)): shift is c x_l rounded, and what the rounding took is a factor
+// 2^-rest next to 1 as long as c x_l is below some millions.  Beyond that the powers summed here leave their range long before the
+// row's own do, and 1 + expm1 cancels: NaN, which callers take as they take a sum that is too large - they sum again, relative to the
+// maximum.
 __device__ __forceinline__ double to_label(double sum, float at_label, float shift, Scale c) {
     const float rest = __builtin_fmaf(at_label, c.lo, __builtin_fmaf(at_label, c.hi, -shift));
+    if (!(fabsf(rest) <= 0.5f)) return __builtin_nan("");
     return sum + sum * expm1f(-0.69314718f * rest);
 }
 

@@ -1,0 +1,71 @@
+"""Rows of logits far from 0 and rows with values that are no numbers, in every form of the token losses: each form is named by
+the sizes and arguments that lead to it."""
+import numpy as np
+import pytest
+
+import training_reference as ref
+from test_gpu_backward_rows import KINDS
+from test_gpu_token_loss import Call, check_policy, policy_case, run_policy
+
+pytestmark = pytest.mark.gpu
+
+
+class FarScores(ref.Scores):
+    """Scores whose log-probabilities stay finite where the label's probability is below the smallest 64-bit number."""
+
+    def __init__(self, logits, labels, scale=1.0, alive=None):
+        super().__init__(logits, labels, scale, alive)
+        z = self.z[self.rows, self.at]
+        with np.errstate(invalid="ignore"):
+            far = z - np.log(np.exp(self.z).sum(1))
+        self.logp = np.where(self.alive & (z < -30.0), far, self.logp)
+
+
+def far_call(ko, rows, cols, kind, scale, magnitudes, seed, pad=0, workspace=True):
+    """Every row around one of +-magnitudes: all columns the same, some steps of the type apart, or one column above the rest;
+    the label among the largest or not."""
+    call = Call(ko, rows, cols, kind, seed, pad, 0, workspace, scale)
+    rng = np.random.default_rng(seed + 1)
+    at = np.arange(rows)
+    level = (np.array(magnitudes, np.float64)[at % len(magnitudes)] * np.where(at // len(magnitudes) % 2, -1.0, 1.0))[:, None]
+    bits = {"f32": 24, "f16": 11, "bf16": 8}[kind]
+    step = 2.0 ** (np.floor(np.log2(np.abs(level))) + 1 - bits)       # the type's distance of numbers there
+    way = (at // (2 * len(magnitudes)) % 3)[:, None]
+    x = np.zeros((rows, call.ld))
+    x[:, :cols] = level + np.where(way == 1, step * rng.integers(0, 4, (rows, cols)), 0.0)
+    label = np.maximum(call.labels, 0)
+    one = (label + (at % 2)) % cols                                   # the label's column or the next one
+    x[at, one] += np.where(way[:, 0] == 2, 8 * step[:, 0], 0.0)
+    x[call.labels < 0] = np.nan
+    x[:, cols:] = np.nan
+    call.stored, values = ref.to_storage(x, kind)
+    call.values = values[:, :cols]
+    assert np.isfinite(call.values[call.labels >= 0]).all()
+    call.keep.upload(call.stored)
+    call.scores = FarScores(call.values, call.labels, scale)
+    return call
+
+
+# rows of one wavefront and of workgroups, whole and cut into pieces, eight to a wavefront, longer than the registers
+FAR_SHAPES = [(47, 19), (95, 1001), (53, 9001), (47, 33000), (47, 70001), (70, 70001), (16391, 40), (32779, 37)]
+
+
+@pytest.mark.parametrize("kind,scale,magnitudes", [("f32", 1 / 0.7, [3e5, 1e6, 3e6, 1e7, 1e8, 1e9, 1e10]),
+                                                   ("f32", 10.0, [1e5, 1e7, 4e7, 1e12]), ("f32", 0.8, [1e9, 1e20]),
+                                                   ("bf16", 1 / 0.7, [1e6, 1e9, 1e12, 1e20]), ("f16", 1e5, [5.0, 70.0, 3000.0, 6e4])])
+@pytest.mark.parametrize("rows,cols", FAR_SHAPES)
+def test_logprob_of_rows_far_from_zero(ko, rows, cols, kind, scale, magnitudes):
+    """The label's logit times scale log2(e) is rounded before it is taken off the others': far from 0 by more than their
+    differences."""
+    call = far_call(ko, rows, cols, kind, scale, magnitudes, 4000 + cols)
+    s = call.scores
+    # each column's exponential may be flushed to 0 below 2^-126; where the label is all but certain logp is minus their sum
+    off = s.logp_off + cols * 2.0 ** -126
+    logp, stats = call.logprob()
+    ref.assert_within(logp, s.logp, off, "logp")
+    np.testing.assert_array_equal(stats[:, 0], s.top.astype(np.float32))
+    ref.assert_within(stats[:, 1], s.logsum, s.logsum_off + cols * 2.0 ** -126, "log sum")
+    case = policy_case(call, cols, False, False)
+    for pad, gradient in ((0, True), (1, True), (0, False)):
+        got = run_policy(call, case, pad, gradient=gradient, kl_coef=0.0)
+        ref.assert_within(got["logp"], s.logp, off, "logp of the policy loss")
