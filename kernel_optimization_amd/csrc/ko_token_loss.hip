@@ -1052,10 +1052,14 @@ __global__ __launch_bounds__(THREADS) void policy_onchip_kernel(PolicyArgs<IO> a
     __syncthreads();
     const RowGradient g = uniform_gradient(shared);
     float reference = g.top, less = 0.0f;
-    if (g.top != at_label || !(fabsf(shift) < 1e30f)) {
-        // the reference is the maximum; one whose multiple by c might overflow is taken off the values
+    // shift is rounded, to half a step of itself: below 2^24 that makes both powers of the product below differ from what they stand
+    // for by a factor of 2 at most; beyond, one may be infinite and the other 0
+    constexpr float kMostShift = 0x1p24f;
+    if (g.top != at_label || !(fabsf(shift) < kMostShift)) {
+        // the reference is the maximum; one that far from 0 is taken off the values (what is close enough to it to count is
+        // so exactly, in the storage type too: two numbers of a type within a factor of two differ by one of its numbers)
         shift = g.top * a.c.hi;
-        if (!(fabsf(shift) < 1e30f)) {
+        if (!(fabsf(shift) < kMostShift)) {
 #pragma unroll
             for (int k = 0; k < VPT; ++k) {
                 asm volatile("" : "+v"(r[k]));

@@ -69,3 +69,49 @@ def test_logprob_of_rows_far_from_zero(ko, rows, cols, kind, scale, magnitudes):
     for pad, gradient in ((0, True), (1, True), (0, False)):
         got = run_policy(call, case, pad, gradient=gradient, kl_coef=0.0)
         ref.assert_within(got["logp"], s.logp, off, "logp of the policy loss")
+
+
+# (beyond 1e30 the differences from the row's maximum were taken first, below nothing is lost)
+@pytest.mark.parametrize("kind,scale,magnitudes", [("f32", 1.0, [1e6, 1e7, 1e8, 1e9, 4e9, 1e10, 1e12, 1e20, 1e32]),
+                                                   ("f32", 1 / 0.7, [4e9, 1e10, 3e29, 1e30]), ("f32", 1e-10, [1e17, 1e20, 1e24]),
+                                                   ("bf16", 1.0, [1e8, 1e10, 1e20, 1e35]), ("bf16", 1 / 0.7, [4e9, 1e12]),
+                                                   ("f16", 1e6, [100.0, 4e3, 6e4]), ("f16", 1e20, [1.0, 6e4])])
+@pytest.mark.parametrize("rows,cols", FAR_SHAPES)
+def test_policy_gradient_of_rows_far_from_zero(ko, rows, cols, kind, scale, magnitudes):
+    """With ratio 1 and no KL term the gradient is -advantage scale (onehot - softmax): with a large scale beyond binary16's
+    numbers, then it is infinite."""
+    call = far_call(ko, rows, cols, kind, scale, magnitudes, 4100 + cols)
+    case = policy_case(call, cols, False, False, False)
+    first = {}
+    for pad in (1, 0):
+        got = run_policy(call, case, pad, kl_coef=0.0)
+        first["dlogits"] = got["dlogits"]
+        d = ref.to_float(np.ascontiguousarray(got.pop("dlogits")), kind)
+        check_policy(call, got, case, 0.0)
+        alive = call.labels >= 0
+        want, off = call.scores.gradient(np.where(alive, -case["advantage"].astype(np.float64), 0.0), 0.0, call.scores.s_off)
+        off = off + ref.rounded(kind, want) * (1 + 1e-6)
+        # (65520 rounds to infinity)
+        large, beyond = (np.abs(want) - off >= 65520, np.abs(want) + off >= 65520) if kind == "f16" else (want != want, want != want)
+        assert (d[large] == np.copysign(np.inf, want[large])).all()
+        either = beyond & ~large & np.isinf(d)
+        assert (np.sign(d[either]) == np.sign(want[either])).all()
+        ref.assert_within(d[~large & ~either], want[~large & ~either], off[~large & ~either], "dlogits")
+        assert not d[~alive].any()
+    got = run_policy(call, case, 0, in_place=True, kl_coef=0.0)
+    np.testing.assert_array_equal(got["dlogits"], first["dlogits"])
+
+
+def test_a_masked_row_with_a_label(ko):
+    """All columns at -1e10, by every length that a workgroup's registers are cut for: the gradient is that of a uniform row."""
+    for cols in (33, 300, 700, 2000, 4100, 8200, 16500, 33000, 65536, 66000):
+        x = np.full((70, cols), -1e10, np.float32)
+        labels = (np.arange(70) * 37 % cols).astype(np.int32)
+        bufs = [ko.DeviceBuffer.from_numpy(a) for a in (x, labels, np.ones(70, np.float32))]
+        loss, d = ko.DeviceBuffer(4 * 70), ko.DeviceBuffer(x.nbytes)
+        ko.policy_loss(bufs[0], bufs[1], bufs[2], loss, 70, cols, dlogits=d)
+        ko.synchronize()
+        want = np.full((70, cols), 1.0 / cols)
+        want[np.arange(70), labels] -= 1.0
+        # the sum of ones is exact to the last step (whole numbers below 2^24), then a division and a product
+        np.testing.assert_allclose(d.download(np.float32, x.shape), want, rtol=8 * ref.U)
