@@ -713,7 +713,8 @@ struct PolicyResult {
 __device__ __forceinline__ PolicyResult policy_row(const PolicyOptions &o, const PolicyRow &in, Total p) {
     const RowScore r = in.label < o.cols ? score_row(p, in.at_label, o.scale, o.c) : nan_score();
     const double adv = in.advantage, w = in.weight;
-    const double ratio = o.old ? expf(static_cast<float>(r.logp - static_cast<double>(in.old_logp))) : 1.0 + 0.0 * r.logp;
+    // (without an old logp: 1, for a label at -inf too, and NaN where logp is)
+    const double ratio = o.old ? expf(static_cast<float>(r.logp - static_cast<double>(in.old_logp))) : r.logp == r.logp ? 1.0 : r.logp;
     const double low = 1.0 - o.clip_low, high = 1.0 + o.clip_high;
     double kept = ratio, slope = -adv * ratio;
     if (adv > 0.0 ? ratio > high : ratio < low) {

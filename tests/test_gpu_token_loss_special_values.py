@@ -115,3 +115,37 @@ def test_a_masked_row_with_a_label(ko):
         want[np.arange(70), labels] -= 1.0
         # the sum of ones is exact to the last step (whole numbers below 2^24), then a division and a product
         np.testing.assert_allclose(d.download(np.float32, x.shape), want, rtol=8 * ref.U)
+
+
+# the policy loss's forms: (rows, columns, padding of the gradient's rows, with a gradient, with a workspace)
+POLICY_FORMS = [(41, 1001, 0, True, True), (41, 9001, 0, True, True), (41, 1001, 1, True, True), (41, 9001, 0, False, True),
+                (7, 70001, 0, True, True), (7, 70001, 0, False, True), (7, 70001, 0, True, False), (70, 70001, 0, True, True),
+                (32779, 37, 0, True, True), (5, 3, 0, True, True)]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows,cols,pad,gradient,workspace", POLICY_FORMS)
+def test_an_impossible_label_of_the_policy_that_trains(ko, rows, cols, pad, gradient, workspace, kind):
+    """Without old log-probabilities the ratio is 1, also for a label at -inf: the loss is -advantage, and the gradient takes
+    weight from the other columns."""
+    call = Call(ko, rows, cols, kind, 4300 + cols, 0, 0, workspace)
+    live = np.flatnonzero(call.labels >= 0)
+    lost = live[::3]
+    x = np.where((call.labels >= 0)[:, None], call.values, np.nan).astype(np.float32)
+    x[lost, call.labels[lost]] = -np.inf
+    call.stored, call.values = ref.to_storage(x, kind)
+    call.keep.upload(call.stored)
+    with np.errstate(divide="ignore"):
+        call.scores = ref.Scores(call.values, call.labels)
+    case = policy_case(call, 14, False, False)
+    got = run_policy(call, case, pad, gradient=gradient, kl_coef=0.0)
+    assert (got["logp"][lost] == -np.inf).all()
+    call.scores.logp[lost] = 0.0        # (the ratio does not depend on it)
+    rest = np.setdiff1d(np.arange(rows), lost)
+    want = ref.policy(call.scores, np.where(call.labels >= 0, case["advantage"], 1.0), None, None,
+                      np.where(call.labels >= 0, case["weight"], 1.0), 0.2, 0.28, 0.0)
+    for name in ("loss", "loss_sum"):
+        ref.assert_within(got[name], *want[name], name)
+    ref.assert_within(got["logp"][rest], want["logp"][0][rest], want["logp"][1][rest], "logp")
+    if gradient:
+        call.check_gradient(got["dlogits"], want["dlogits"])
