@@ -721,7 +721,7 @@ __device__ __forceinline__ PolicyResult policy_row(const PolicyOptions &o, const
         kept = adv > 0.0 ? high : low;
         slope = 0.0;
     }
-    if (adv == 0.0) slope = kept = 0.0;  // (no surrogate, however large the ratio)
+    if (adv == 0.0 && ratio == ratio) slope = kept = 0.0;  // (no surrogate, however large the ratio; a broken row stays NaN)
     double total = -adv * kept;
     float kl = 0.0f;
     if (o.ref) {

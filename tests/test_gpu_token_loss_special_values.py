@@ -149,3 +149,37 @@ def test_an_impossible_label_of_the_policy_that_trains(ko, rows, cols, pad, grad
     ref.assert_within(got["logp"][rest], want["logp"][0][rest], want["logp"][1][rest], "logp")
     if gradient:
         call.check_gradient(got["dlogits"], want["dlogits"])
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows,cols,pad,gradient,workspace", POLICY_FORMS)
+def test_no_advantage_hides_no_broken_row(ko, rows, cols, pad, gradient, workspace, kind):
+    """A NaN or +inf logit, or a label beyond the vocabulary, makes a row's outputs and gradient NaN also where its advantage is 0
+    and no KL term counts; a sound row without advantage has loss and gradient 0."""
+    call = Call(ko, rows, cols, kind, 4200 + cols, 0, 0, workspace)
+    alive = call.labels >= 0
+    case = policy_case(call, 13)
+    case["advantage"][alive] = 0.0
+    x = np.where(alive[:, None], call.values, np.nan).astype(np.float32)
+    bad = np.flatnonzero(alive)[:4]
+    assert len(bad) >= 3
+    call.labels[bad[0]] = cols
+    x[bad[1], cols // 2] = np.nan
+    x[bad[2], (call.labels[bad[2]] + 1) % cols] = np.inf
+    if len(bad) > 3:
+        x[bad[3], call.labels[bad[3]]] = np.inf
+    for name in ("old", "ref"):
+        case[name][bad] = -1.0
+    call.keep.upload(ref.to_storage(x, kind)[0])
+    call.d_labels.upload(call.labels)
+    sound = np.setdiff1d(np.arange(rows), bad)
+    for old, reference in ((True, True), (True, False), (False, False)):
+        given = dict(case, old=case["old"] if old else None, ref=case["ref"] if reference else None)
+        got = run_policy(call, given, pad, gradient=gradient, kl_coef=0.0)
+        assert np.isnan(got["logp"][bad]).all() and np.isnan(got["loss"][bad]).all() and np.isnan(got["loss_sum"]).all()
+        assert not got["loss"][sound].any() and np.isfinite(got["logp"][sound]).all()
+        if reference:
+            assert np.isnan(got["kl"][bad]).all()
+        if gradient:
+            d = ref.to_float(np.ascontiguousarray(got["dlogits"]), kind)
+            assert np.isnan(d[bad]).all() and not d[sound].any()
