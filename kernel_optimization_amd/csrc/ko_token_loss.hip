@@ -1208,7 +1208,9 @@ __device__ __forceinline__ float pair_result(const PreferenceArgs &a, int64_t pa
     const double slope = a.eps - 1.0 / (1.0 + exp(h));
     if (write) {
         const double both = log1p(exp(-fabs(h)));
-        double l = (1.0 - a.eps) * (both + (h < 0.0 ? -h : 0.0));
+        // (a side without a share adds nothing, however far apart the rewards)
+        double l = 0.0;
+        if (a.eps != 1.0f) l = (1.0 - a.eps) * (both + (h < 0.0 ? -h : 0.0));
         if (a.eps != 0.0f) l += a.eps * (both + (h > 0.0 ? h : 0.0));
         loss = static_cast<float>(l);
         a.pair_loss[pair] = loss;

@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 import training_reference as ref
-from test_gpu_backward_rows import KINDS
+from test_gpu_backward_rows import KINDS, Out
 from test_gpu_token_loss import Call, check_policy, policy_case, run_policy
 
 pytestmark = pytest.mark.gpu
@@ -183,3 +183,26 @@ def test_no_advantage_hides_no_broken_row(ko, rows, cols, pad, gradient, workspa
         if gradient:
             d = ref.to_float(np.ascontiguousarray(got["dlogits"]), kind)
             assert np.isnan(d[bad]).all() and not d[sound].any()
+
+
+@pytest.mark.parametrize("pairs", [1, 4, 7, 40])
+def test_preference_loss_of_certain_pairs(ko, pairs):
+    """A chosen or rejected token of probability 0 puts the rewards infinitely far apart: a side whose share of the loss is 0
+    adds nothing."""
+    tokens = 2 * pairs
+    offsets = np.arange(tokens + 1, dtype=np.int32)
+    rf = np.full(tokens, -1.0, np.float32)
+    bufs = [ko.DeviceBuffer.from_numpy(a) for a in (rf, offsets)]
+    for side, sign in ((0, -1.0), (1, 1.0)):        # the chosen or the rejected token is the impossible one: margin -inf or inf
+        logp = np.full(tokens, -1.0, np.float32)
+        logp[side::2] = -np.inf
+        d_logp = ko.DeviceBuffer.from_numpy(logp)
+        for eps, want in ((0.0, 0.0 if sign > 0 else np.inf), (1.0, np.inf if sign > 0 else 0.0), (0.5, np.inf)):
+            loss, dlogp, total = Out(ko, 4 * pairs), Out(ko, 4 * tokens), Out(ko, 4)
+            ko.preference_loss(d_logp, bufs[0], bufs[1], pairs, tokens, loss.ptr, beta=0.5, label_smoothing=eps, pair_weight=1.0,
+                               dlogp=dlogp.ptr, loss_sum=total.ptr)
+            ko.synchronize()
+            assert (loss.get(np.float32, (pairs,)) == want).all(), (sign, eps)
+            assert total.get(np.float32, (1,))[0] == want * pairs if want else total.get(np.float32, (1,))[0] == 0.0
+            slope = 0.5 * (eps - (1.0 if sign < 0 else 0.0))       # d loss / d margin, times beta
+            np.testing.assert_array_equal(dlogp.get(np.float32, (tokens,)), np.tile([slope, -slope], pairs))
