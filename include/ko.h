@@ -247,7 +247,9 @@ int ko_policy_loss_16(const void *logits, int64_t ld, const int32_t *labels, con
  *      pair_loss = -(1 - label_smoothing) log sigmoid(h) - label_smoothing log sigmoid(-h),
  * loss_sum = pair_weight sum pair_loss, dlogp = d loss_sum / d logp.  labels (NULL: every token counts): tokens with a
  * negative label count for nothing, whatever logp and ref_logp hold there, and get dlogp 0.  rewards [2 pairs], dlogp,
- * loss_sum: NULL if not wanted.  dlogp of tokens that belong to no sequence is left as it was. */
+ * loss_sum: NULL if not wanted.  dlogp of tokens that belong to no sequence is left as it was.  Where offsets go backwards from
+ * one pair to the next, so that pairs share tokens, each pair's rewards and loss are those of its own offsets, and a pair writes
+ * dlogp only from the largest of all offsets up to its own first one on: no token is written by two pairs. */
 int ko_preference_loss_f32(const float *logp, const float *ref_logp, const int32_t *labels, const int32_t *offsets, int64_t pairs,
                            int64_t tokens, float beta, float label_smoothing, float pair_weight, float *pair_loss,
                            float *rewards, float *dlogp, float *loss_sum, ko_stream_t stream);

@@ -206,3 +206,56 @@ def test_preference_loss_of_certain_pairs(ko, pairs):
             assert total.get(np.float32, (1,))[0] == want * pairs if want else total.get(np.float32, (1,))[0] == 0.0
             slope = 0.5 * (eps - (1.0 if sign < 0 else 0.0))       # d loss / d margin, times beta
             np.testing.assert_array_equal(dlogp.get(np.float32, (tokens,)), np.tile([slope, -slope], pairs))
+
+
+def _random_offsets(pairs, back, seed):
+    """Offsets that run forwards on the whole and backwards by up to `back` at every turn, some of them far out."""
+    rng = np.random.default_rng(seed)
+    offsets = 7 * np.arange(2 * pairs + 1) + rng.integers(-back, back + 1, 2 * pairs + 1)
+    wild = rng.random(2 * pairs + 1) < 0.5 / (pairs + 1)
+    offsets[wild] = rng.choice([-2 ** 31, -5, 2 ** 31 - 1], int(wild.sum()))
+    if pairs > 2:
+        offsets[[2, 4]] = offsets[[4, 2]]
+    return offsets.astype(np.int32)
+
+
+@pytest.mark.parametrize("labelled", [True, False])
+@pytest.mark.parametrize("pairs,back", [(1, 40), (2, 9), (3, 30), (7, 0), (16, 12), (17, 12), (300, 25), (1024, 9), (1025, 9), (9001, 100),
+                                        (30000, 0)])
+def test_pairs_that_share_tokens(ko, pairs, back, labelled):
+    """Offsets that go backwards between pairs: rewards and losses are those of a pair's own offsets; a pair writes the gradient
+    from the largest offset before it on, so that no token is written twice, and the same bits come from call to call."""
+    tokens = 14 * pairs - 3
+    offsets = _random_offsets(pairs, back, pairs)
+    rng = np.random.default_rng(pairs + 1)
+    logp, rf = rng.normal(-2, 1, tokens).astype(np.float32), rng.normal(-2, 1, tokens).astype(np.float32)
+    labels = np.where(rng.random(tokens) < 0.2, -1, 7).astype(np.int32) if labelled else None
+    want = ref.preference(logp, rf, offsets, labels, 0.3, 0.1)
+    slope, touched = np.zeros(tokens), np.zeros(tokens, bool)
+    most = np.clip(np.maximum.accumulate(offsets.astype(np.int64)), 0, tokens)
+    share = float(np.float32(0.3)) * float(np.float32(1.0 / pairs))
+    for p in range(pairs):
+        at = np.clip(np.maximum.accumulate(np.maximum(offsets[2 * p:2 * p + 3].astype(np.int64), 0)), 0, tokens)
+        margin = want["rewards"][0][2 * p] - want["rewards"][0][2 * p + 1]
+        up = (float(np.float32(0.1)) - 1.0 / (1.0 + np.exp(margin))) * share
+        begin = most[2 * p]
+        slope[begin:max(begin, at[1])], slope[max(begin, at[1]):max(begin, at[2])] = up, -up
+        touched[begin:max(begin, at[2])] = True
+    if labels is not None:
+        slope[labels < 0] = 0.0
+    d = [ko.DeviceBuffer.from_numpy(a) for a in (logp, rf, offsets)]
+    d_labels = None if labels is None else ko.DeviceBuffer.from_numpy(labels)
+    before = None
+    for _ in range(3):
+        outs = dict(pair_loss=Out(ko, 4 * pairs), rewards=Out(ko, 8 * pairs), dlogp=Out(ko, 4 * tokens), loss_sum=Out(ko, 4))
+        ko.preference_loss(d[0], d[1], d[2], pairs, tokens, outs["pair_loss"].ptr, labels=d_labels, beta=0.3, label_smoothing=0.1,
+                           rewards=outs["rewards"].ptr, dlogp=outs["dlogp"].ptr, loss_sum=outs["loss_sum"].ptr)
+        ko.synchronize()
+        for name, n in (("pair_loss", pairs), ("rewards", 2 * pairs), ("loss_sum", 1)):
+            ref.assert_within(outs[name].get(np.float32, (n,)), *want[name], name)
+        raw = outs["dlogp"].get(np.uint32, (tokens,))
+        assert (raw[~touched] == 0xFFFFFFFF).all()
+        ref.assert_within(raw.view(np.float32)[touched], slope[touched], (2 * ref.U * np.abs(slope) + 1e-13)[touched], "dlogp")
+        if before is not None:
+            np.testing.assert_array_equal(raw, before)
+        before = raw
