@@ -38,46 +38,62 @@ struct Args {
 };
 
 // dgamma and dbeta of a strip of COLUMNS columns alone, by a workgroup: THREADS / COLUMNS slices of the rows from `first` on, every
-// `step`-th row, side by side, then folded in order.  The sums come back in the first COLUMNS threads.
-template <int IO, int THREADS, int COLUMNS>
+// `step`-th row, side by side, then folded in order.  The sums come back in the first COLUMNS threads.  Sum: what eight rows'
+// sums in 32 bits are added up in; without a workspace a thread goes through a quarter of all rows, and 196608 additions in 32 bits
+// of terms of one sign were off by 190 half steps.
+template <int IO, int THREADS, int COLUMNS, class Sum>
 __device__ __forceinline__ void column_strip(const Args<IO> &a, int strip, int64_t split, int64_t splits, float &sum_g, float &sum_b) {
     constexpr int SLICES = THREADS / COLUMNS;
     constexpr int UNROLL = 8;
-    __shared__ float sums[2][SLICES][COLUMNS + 1];
+    __shared__ Sum sums[2][SLICES][COLUMNS + 1];
     const int lane = threadIdx.x % COLUMNS;
     const int slice = threadIdx.x / COLUMNS;
     const int c = strip * COLUMNS + lane;
-    float sg = 0.0f, sb = 0.0f;
+    Sum sg = 0, sb = 0;
     if (c < a.cols) {
         const int64_t step = SLICES * splits;
         for (int64_t row0 = SLICES * split + slice; row0 < a.rows; row0 += step * UNROLL) {
+            // (beyond the last row: the last one, counted as nothing; loads under conditions, or next to their use, wait one by one)
+            typename Io<IO>::elem dy[UNROLL], x[UNROLL];
+            float mean[UNROLL], rstd[UNROLL];
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u) {
+                const int64_t row = row0 + u * step < a.rows ? row0 + u * step : a.rows - 1;
+                dy[u] = a.dy[row * a.cols + c];
+                x[u] = a.x[row * a.cols + c];
+                mean[u] = a.mean[row];
+                rstd[u] = a.rstd[row];
+            }
+            asm volatile("" ::: "memory");
             float d[UNROLL], xh[UNROLL];
 #pragma unroll
             for (int u = 0; u < UNROLL; ++u) {
-                const int64_t row = row0 + u * step;
-                d[u] = xh[u] = 0.0f;
-                if (row < a.rows) {
-                    d[u] = Io<IO>::scalar(a.dy + row * a.cols + c);
-                    xh[u] = (Io<IO>::scalar(a.x + row * a.cols + c) - a.mean[row]) * a.rstd[row];
-                }
+                const bool here = row0 + u * step < a.rows;
+                d[u] = here ? Io<IO>::scalar(&dy[u]) : 0.0f;
+                xh[u] = here ? (Io<IO>::scalar(&x[u]) - mean[u]) * rstd[u] : 0.0f;
             }
+            float g = 0.0f, b = 0.0f;
 #pragma unroll
             for (int u = 0; u < UNROLL; ++u) {
-                sg = __builtin_fmaf(d[u], xh[u], sg);
-                sb += d[u];
+                g = __builtin_fmaf(d[u], xh[u], g);
+                b += d[u];
             }
+            sg += g;
+            sb += b;
         }
     }
     sums[0][slice][lane] = sg;
     sums[1][slice][lane] = sb;
     __syncthreads();
-    sum_g = sum_b = 0.0f;
     if (threadIdx.x >= COLUMNS) return;
+    sg = sb = 0;
 #pragma unroll 8
     for (int i = 0; i < SLICES; ++i) {
-        sum_g += sums[0][i][lane];
-        sum_b += sums[1][i][lane];
+        sg += sums[0][i][lane];
+        sb += sums[1][i][lane];
     }
+    sum_g = static_cast<float>(sg);
+    sum_b = static_cast<float>(sb);
 }
 
 // A strip over all rows, to the results: the few-rows form.
@@ -85,7 +101,7 @@ constexpr int kStripColumns = 16;
 template <int IO, int THREADS>
 __device__ __forceinline__ void whole_strip(const Args<IO> &a, int strip) {
     float sum_g, sum_b;
-    column_strip<IO, THREADS, kStripColumns>(a, strip, 0, 1, sum_g, sum_b);
+    column_strip<IO, THREADS, kStripColumns, float>(a, strip, 0, 1, sum_g, sum_b);  // (few rows)
     const int c = strip * kStripColumns + threadIdx.x;
     if (threadIdx.x < kStripColumns && c < a.cols) {
         if (a.dgamma) a.dgamma[c] = sum_g;
@@ -435,7 +451,7 @@ __global__ __launch_bounds__(THREADS) void layernorm_backward_reread_kernel(Args
 template <int IO>
 __global__ __launch_bounds__(256) void layernorm_backward_columns_kernel(Args<IO> a) {
     float sg, sb;
-    column_strip<IO, 256, 64>(a, blockIdx.x, blockIdx.y, gridDim.y, sg, sb);
+    column_strip<IO, 256, 64, double>(a, blockIdx.x, blockIdx.y, gridDim.y, sg, sb);
     const int c = static_cast<int>(blockIdx.x) * 64 + threadIdx.x;
     if (threadIdx.x >= 64 || c >= a.cols) return;
     if (gridDim.y == 1) {
