@@ -3,6 +3,7 @@
 
 #include <type_traits>
 
+#include "ko_internal.h"
 #include "wave64.h"
 
 namespace ko {
@@ -180,9 +181,10 @@ __device__ __forceinline__ void block_sum(float (&v)[N], float (*slot)[N]) {
 constexpr int64_t kMaxColumns = 1 << 28;
 
 // One workgroup per row (or group of rows), as far as a grid goes: its threads number less than 2^32, and the kernels walk on
-// from there.
+// from there.  (The knob is for tests of the walk, which otherwise begins with millions of rows.)
 inline dim3 row_grid(int64_t groups, int threads) {
-    const int64_t most = 0xffffffffll / threads;
+    const int knob = tuning(knob_rows_most_workgroups);
+    const int64_t most = knob > 0 ? knob : 0xffffffffll / threads;
     return dim3(static_cast<unsigned>(groups < most ? groups : most));
 }
 

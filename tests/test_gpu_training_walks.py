@@ -1,0 +1,98 @@
+"""Forms of the training-side operators that only many rows reach: workgroups that walk over rows, here on grids cut to three of
+them, and eight rows of two vectors per lane to a wavefront."""
+import numpy as np
+import pytest
+
+import test_gpu_token_loss as token_loss
+import training_reference as ref
+from kernel_optimization_amd import inputs
+from test_gpu_backward_rows import KINDS, _softmax, check_layernorm_backward, check_softmax_backward, layernorm_case
+from test_gpu_token_loss import Call, policy_case, run_policy
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture
+def three_workgroups(ko):
+    ko.set_tuning("rows.most_workgroups", 3)
+    yield
+    ko.set_tuning("rows.most_workgroups", 0)
+
+
+# every number of threads per row of the log-probabilities and of the policy loss without a gradient, one row at a time and eight
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows,cols", [(61, 257), (61, 1001), (50, 2049), (50, 4100), (40, 8200), (50, 12000), (40, 33001), (40, 70001),
+                                       (16400, 130), (16391, 300)])
+def test_walks_of_the_token_losses(ko, three_workgroups, rows, cols, kind):
+    """Rows without a label, with one beyond the vocabulary and with one far below the others, which is summed twice, between
+    ordinary ones, so that what one row left in LDS is there when another comes."""
+    call = Call(ko, rows, cols, kind, 5000 + cols, 3, 0, False)
+    live = np.flatnonzero(call.labels >= 0)
+    x = np.where((call.labels >= 0)[:, None], call.values, np.nan).astype(np.float32)
+    far = live[::3]
+    x[far, call.labels[far]] -= 70.0
+    stored = np.full((rows, call.ld), np.nan, np.float32)
+    stored[:, :cols] = x
+    call.stored, values = ref.to_storage(stored, kind)
+    call.values = values[:, :cols]
+    call.keep.upload(call.stored)
+    alive = call.labels >= 0
+    beyond = np.zeros(rows, bool)
+    beyond[live[1::4]] = True
+    call.scores = ref.Scores(call.values, call.labels, 1.0, ~beyond)
+    call.labels[beyond] = cols + np.arange(beyond.sum())
+    call.d_labels.upload(call.labels)
+    sound, dead = alive & ~beyond, ~alive
+    logp, stats = call.logprob()
+    s = call.scores
+    assert np.isnan(logp[beyond]).all() and np.isnan(stats[beyond]).all() and not logp[dead].any()
+    ref.assert_within(logp[sound], s.logp[sound], s.logp_off[sound], "logp")
+    np.testing.assert_array_equal(stats[sound, 0], s.top[sound].astype(np.float32))
+    ref.assert_within(stats[sound, 1], s.logsum[sound], s.logsum_off[sound], "log sum")
+    case = policy_case(call, cols)
+    for name in ("old", "ref", "weight"):
+        case[name][beyond] = 0.5
+    clean = {k: np.where(sound, v, 1.0).astype(np.float64) for k, v in case.items()}
+    want = ref.policy(s, clean["advantage"], clean["old"], clean["ref"], clean["weight"], 0.2, 0.28, 0.05)
+    for gradient, pad in ((False, 3), (True, 4)):       # (with rows that lie differently: a second read, by elements)
+        got = run_policy(call, case, pad, gradient=gradient)
+        assert np.isnan(got["loss_sum"]).all()
+        for name in ("logp", "kl", "loss"):
+            assert np.isnan(got[name][beyond]).all() and not got[name][dead].any()
+            ref.assert_within(got[name][sound], want[name][0][sound], want[name][1][sound], name)
+        if gradient:
+            d = ref.to_float(np.ascontiguousarray(got["dlogits"]), kind)
+            assert np.isnan(d[beyond]).all() and not d[dead].any()
+            value, off = want["dlogits"]
+            ref.assert_within(d[sound], value[sound], (off + ref.rounded(kind, value) * (1 + 1e-6))[sound], "dlogits")
+
+
+@pytest.mark.parametrize("lens", [[1] * 600, [40, 17, 3, 200, 1, 1] * 20, [5000, 2600, 1, 4097], [3, 1] * 1500])
+def test_walks_of_the_preference_loss(ko, three_workgroups, lens):
+    token_loss.test_preference_loss(ko, lens, 0.1)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows,cols,rps", [(301, 37, 3), (301, 512, 4), (70, 1001, 1), (31, 3000, 2), (25, 8200, 3), (17, 20000, 1),
+                                           (11, 70001, 1), (70, 66000, 1)])
+def test_walks_of_the_softmax_gradient(ko, three_workgroups, rows, cols, rps, kind):
+    x = inputs.normal_f32((rows, cols), 5100 + cols, 0.0, 4.0).astype(np.float64)
+    dy, _ = ref.to_storage(inputs.normal_f32((rows, cols), 5101 + cols), kind)
+    y, _ = ref.to_storage(_softmax(x), kind)
+    check_softmax_backward(ko, y, dy, kind, workspace=False)
+    lens = (np.arange((rows + rps - 1) // rps) * 977 % (cols + 3) - 1).astype(np.int32)
+    keep = ref.keep_columns(rows, cols, lens, rps)
+    y, _ = ref.to_storage(_softmax(np.where(keep, x, -10000.0)), kind)
+    check_softmax_backward(ko, y, dy, kind, lens, rps, workspace=False)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows,cols", [(300, 3), (20, 17000), (15, 40001)])
+def test_walks_of_the_layernorm_gradient(ko, three_workgroups, rows, cols, kind):
+    check_layernorm_backward(ko, layernorm_case(rows, cols, kind, 5200 + cols), kind)
+
+
+@pytest.mark.parametrize("kind,cols", [("f16", 520), ("f16", 703), ("bf16", 777), ("bf16", 1024), ("f16", 1031), ("f32", 300), ("f32", 404),
+                                       ("f32", 511)])
+def test_many_rows_of_two_vectors_per_lane(ko, kind, cols):
+    token_loss.test_token_logprob_and_its_gradient(ko, 16391, cols, kind)
