@@ -259,3 +259,33 @@ def test_pairs_that_share_tokens(ko, pairs, back, labelled):
         if before is not None:
             np.testing.assert_array_equal(raw, before)
         before = raw
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows,cols,pad", [(41, 90, 0), (41, 1001, 0), (41, 1001, 1), (30, 9001, 0), (7, 70001, 0), (16391, 40, 0),
+                                           (16391, 600, 0)])
+def test_broken_rows_of_every_type(ko, rows, cols, pad, kind):
+    """NaN and infinite logits and labels beyond the vocabulary stay in their own rows, in log-probabilities, statistics and
+    gradients; the gradient takes the statistics that the forward call left."""
+    call = Call(ko, rows, cols, kind, 4400 + cols, 0, 4)
+    live = np.flatnonzero(call.labels >= 0)
+    bad = live[:4]
+    x = np.where((call.labels >= 0)[:, None], call.values, np.nan).astype(np.float32)
+    x[bad[0], cols // 2] = np.nan
+    x[bad[1], (call.labels[bad[1]] + 1) % cols] = np.inf
+    x[bad[2], call.labels[bad[2]]] = np.nan
+    call.labels[bad[3]] = 2 ** 31 - 1
+    call.keep.upload(np.concatenate([np.zeros(4, np.uint8), ref.to_storage(x, kind)[0].reshape(-1).view(np.uint8)]))
+    call.d_labels.upload(call.labels)
+    sound = np.setdiff1d(np.arange(rows), bad)
+    logp, stats = call.logprob()
+    s = call.scores
+    assert np.isnan(logp[bad]).all() and np.isnan(stats[bad, 1]).all()
+    ref.assert_within(logp[sound], s.logp[sound], s.logp_off[sound], "logp")
+    dlogp = np.linspace(-1.0, 1.0, rows).astype(np.float32) + np.float32(0.01)
+    s.top, s.logsum = stats[:, 0].astype(np.float64), stats[:, 1].astype(np.float64)
+    got = ref.to_float(np.ascontiguousarray(call.backward(dlogp, pad)), kind)
+    assert np.isnan(got[bad]).all()
+    value, off = s.gradient(dlogp.astype(np.float64), 0.0, s.logsum_off + 3 * ref.U * np.abs(s.logsum) + 2 * ref.U)
+    off = off + ref.rounded(kind, value) * (1 + 1e-6)
+    ref.assert_within(got[sound], value[sound], off[sound], "dlogits")
