@@ -30,3 +30,54 @@ def test_column_sums_over_many_rows(ko, rows, cols, kind):
         # xh carries two roundings, its product with dy one
         ref.assert_within(dgamma, want_g, (depth + 3) * U * want_g, "dgamma, workspace %s" % workspace)
         ref.assert_within(dbeta, want_b, depth * U * want_b, "dbeta, workspace %s" % workspace)
+
+
+# scale log2(e) as one 32-bit number is off by 1e-9 of itself for scale 1; for these by at least 0.9 of half a step
+def _awkward_scale(near):
+    log2e = 1.4426950408889634
+    for scale in np.float32(near) + np.arange(2000, dtype=np.float32) * np.spacing(np.float32(near)):
+        c = float(scale) * log2e
+        step = float(np.spacing(np.float32(c)))
+        if 0.45 * step <= abs(float(np.float32(c)) - c) and c < 1.1 * 2.0 ** np.floor(np.log2(c)):
+            return float(scale)
+    raise AssertionError("no such scale")
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("cols", [30522, 128256])
+def test_log_probabilities_are_differences_of_more_than_32_bits(ko, cols, kind):
+    """A KL term sees the log-probability before it is rounded: kl(d) with d = reference - logp near 0.4 moves by 0.49 of logp's
+    error.  At labels of logp about -24 a logarithm in 32 bits is off by up to half a step of numbers from 16 to 32, 9.5e-7, 5.5e-7 in
+    root mean square, and scale log2(e) in one 32-bit number by 5.7e-8 of some 14 (the distance from the label to where the other
+    columns' weight lies), 8e-7 and the same way in every row: 2.7e-7 and 4e-7 of kl.  What the kernels may be off by, of kl: d's own
+    rounding 1.5e-8 at most, three roundings of kl around 0.09 2e-8 at most, a bias of half a step in the exponentials 1.5e-8;
+    their arguments' rounding (9.5e-7 as a part of one column's weight, spread over ten thousand columns) and the sums' (32 bits in
+    a few hundred threads) below 1e-8.  Root mean square of them together: below 5e-8."""
+    rows = 48
+    rng = np.random.default_rng(cols)
+    scale = _awkward_scale(0.7)
+    x = rng.normal(0.0, 1.2, (rows, cols)).astype(np.float32)
+    labels = rng.integers(0, cols, rows).astype(np.int32)
+    at = np.arange(rows)
+    x[at, labels] = rng.uniform(-20.0, -18.0, rows)
+    stored, values = ref.to_storage(x, kind)
+    z = values * scale
+    top = z.max(1)
+    logp = z[at, labels] - top - np.log(np.exp(z - top[:, None]).sum(1))
+    assert -30 < logp.min() and logp.max() < -16
+    reference = (logp + 0.4).astype(np.float32)
+    d = reference.astype(np.float64) - logp
+    want = np.expm1(d) - d
+    bufs = [ko.DeviceBuffer.from_numpy(a) for a in (stored, labels, reference, np.zeros(rows, np.float32))]
+    loss, kl, grad = ko.DeviceBuffer(4 * rows), ko.DeviceBuffer(4 * rows), ko.DeviceBuffer(stored.nbytes)
+    n = ko.token_logprob_workspace_bytes(rows, cols)
+    ws = ko.DeviceBuffer(max(n, 16))
+    typed = {} if kind == "f32" else dict(dtype=ko.BF16)
+    op = ko.policy_loss if kind == "f32" else ko.policy_loss16
+    for gradient, work in ((True, False), (False, False), (True, True)):
+        op(bufs[0], bufs[1], bufs[3], loss, rows, cols, ref_logp=bufs[2], scale=scale, kl=kl, dlogits=grad if gradient else None,
+           workspace=ws if work and n else None, workspace_bytes=n if work else 0, **typed)
+        ko.synchronize()
+        off = kl.download(np.float32, (rows,)) - want
+        rms = np.sqrt((off ** 2).mean())
+        assert rms < 5e-8, (gradient, work, rms)

@@ -96,3 +96,42 @@ def test_walks_of_the_layernorm_gradient(ko, three_workgroups, rows, cols, kind)
                                        ("f32", 511)])
 def test_many_rows_of_two_vectors_per_lane(ko, kind, cols):
     token_loss.test_token_logprob_and_its_gradient(ko, 16391, cols, kind)
+
+
+def test_rows_behind_32_bit_offsets_against_64_bits(ko):
+    """66000 rows of 33000 bf16 columns: rows next to where 32-bit offsets in elements (65075.2 rows) and in bytes (32537.6) end, and the
+    last ones, against the formulas."""
+    rows, cols = 66000, 33000
+    size = rows * cols * 2
+    a, b, d = ko.DeviceBuffer(size), ko.DeviceBuffer(size), ko.DeviceBuffer(size)
+    ko.fill_uniform_16(a, rows * cols, 84, dtype=ko.BF16)
+    ko.fill_uniform_16(b, rows * cols, 85, dtype=ko.BF16)
+    rng = np.random.default_rng(86)
+    some = np.array([0, 32537, 32538, 65074, 65075, 65076, 65999])
+    labels = rng.integers(0, cols, rows).astype(np.int32)
+    f = {k: rng.uniform(*v, rows).astype(np.float32) for k, v in dict(mean=(-.1, .1), rstd=(.5, 2), dlogp=(.5, 1), adv=(-1, 1)).items()}
+    dev = {k: ko.DeviceBuffer.from_numpy(v) for k, v in f.items()}
+    dl, logp, stats, loss = ko.DeviceBuffer.from_numpy(labels), *(ko.DeviceBuffer(n * rows) for n in (4, 8, 4))
+
+    def fetch(buf):
+        return np.stack([ref.to_float(buf.download(np.uint16, (cols,), int(r) * cols * 2), "bf16") for r in some])
+
+    def check(value, off, name):
+        ref.assert_within(fetch(d), value, off + ref.rounded("bf16", value) * (1 + 1e-6), name)
+
+    x, y = fetch(a), fetch(b)
+    typed = dict(dtype=ko.BF16)
+    ko.layernorm_backward16(a, b, dev["mean"], dev["rstd"], d, rows, cols, **typed)
+    (value, _, _), (off, _, _) = ref.layernorm_backward(x, y, f["mean"][some].astype(np.float64), f["rstd"][some].astype(np.float64))
+    check(value, off, "LayerNorm")
+    ko.softmax_backward16(a, b, d, rows, cols, **typed)
+    check(*ref.softmax_backward(x, y), "softmax")
+    ko.token_logprob16(a, dl, logp, rows, cols, row_stats=stats, **typed)
+    ko.token_logprob_backward16(a, dl, stats, dev["dlogp"], d, rows, cols, **typed)
+    s = ref.Scores(x, labels[some])
+    ref.assert_within(logp.download(np.float32, (rows,))[some], s.logp, s.logp_off, "logp")
+    check(*s.gradient(f["dlogp"][some].astype(np.float64), 0.0, s.logsum_off + 3 * ref.U * np.abs(s.logsum) + 2 * ref.U), "logp gradient")
+    ko.policy_loss16(a, dl, dev["adv"], loss, rows, cols, dlogits=d, **typed)
+    want = ref.policy(s, f["adv"][some].astype(np.float64))
+    ref.assert_within(loss.download(np.float32, (rows,))[some], *want["loss"], "loss")
+    check(*want["dlogits"], "policy gradient")
