@@ -909,8 +909,10 @@ __global__ __launch_bounds__(64) void policy_short_kernel(PolicyArgs<IO> a) {
 // Rows have columns for more than ABOVE vectors: only a thread's last ones can lie past the
 // row's end.  REST: rows longer than the registers.  What does not fit is added up before the registers fill, and read a second
 // time for its gradient.
+// Up to three vectors per thread 1024 threads have to leave room for a second workgroup, which the compiler has to be told: in 79
+// registers instead of 58 a compute unit held one of them (24576 bf16 columns 515 us, 344 with two).
 template <int IO, int ABOVE, int THREADS, int VPT, bool REST = false>
-__global__ __launch_bounds__(THREADS) void policy_onchip_kernel(PolicyArgs<IO> a) {
+__global__ __launch_bounds__(THREADS, THREADS == 1024 && VPT <= 3 ? 8 : 1) void policy_onchip_kernel(PolicyArgs<IO> a) {
     constexpr int E = Io<IO>::E;
     // (up to a 128-byte boundary a row loses less than eight of the vectors that its columns make: it has ABOVE - 7 at least)
     constexpr int WHOLE = ABOVE < 7 ? 0 : (ABOVE - 7) / THREADS;
