@@ -82,14 +82,23 @@ __device__ __forceinline__ int piece_begin(int n, int parts, int part) {
 struct Pair {
     float m, s;
 };
-// scale log2(e) in two parts: of one float it would be off by up to 2^-24 of itself, the same way in every exponential of a
-// row, which 100000 of them do not average out (1e-6 in a logp of -13).  lo is positive.
+// scale log2(e): as one float (all), off by up to 2^-24 of itself, the same way in every exponential of a row, which 100000 of them
+// do not average out (1e-6 in a logp of -13); and in two parts.  hi has 16 bits: the second part's products are then large enough
+// to count where they are added to rounded ones (next to a hi of 24 bits they are rounded away: logits around 20 gave a logp off by
+// 4e-7, in every row alike).  lo is positive.
 struct Scale {
-    float hi, lo;
+    float hi, lo, all;
 };
 // exp(scale d).  exp_sum: for sums; exp_scaled: where the result is rounded next.
-__device__ __forceinline__ float exp_sum(float d, Scale c) { return __builtin_amdgcn_exp2f(__builtin_fmaf(d, c.lo, d * c.hi)); }
-__device__ __forceinline__ float exp_scaled(float d, Scale c) { return __builtin_amdgcn_exp2f(d * c.hi); }
+__device__ __forceinline__ float exp_sum(float d, Scale c) { return __builtin_amdgcn_exp2f(__builtin_fmaf(d, c.hi, d * c.lo)); }
+__device__ __forceinline__ float exp_scaled(float d, Scale c) { return __builtin_amdgcn_exp2f(d * c.all); }
+// c times a label's logit, for sums relative to it: to a multiple of 2^-8.  With bfloat16's few numbers hi x - shift is then mostly exact;
+// if it were rounded, that would go by the last bits of shift, the same way in all of a row's columns.
+__device__ __forceinline__ float shift_of(float at_label, Scale c) { return __builtin_rintf(at_label * c.all * 256.0f) * 0.00390625f; }
+// 2^(c x - shift)
+__device__ __forceinline__ float power_of(float x, float shift, Scale c) {
+    return __builtin_amdgcn_exp2f(__builtin_fmaf(x, c.lo, __builtin_fmaf(x, c.hi, -shift)));
+}
 // An empty pair is (-FLT_MAX, 0).
 
 // Adds N values (absent ones: -inf) at once: the sum is rescaled at most once for all of them, and only where a lane of
@@ -153,12 +162,12 @@ __device__ __forceinline__ Total block_pair(Pair p, Total *slot, Scale c) {
 }
 
 // From a sum of 2^(c x_j - shift) to one of exp(scale (x_j - x_l)): shift is c x_l rounded, and what the rounding took is a factor
-// 2^-rest next to 1 as long as c x_l is below some millions.  Beyond that the powers summed here leave their range long before the
-// row's own do, and 1 + expm1 cancels: NaN, which callers take as they take a sum that is too large - they sum again, relative to the
-// maximum.
+// 2^-rest next to 1.  c x - shift is put together in two steps, the first of which is rounded at some 2^-15 of shift: within 2^-24 up to
+// a shift of 2^16.  Beyond that NaN, which callers take as they take a sum that is too large: they sum again, relative to the maximum.
+// (Far beyond, the powers here leave their range long before the row's own do.)
 __device__ __forceinline__ double to_label(double sum, float at_label, float shift, Scale c) {
+    if (!(fabsf(shift) <= 0x1p16f)) return __builtin_nan("");
     const float rest = __builtin_fmaf(at_label, c.lo, __builtin_fmaf(at_label, c.hi, -shift));
-    if (!(fabsf(rest) <= 0.5f)) return __builtin_nan("");
     return sum + sum * expm1f(-0.69314718f * rest);
 }
 
@@ -372,7 +381,7 @@ __device__ __forceinline__ void add_vector(const typename Io<IO>::raw &r, int j,
 #pragma unroll
     for (int e = 0; e < E; ++e) {
         top = fmaxf(top, x[e]);
-        s[e % 4] += __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], c.lo, __builtin_fmaf(x[e], c.hi, -shift)));
+        s[e % 4] += power_of(x[e], shift, c);
     }
 }
 // A thread's single elements.
@@ -383,7 +392,7 @@ __device__ __forceinline__ void add_singles(const typename Io<IO>::elem *src, co
         const int column = single_column(span, i);
         const float x = column == label ? -INFINITY : Io<IO>::scalar(src + column);
         top = fmaxf(top, x);
-        s[1] += __builtin_amdgcn_exp2f(__builtin_fmaf(x, c.lo, __builtin_fmaf(x, c.hi, -shift)));
+        s[1] += power_of(x, shift, c);
     }
 }
 // The score of a row from its label's logit, the sum relative to that and the row's maximum.
@@ -422,7 +431,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(6))) vo
         // vectors past the row's end read as zeros, without traffic
         const Buffer from = buffer_of(src + span.head, Io<IO>::kBytes * span.nvec);
         const float at_label = Io<IO>::scalar(src + label);
-        const float shift = at_label * a.c.hi;
+        const float shift = shift_of(at_label, a.c);
         const int in_vecs = label - span.head;
         const int label_vec = in_vecs >= 0 && in_vecs < span.nvec * E ? in_vecs / E : -1;
         float top = at_label;
@@ -519,7 +528,7 @@ __global__ __launch_bounds__(64) void token_logprob_short_kernel(ScoreArgs<IO> a
             const RowSpan<IO> span = span_of<IO>(src, a.cols);
             const int in_vecs = label - span.head;
             const float at_label = of(my_at, i);
-            const float shift = at_label * a.c.hi;
+            const float shift = shift_of(at_label, a.c);
             float top = at_label;
             float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -535,7 +544,7 @@ __global__ __launch_bounds__(64) void token_logprob_short_kernel(ScoreArgs<IO> a
                 my_top = top;
             }
         }
-        mine.s = to_label(mine.s, my_at, my_at * a.c.hi, a.c);
+        mine.s = to_label(mine.s, my_at, shift_of(my_at, a.c), a.c);
         // unlikely labels, special values: against the maximum, a row at a time
         uint64_t again = __ballot(reads && !(static_cast<float>(mine.s) < 0x1p40f));
         while (again) {
@@ -848,7 +857,7 @@ __global__ __launch_bounds__(64) void policy_short_kernel(PolicyArgs<IO> a) {
         const Elem *src = a.logits + (row0 + i) * a.ld;
         const RowSpan<IO> span = span_of<IO>(a.dlogits + (row0 + i) * a.ldd, a.cols);
         const int label = __builtin_amdgcn_readlane(my_label, i);
-        const float shift = of(my_at, i) * a.c.hi;
+        const float shift = shift_of(of(my_at, i), a.c);
         float top = 0.0f;
         float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         add_vector<IO>(r[i], lane, true, span.nvec, label - span.head, shift, a.c, s, top);
@@ -856,7 +865,7 @@ __global__ __launch_bounds__(64) void policy_short_kernel(PolicyArgs<IO> a) {
         const double sum = wave_total((s[0] + s[1]) + (s[2] + s[3]));
         if (lane == i) mine.s = sum;
     }
-    mine.s = to_label(mine.s, my_at, my_at * a.c.hi, a.c);
+    mine.s = to_label(mine.s, my_at, shift_of(my_at, a.c), a.c);
     uint64_t again = __ballot(reads && !(static_cast<float>(mine.s) < 0x1p40f));
     while (again) {
         const int i = __builtin_ctzll(again);
@@ -942,7 +951,7 @@ __global__ __launch_bounds__(THREADS, THREADS == 1024 && VPT <= 3 ? 8 : 1) void 
         return first + k * Io<IO>::kBytes * THREADS;
     };
     float at_label = label < a.cols ? Io<IO>::scalar(src + label) : 0.0f;
-    float shift = at_label * a.c.hi;
+    float shift = shift_of(at_label, a.c);
     float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     const int in_vecs = label - span.head;
     constexpr int BATCH = 8;  // vectors per thread at a time of the rest
@@ -964,7 +973,7 @@ __global__ __launch_bounds__(THREADS, THREADS == 1024 && VPT <= 3 ? 8 : 1) void 
                 rest_others(v[u], j + u * THREADS, x);
 #pragma unroll
                 for (int e = 0; e < E; ++e)
-                    s[e % 4] += __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], a.c.lo, __builtin_fmaf(x[e], a.c.hi, -shift)));
+                    s[e % 4] += power_of(x[e], shift, a.c);
             }
         }
     }
@@ -1009,11 +1018,11 @@ __global__ __launch_bounds__(THREADS, THREADS == 1024 && VPT <= 3 ? 8 : 1) void 
         others(k, x);
 #pragma unroll
         for (int e = 0; e < E; ++e)
-            s[e % 4] += __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], a.c.lo, __builtin_fmaf(x[e], a.c.hi, -shift)));
+            s[e % 4] += power_of(x[e], shift, a.c);
     }
 #pragma unroll
     for (int i = 0; i < SINGLES; ++i)
-        s[i % 4] += __builtin_amdgcn_exp2f(__builtin_fmaf(other_single(i), a.c.lo, __builtin_fmaf(other_single(i), a.c.hi, -shift)));
+        s[i % 4] += power_of(other_single(i), shift, a.c);
     double total = wave_total((s[0] + s[1]) + (s[2] + s[3]));
     if constexpr (THREADS > 64) {
         if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = total;
@@ -1061,7 +1070,7 @@ __global__ __launch_bounds__(THREADS, THREADS == 1024 && VPT <= 3 ? 8 : 1) void 
     if (g.top != at_label || !(fabsf(shift) < kMostShift)) {
         // the reference is the maximum; one that far from 0 is taken off the values (what is close enough to it to count is
         // so exactly, in the storage type too: two numbers of a type within a factor of two differ by one of its numbers)
-        shift = g.top * a.c.hi;
+        shift = g.top * a.c.all;
         if (!(fabsf(shift) < kMostShift)) {
 #pragma unroll
             for (int k = 0; k < VPT; ++k) {
@@ -1078,16 +1087,16 @@ __global__ __launch_bounds__(THREADS, THREADS == 1024 && VPT <= 3 ? 8 : 1) void 
             reference = shift = 0.0f;
         }
     }
-    // factor 2^(c x - shift); c.lo makes no difference to what is rounded here.  (A row that counts and has no gradient, factor
+    // factor 2^(c x - shift), c of one float: the result is rounded next.  (A row that counts and has no gradient, factor
     // 0, has finite powers: its products are 0.)
-    const float factor = g.a * __builtin_amdgcn_exp2f(-__builtin_fmaf(reference, a.c.hi, -shift));
+    const float factor = g.a * __builtin_amdgcn_exp2f(-__builtin_fmaf(reference, a.c.all, -shift));
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
         convert_again<IO>(r[k]);
         float x[E];
         Io<IO>::unpack(r[k], x);
 #pragma unroll
-        for (int e = 0; e < E; ++e) x[e] = factor * __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], a.c.hi, -shift));
+        for (int e = 0; e < E; ++e) x[e] = factor * __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], a.c.all, -shift));
         if (label_k == k) {
             const int j = static_cast<int>(threadIdx.x) + k * THREADS;
 #pragma unroll
@@ -1109,7 +1118,7 @@ __global__ __launch_bounds__(THREADS, THREADS == 1024 && VPT <= 3 ? 8 : 1) void 
 #pragma unroll
                 for (int e = 0; e < E; ++e)
                     x[e] = E * at + e == in_vecs ? g.label_grad
-                                                 : factor * __builtin_amdgcn_exp2f(__builtin_fmaf(x[e] - less, a.c.hi, -shift));
+                                                 : factor * __builtin_amdgcn_exp2f(__builtin_fmaf(x[e] - less, a.c.all, -shift));
                 buffer_store<IO>(to, Io<IO>::kBytes * static_cast<uint32_t>(at), x);
             }
         }
@@ -1119,7 +1128,7 @@ __global__ __launch_bounds__(THREADS, THREADS == 1024 && VPT <= 3 ? 8 : 1) void 
         if (has_single[i]) {
             constexpr int ONE = io_by_element(IO);
             const float x[1] = {column[i] == label ? g.label_grad
-                                                   : factor * __builtin_amdgcn_exp2f(__builtin_fmaf(single[i], a.c.hi, -shift))};
+                                                   : factor * __builtin_amdgcn_exp2f(__builtin_fmaf(single[i], a.c.all, -shift))};
             Io<ONE>::template store<true>(dst + column[i], x);
         }
     }
@@ -1415,11 +1424,12 @@ size_t workspace_bytes(int64_t rows, int64_t cols) {
 
 Scale two_parts(float scale) {
     const double c = static_cast<double>(scale) * 1.4426950408889634;
-    float hi = static_cast<float>(c);
-    if (hi > c) hi = nextafterf(hi, 0.0f);
+    int exponent;
+    const double fraction = frexp(c, &exponent);
+    const float hi = static_cast<float>(ldexp(floor(ldexp(fraction, 16)), exponent - 16));
     // (lo > 0: -inf times either part is -inf)
     const float lo = static_cast<float>(c - hi);
-    return Scale{hi, lo > 1e-37f ? lo : 1e-37f};
+    return Scale{hi, lo > 1e-37f ? lo : 1e-37f, static_cast<float>(c)};
 }
 
 // What every entry on rows of logits checks.
