@@ -251,17 +251,26 @@ __device__ __forceinline__ double log_in_parts(double t) {
     p = __builtin_fma(w, p, 1.0);
     return __builtin_fma(static_cast<double>(k), 0.69314718055994531, 2.0 * u * p);
 }
+// exp(scale (x - top)), x <= top: what a row's whole sum is multiplied by.  The argument in base 2 has more than 32 bits, of which the
+// hardware takes 32; the others are worked in to first order.  (Rounded to 32 bits at -30 it put 4e-7 on all of a sum.)
+__device__ __forceinline__ double exp_below(float x, float top, Scale c) {
+    const double a = (static_cast<double>(x) - static_cast<double>(top)) * (static_cast<double>(c.hi) + static_cast<double>(c.lo));
+    if (a < -150.0) return 0.0;
+    const float rounded = static_cast<float>(a);
+    const double e = __builtin_amdgcn_exp2f(rounded);
+    return __builtin_fma(e, 0.69314718 * (a - rounded), e);
+}
 // From the pair of the other columns and the label's logit.
 __device__ __forceinline__ RowScore score_row(Total p, float at_label, float scale, Scale c) {
     RowScore r;
     r.top = fmaxf(p.m, at_label);
-    const double s = p.s * exp_sum(p.m - r.top, c);
+    const double s = p.s * exp_below(p.m, r.top, c);
     const double z = (static_cast<double>(at_label) - static_cast<double>(r.top)) * static_cast<double>(scale);
-    const float e = expf(static_cast<float>(z));
+    const double e = exp_below(at_label, r.top, c);
     const double total = s + e;
     if (s <= e) {  // a likely label: relative to a logarithm close to 0
         // (e is 1 here: no other column reaches the label's; or 0, in a row of nothing but -inf: NaN)
-        r.logp = !(e > 0.0f) ? __builtin_nan("") : s < 0.03125 ? -log1pf(static_cast<float>(s)) : -log_in_parts(1.0 + s);
+        r.logp = !(e > 0.0) ? __builtin_nan("") : s < 0.03125 ? -log1pf(static_cast<float>(s)) : -log_in_parts(1.0 + s);
         r.logsum = z - r.logp;
     } else {
         r.logsum = log_in_parts(total);

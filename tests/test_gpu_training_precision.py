@@ -85,3 +85,40 @@ def test_log_probabilities_are_differences_of_more_than_32_bits(ko, cols, kind, 
         off = kl.download(np.float32, (rows,)) - want
         rms = np.sqrt((off ** 2).mean())
         assert rms < 4e-8 + (0.0 if kind == "f32" or level == 0.0 else 2 * (3.2e-8 if level == 20.0 else 4.5e-8)), (gradient, work, rms)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("cols", [1001, 9001, 70001])
+def test_all_but_certain_labels(ko, cols, kind):
+    """A label 20 to 30 above the others: logp is minus their sum, relative to the label.  From the sum relative to the largest of the
+    others that is one factor of exp(-16 to -26), whose argument in 32 bits would put 3.8e-7 in root mean square on all of logp (half
+    a step of numbers from 16 to 64 in base 2, 9.5e-7 or more).  What may be off: logp's own rounding and that of its series 3e-8
+    each in root mean square, a hardware exponential 3e-8, the sum 2e-8 (bf16: the arguments of some hundred different logits, 0 to 8
+    below the maximum, 1.4e-7 by the square root of fifty): below 7e-8 together."""
+    rows = 60
+    rng = np.random.default_rng(cols + 7)
+    x = rng.normal(0.0, 1.0, (rows, cols)).astype(np.float32)
+    labels = rng.integers(0, cols, rows).astype(np.int32)
+    at = np.arange(rows)
+    x[at, labels] = rng.uniform(20.0, 30.0, rows)
+    stored, values = ref.to_storage(x, kind)
+    others = np.exp(values - values[at, labels][:, None])
+    others[at, labels] = 0.0
+    want = -np.log1p(others.sum(1))
+    bufs = [ko.DeviceBuffer.from_numpy(a) for a in (stored, labels, np.zeros(rows, np.float32))]
+    logp, loss, grad = ko.DeviceBuffer(4 * rows), ko.DeviceBuffer(4 * rows), ko.DeviceBuffer(rows * (cols + 1) * 4)
+    n = ko.token_logprob_workspace_bytes(rows, cols)
+    ws = ko.DeviceBuffer(max(n, 16))
+    typed = {} if kind == "f32" else dict(dtype=ko.BF16)
+    score, policy = (ko.token_logprob, ko.policy_loss) if kind == "f32" else (ko.token_logprob16, ko.policy_loss16)
+    forms = dict(score=lambda w: score(bufs[0], bufs[1], logp, rows, cols, **w, **typed),
+                 policy=lambda w: policy(bufs[0], bufs[1], bufs[2], loss, rows, cols, logp=logp, dlogits=grad, **w, **typed),
+                 alone=lambda w: policy(bufs[0], bufs[1], bufs[2], loss, rows, cols, logp=logp, **w, **typed),
+                 apart=lambda w: policy(bufs[0], bufs[1], bufs[2], loss, rows, cols, logp=logp, dlogits=grad, ldd=cols + 1, **w, **typed))
+    for name, run in forms.items():
+        for w in ({}, dict(workspace=ws, workspace_bytes=n)):
+            run(w)
+            ko.synchronize()
+            off = logp.download(np.float32, (rows,)) / want - 1.0
+            rms = np.sqrt((off ** 2).mean())
+            assert rms < 1e-7, (name, bool(w), rms)
