@@ -764,9 +764,11 @@ __device__ __forceinline__ void put_policy(const PolicyArgs<IO> &a, int64_t row,
 }
 __device__ __forceinline__ PolicyResult no_policy() { return PolicyResult{0.0f, 0.0f, 0.0f, RowGradient{0.0f, 0.0f, 0.0f, false}}; }
 
-// One workgroup per row, any length and alignment: the sums, then a second read.
+// One workgroup per row, any length and alignment: the sums, then a second read.  (Six wavefronts per SIMD as in
+// token_logprob_row_kernel: 32768 rows of 8192 bf16 columns without a
+// gradient 300 us with five, 230 with six.)
 template <int IO, int THREADS>
-__global__ __launch_bounds__(THREADS) void policy_reread_kernel(PolicyArgs<IO> a) {
+__global__ __launch_bounds__(THREADS, THREADS < 1024 ? 6 : 1) void policy_reread_kernel(PolicyArgs<IO> a) {
     __shared__ Total slots[2][THREADS / 64];
     __shared__ RowGradient shared[2];
     int turn = 1;  // (alternates between the rows that count: others pass no barrier)
