@@ -199,12 +199,14 @@ int ko_layernorm_backward_16(const void *dy, const void *in, const float *mean, 
  * logits: [rows] rows of cols elements, ld >= cols elements from one row to the next (what lies between is never read
  * or, in dlogits with its ldd, written).  cols up to 2^28; any cols, ld and element-aligned address run on 16-byte vectors; a
  * dlogits whose rows lie differently in their 16-byte vectors than the logits' rows is walked element by element.  How a row's
- * sum is split depends on its length, on where it starts in a 128-byte line and, from 65537 columns on with a workspace and in
- * the policy loss up to 512 (fp32: 256) columns, on the number of rows; on nothing else.
+ * sum is split depends on its length, on where it starts in a 128-byte line (with a gradient: where the gradient's row does) and, from
+ * 65537 columns on with a workspace and up to 519 columns (fp32: 259) in the policy loss, on the number of rows; on nothing else.
  * labels: device int32[rows].  A negative label marks a row that takes no part (a prompt's, padding): its logits are
  * never read, its outputs and its gradient are 0.  A label >= cols reads nothing out of place and makes the row's
- * outputs and its gradient NaN.  scale multiplies the logits (1 / temperature), from 1e-20 to 1e20.
+ * outputs and its gradient NaN, whatever its advantage.  scale multiplies the logits (1 / temperature), from 1e-20 to 1e20.
  * Special values: a NaN or +inf among a row's logits makes its outputs NaN; -inf elements have probability 0.
+ * Log-probabilities are worked out to some 1e-8 and rounded to fp32 where they are stored: a KL term sees the former; the gradient of
+ * token_logprob takes a log sum in fp32 (whose rounding is up to 5e-7 of every entry), rewards are sums of fp32 differences.
  * One workspace size serves all of them (see above). */
 size_t ko_token_logprob_workspace_bytes(int64_t rows, int64_t cols);
 
@@ -215,7 +217,7 @@ int ko_token_logprob_f32(const float *logits, int64_t ld, const int32_t *labels,
 int ko_token_logprob_16(const void *logits, int64_t ld, const int32_t *labels, float scale, float *logp, float *row_stats,
                         int64_t rows, int64_t cols, int dtype, void *workspace, size_t workspace_bytes, ko_stream_t stream);
 /* dlogits = dlogp scale (onehot(label) - softmax(scale logits)).  dlogits may be logits (with ldd = ld).  A row whose dlogp
- * is 0 gets zeros, its logits unread. */
+ * is 0 gets zeros, its logits unread and whatever its label. */
 int ko_token_logprob_backward_f32(const float *logits, int64_t ld, const int32_t *labels, float scale, const float *row_stats,
                                   const float *dlogp, float *dlogits, int64_t ldd, int64_t rows, int64_t cols,
                                   ko_stream_t stream);
@@ -229,7 +231,7 @@ int ko_token_logprob_backward_16(const void *logits, int64_t ld, const int32_t *
  *      kl = exp(d) - 1 - d,  d = ref_logp - logp,  loss = weight (-s + kl_coef kl),
  * loss_sum = sum_r loss[r] (NULL if not wanted), dlogits = d loss_sum / d logits (NULL if not wanted; may be logits with
  * ldd = ld).  At a border of the clip range the gradient is the unclipped side's.  old_logp NULL: ratio 1, the policy
- * that sampled is the one that trains.  ref_logp NULL: no KL term.  weight NULL: 1; a row whose weight is 0 is treated as one without a label.  logp, kl (unweighted): [rows],
+ * that sampled is the one that trains (for a label at -inf, too).  ref_logp NULL: no KL term.  weight NULL: 1; a row whose weight is 0 is treated as one without a label.  logp, kl (unweighted): [rows],
  * NULL if not wanted; loss: [rows].  clip_low in [0, 1], clip_high >= 0. */
 int ko_policy_loss_f32(const float *logits, int64_t ld, const int32_t *labels, const float *old_logp, const float *ref_logp,
                        const float *advantage, const float *weight, float scale, float clip_low, float clip_high, float kl_coef,

@@ -380,7 +380,8 @@ __global__ __launch_bounds__(group_threads<LPR>(), LPR == 1024 ? 4 : LPR <= 64 &
     }
 }
 
-// ---- rows of any length: the sums first, then a second read; no share of dgamma and dbeta (the column kernel's)
+// ---- rows of any length: the sums first, then a second read; no share of dgamma and dbeta (the column kernel's): dy and x are
+// read three times where those are wanted (1 GiB of bf16 rows of 20000 columns 1137 us, 2.8 TB/s of dy, x and dx; 40000 columns 1230)
 template <int IO, int THREADS, bool RAGGED>
 __global__ __launch_bounds__(THREADS) void layernorm_backward_reread_kernel(Args<IO> a) {
     constexpr int E = Io<IO>::E;
@@ -447,7 +448,8 @@ __global__ __launch_bounds__(THREADS) void layernorm_backward_reread_kernel(Args
     }
 }
 
-// ---- dgamma and dbeta alone: workgroup (strip, split) takes 64 columns and every gridDim.y-th group of rows
+// ---- dgamma and dbeta alone: workgroup (strip, split) takes 64 columns and every gridDim.y-th group of rows.  Without
+// a workspace there is one split, and a few workgroups read everything (16384 x 768 bf16 0.57 ms; with one 17 us in all).
 template <int IO>
 __global__ __launch_bounds__(256) void layernorm_backward_columns_kernel(Args<IO> a) {
     float sg, sb;

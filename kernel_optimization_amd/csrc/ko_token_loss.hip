@@ -14,8 +14,11 @@
 // 50272 bf16 columns, their odd ones 64 bytes into a line: gradient 383 us with vectors from 64-byte boundaries on).  So a
 // vocabulary of 50257 contiguous columns runs on vectors, too.
 //
-// Bound: memory.  The sums are one pass with a running maximum; the policy loss keeps the whole row in a workgroup's
-// registers between the sum and the gradient, so that the logits are read once and the gradient written once.
+// Bound: memory.  The sums are one pass, relative to the label's logit and, where that is far below the others or far from 0, a second
+// one with a running maximum; in pieces of rows and in the policy loss without a gradient, one with a running maximum.  The policy
+// loss keeps the whole row in a workgroup's registers between the sum and the gradient, so that the logits are read once and the
+// gradient written once.  Gradients of rows that lie differently in the two matrices go element by element, in the policy loss after
+// a second read (1 GiB of 50257 bf16 columns into rows of 50264: 962 us instead of 349, policy loss 2310 instead of 365).
 #include "ko_internal.h"
 
 #include "row_reduce.h"
@@ -417,10 +420,9 @@ __device__ __forceinline__ RowScore label_score(const A &a, Total p, float at_la
 // One workgroup per row, the next batch of U vectors per thread in flight while this one is added up.  As in
 // policy_onchip_kernel the exponentials are taken against the label's logit, and the row's maximum is noted by the way; a label
 // so unlikely that the sum reaches 2^40, or a sum that is not a number, is summed again with a running maximum.  Bound: memory
-// (1 GiB of bf16 logits: 128256 columns 160 us, 6.7 TB/s, 50257 columns 153 us, 7.0 TB/s, 4096 columns 206 us; the
+// (1 GiB of bf16 logits: 128256 columns 161 us, 6.7 TB/s, 50257 columns 154 us, 7.0 TB/s, 8192 columns 197 us, 4096 columns 200; the
 // arithmetic close behind: nine instructions' time per value; six wavefronts per SIMD, which the compiler has to be told: with five
-// 8192 columns took 216 us, with six 195).  A running maximum without loads ahead took 164 us at 32000
-// columns and 329 at 8192.
+// 8192 columns took 216 us when six took 195).  A running maximum without loads ahead took 329 us at 8192 columns.
 template <int IO, int THREADS, int U>
 __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(6))) void token_logprob_row_kernel(ScoreArgs<IO> a) {
     constexpr int E = Io<IO>::E;
@@ -498,8 +500,8 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(6))) vo
 }
 
 // Many short rows, of U 64 vectors at most: a wavefront takes kShortRows of them, and the arithmetic of a row's score - several times
-// that of its sum, in one lane - is done for all of them at once, a row per lane (1 GiB of bf16 rows: 512 columns 242 us, 1024
-// columns 201; when tried, eight rows 227 and 197, a row per wavefront 471 and 281, four rows 252 and 206, sixteen 238 and, for
+// that of its sum, in one lane - is done for all of them at once, a row per lane (1 GiB of bf16 rows: 512 columns 234 us, 1024
+// columns 192; when tried, eight rows 227 and 197, a row per wavefront 471 and 281, four rows 252 and 206, sixteen 238 and, for
 // want of registers, 257).
 constexpr int kShortRows = 8;
 // Fewer rows are better off with a wavefront each: eight rows in turn take 2 to 4 us longer than one (64 rows of 512 bf16
@@ -836,8 +838,8 @@ __global__ __launch_bounds__(THREADS) void policy_pieces_kernel(PolicyArgs<IO> a
 }
 
 // Many short rows, of 64 vectors at most, as in token_logprob_short_kernel: the rows stay in the registers of a wavefront, the losses
-// are worked out a row per lane, and each row's gradient follows (1 GiB of bf16 logits in rows of 512 columns 390 us, 5.5 TB/s; a
-// wavefront per row 545).
+// are worked out a row per lane, and each row's gradient follows (1 GiB of bf16 logits in rows of 512 columns 399 us, 5.4 TB/s, and
+// 443 with loss_sum, whose launch follows the million rows; a wavefront per row 545 without it).
 template <int IO>
 __global__ __launch_bounds__(64) void policy_short_kernel(PolicyArgs<IO> a) {
     constexpr int E = Io<IO>::E;
@@ -1147,7 +1149,7 @@ __global__ __launch_bounds__(THREADS, THREADS == 1024 && VPT <= 3 ? 8 : 1) void 
 
 // ------------------------------------------------------------------------------------------------------- sums
 // out[0] = factor * sum of n values, in 64 bits and in a fixed order: one workgroup, with sixteen loads per thread in flight
-// (a row's logits take longer than its loss here).
+// (a million values 44 us, behind 399 us of kernels over their rows of 512 bf16 columns).
 __global__ __launch_bounds__(1024) void loss_sum_kernel(const float *__restrict__ values, int64_t n, float factor, float *out) {
     __shared__ double sums[16];
     double s = 0.0;
@@ -1371,8 +1373,10 @@ __global__ __launch_bounds__(kPreferenceThreads) void preference_kernel(Preferen
 }
 
 // Few pairs of few tokens: all of them in one workgroup, 16 / SIDE wavefronts per pair, and the sum of their losses with them -
-// one launch instead of two (2 pairs of 2 x 40 tokens 4.5 us instead of 7.0, 8 pairs of 2 x 512 6.3 and 7.1; 8 pairs of 2 x 1000
-// 9.5 against 7.6).
+// one launch instead of two (called over and over on data in the caches: 2 pairs of 2 x 40 tokens 4.5 us instead of 7.0, 8 pairs of
+// 2 x 512 6.3 and 7.1; 8 pairs of 2 x 1000 9.5 against 7.6).  Behind a kernel over logits, with nothing in the caches, 8 pairs of
+// 2 x 128 to 2 x 512 tokens take 10.5 to 11.6 us: 5 to 8 pairs have one wavefront each, half of the workgroup, and wait for their labels
+// before they ask for the rest.
 constexpr int kFewPairs = 16;
 constexpr int64_t kFewTokens = 8192;
 template <int SIDE>
@@ -1510,9 +1514,9 @@ int logprob_entry(const void *logits, int64_t ld, const int32_t *labels, float s
     }
     const dim3 grid = row_grid(rows, 1024);
     const int nvec = a.cols / Io<IO>::E;
-    // rows of few vectors: as many threads as make one batch of them (8192 bf16 columns 187 us for 1 GiB, 208 with 512 threads and
-    // 4096 columns 190 against 383 with 256, half of them idle).  Long rows: 1024 threads took 258 us for 1 GiB of rows of
-    // 50257 bf16 columns, 512 take 152, and 32 such rows 6.7 against 7.2.
+    // rows of few vectors: as many threads as make one batch of them (when tried, 1 GiB of bf16 rows: 8192 columns 187 us, 208 with
+    // 512 threads; 4096 columns 190, 383 with 256 threads, half of them idle).  Long rows: 1024 threads took 258 us for 1 GiB of rows of
+    // 50257 bf16 columns, 512 take 154, and 32 such rows 6.7 against 7.2.
     if (nvec <= 128 && rows >= kManyRows) {
         const dim3 g = row_grid((rows + kShortRows - 1) / kShortRows, 64);
         if (nvec <= 64) token_logprob_short_kernel<IO, 1><<<g, dim3(64), 0, a.stream>>>(a);
@@ -1607,7 +1611,8 @@ int launch_policy(const PolicyArgs<IO> &a, void *workspace) {
             // Four vectors per thread, where the rows fit a workgroup that way: 4096 bf16 columns 338 us for 1 GiB of logits
             // against 356 with eight and 372 with two per thread, 1024 columns 393 against 675 with one.  Long rows: 512 threads
             // (two workgroups per compute unit, one of which loads or stores) as far as their registers go, 49152 columns
-            // 369 us against 412 with 1024 threads; three per thread where that is the number (24576 columns, 349 against 370).
+            // 369 us against 412 with 1024 threads; three per thread where that is the number (24576 columns 344,
+            // with 512 threads and eight 352; 16400 columns 451 and 433).
             if (nvec <= 64 && a.rows >= 2 * kManyRows) return launch_short<IO>(a);
             if (nvec <= 64) return launch_onchip<IO, 0, 64, 1>(a);
             if (nvec <= 128) return launch_onchip<IO, 64, 64, 2>(a);
@@ -1628,7 +1633,8 @@ int launch_policy(const PolicyArgs<IO> &a, void *workspace) {
             return launch_onchip<IO, 16 * 1024, 1024, 15, true>(a);
         }
     }
-    // no gradient, rows that lie differently in the two matrices, a row or two's vectors, and rows longer than the registers
+    // no gradient (1 GiB of bf16 logits: 512 columns 2.6 ms, 8192 columns 442 us, 50257 columns 318), and rows that lie differently in
+    // the two matrices
     const dim3 grid = row_grid(a.rows, 1024);
     if (a.cols <= 4096) policy_reread_kernel<IO, 256><<<grid, dim3(256), 0, a.stream>>>(a);
     else if (a.cols <= 32768) policy_reread_kernel<IO, 512><<<grid, dim3(512), 0, a.stream>>>(a);

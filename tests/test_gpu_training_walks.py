@@ -135,3 +135,26 @@ def test_rows_behind_32_bit_offsets_against_64_bits(ko):
     want = ref.policy(s, f["adv"][some].astype(np.float64))
     ref.assert_within(loss.download(np.float32, (rows,))[some], *want["loss"], "loss")
     check(*want["dlogits"], "policy gradient")
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("per_row", [9, 64, 65, 127, 128, 129])
+def test_the_number_of_rows_does_not_matter(ko, per_row, kind):
+    """Many rows go eight to a wavefront up to 128 vectors, in the policy loss up to 64: log-probabilities have the bits of a few rows'
+    call, the policy loss beyond 64 vectors, too."""
+    many, few, cols = 33003, 200, per_row * (4 if kind == "f32" else 8) + 1
+    call = Call(ko, few, cols, kind, 5300 + cols, 7 if kind == "f32" else 15)     # (rows of whole vectors, started anywhere)
+    case = policy_case(call, 5)
+    alone, scored = call.logprob(), run_policy(call, case, 7)
+    rows = np.concatenate([np.arange(few), np.random.default_rng(5).integers(0, few, many - few)])
+    call.rows, call.stored, call.labels = many, call.stored[rows], call.labels[rows]
+    call.keep, call.logits = ko.DeviceBuffer.from_numpy(call.stored), None
+    call.logits = call.keep.ptr
+    call.d_labels = ko.DeviceBuffer.from_numpy(call.labels)
+    case = {k: None if v is None else v[rows] for k, v in case.items()}
+    for got, want in zip(call.logprob(), alone):
+        np.testing.assert_array_equal(got[:few], want)
+    if cols // (4 if kind == "f32" else 8) > 64:
+        got = run_policy(call, case, 7)
+        for name in ("logp", "kl", "loss", "dlogits"):
+            np.testing.assert_array_equal(got[name][:few], scored[name], err_msg=name)
