@@ -767,8 +767,7 @@ __device__ __forceinline__ void put_policy(const PolicyArgs<IO> &a, int64_t row,
 __device__ __forceinline__ PolicyResult no_policy() { return PolicyResult{0.0f, 0.0f, 0.0f, RowGradient{0.0f, 0.0f, 0.0f, false}}; }
 
 // One workgroup per row, any length and alignment: the sums, then a second read.  (Six wavefronts per SIMD as in
-// token_logprob_row_kernel: 32768 rows of 8192 bf16 columns without a
-// gradient 300 us with five, 230 with six.)
+// token_logprob_row_kernel: 32768 rows of 8192 bf16 columns without a gradient 300 us with five, 230 with six.)
 template <int IO, int THREADS>
 __global__ __launch_bounds__(THREADS, THREADS < 1024 ? 6 : 1) void policy_reread_kernel(PolicyArgs<IO> a) {
     __shared__ Total slots[2][THREADS / 64];
@@ -1077,8 +1076,8 @@ __global__ __launch_bounds__(THREADS, THREADS == 1024 && VPT <= 3 ? 8 : 1) void 
     __syncthreads();
     const RowGradient g = uniform_gradient(shared);
     float reference = g.top, less = 0.0f;
-    // shift is rounded, to half a step of itself: below 2^24 that makes both powers of the product below differ from what they stand
-    // for by a factor of 2 at most; beyond, one may be infinite and the other 0
+    // shift is rounded, in the end to half a step of itself: below 2^24 that makes both powers of the product below differ from what they
+    // stand for by a factor of 2 at most; beyond, one may be infinite and the other 0
     constexpr float kMostShift = 0x1p24f;
     if (g.top != at_label || !(fabsf(shift) < kMostShift)) {
         // the reference is the maximum; one that far from 0 is taken off the values (what is close enough to it to count is

@@ -14,7 +14,8 @@ class FarScores(ref.Scores):
     """Scores whose log-probabilities stay finite where the label's probability is below the smallest 64-bit number."""
 
     def __init__(self, logits, labels, scale=1.0, alive=None):
-        super().__init__(logits, labels, scale, alive)
+        with np.errstate(over="ignore"):
+            super().__init__(logits, labels, scale, alive)
         z = self.z[self.rows, self.at]
         with np.errstate(invalid="ignore"):
             far = z - np.log(np.exp(self.z).sum(1))

@@ -1,5 +1,7 @@
 """Forms of the training-side operators that only many rows reach: workgroups that walk over rows, here on grids cut to three of
 them, and eight rows of two vectors per lane to a wavefront."""
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -7,6 +9,7 @@ import test_gpu_token_loss as token_loss
 import training_reference as ref
 from kernel_optimization_amd import inputs
 from test_gpu_backward_rows import KINDS, _softmax, check_layernorm_backward, check_softmax_backward, layernorm_case
+from test_gpu_streams_and_graphs import _hip_runtime
 from test_gpu_token_loss import Call, policy_case, run_policy
 
 pytestmark = pytest.mark.gpu
@@ -158,3 +161,61 @@ def test_the_number_of_rows_does_not_matter(ko, per_row, kind):
         got = run_policy(call, case, 7)
         for name in ("logp", "kl", "loss", "dlogits"):
             np.testing.assert_array_equal(got[name][:few], scored[name], err_msg=name)
+
+
+def test_many_pairs_in_a_graph(ko):
+    """More pairs than one workgroup each looks through: the launch that prepares them passes its results through pair_loss, in every
+    replay anew, with eager calls of other sizes in between."""
+    hip = _hip_runtime()
+    rng = np.random.default_rng(54)
+    steps = []
+    for pairs in (1025, 1024, 5000):
+        offsets = np.concatenate([[0], np.cumsum(rng.integers(0, 9, 2 * pairs))])
+        offsets[rng.integers(1, 2 * pairs, pairs // 50)] -= 30                    # some lead into earlier pairs
+        tokens = int(offsets.max()) + 3
+        bufs = [ko.DeviceBuffer.from_numpy(v) for v in (rng.normal(-2, 1, tokens).astype(np.float32),
+                                                        rng.normal(-2, 1, tokens).astype(np.float32), offsets.astype(np.int32))]
+        outs = {k: (ko.DeviceBuffer(4 * n), n) for k, n in dict(pair_loss=pairs, dlogp=tokens, loss_sum=1).items()}
+        steps.append((pairs, tokens, bufs, outs))
+
+    def run(step, stream):
+        pairs, tokens, (logp, rf, offsets), outs = step
+        ko.preference_loss(logp, rf, offsets, pairs, tokens, outs["pair_loss"][0], dlogp=outs["dlogp"][0],
+                           loss_sum=outs["loss_sum"][0], stream=stream)
+
+    def clear():
+        for step in steps:
+            for buf, n in step[3].values():
+                buf.upload(np.full(n, np.nan, np.float32))
+
+    def results():
+        return [buf.download(np.uint32, (n,)) for step in steps for buf, n in step[3].values()]
+
+    clear()
+    for step in steps:
+        run(step, None)
+    ko.synchronize()
+    want = results()
+    stream, graph, graph_exec = ko.Stream(), ctypes.c_void_p(), ctypes.c_void_p()
+    assert hip.hipStreamBeginCapture(stream.handle, 0) == 0
+    try:
+        for step in steps[::2]:
+            run(step, stream)
+    finally:
+        rc = hip.hipStreamEndCapture(stream.handle, ctypes.byref(graph))
+    assert rc == 0 and graph.value
+    try:
+        assert hip.hipGraphInstantiate(ctypes.byref(graph_exec), graph, None, None, 0) == 0
+        for _ in range(4):
+            clear()
+            ko.synchronize()
+            assert hip.hipGraphLaunch(graph_exec, stream.handle) == 0
+            run(steps[1], None)
+            stream.synchronize()
+            ko.synchronize()
+            for got, expected in zip(results(), want):
+                np.testing.assert_array_equal(got, expected)
+    finally:
+        if graph_exec.value:
+            hip.hipGraphExecDestroy(graph_exec)
+        hip.hipGraphDestroy(graph)
